@@ -371,6 +371,131 @@ mgb_status mgb_embedding(int32_t format, const void *w, uint64_t stored_rows, ui
 mgb_status mgb_quantize_rows(const float *x, uint64_t len, int8_t *values, float *scales,
                              int32_t *sums, void *stream);
 
+/* ---- rows that choose: adapters, experts and sampled tokens -------------------------- */
+
+/* Operators in which every activation row of a batch picks what it meets: the
+ * low-rank adapter added to a shared projection, the experts of a mixture, the
+ * next token.  No counterparts on the reference's packed path.  Device
+ * pointers of the current device throughout; work is queued on `stream` and
+ * nothing is allocated, synchronised or kept between calls.  As in
+ * `mgb_embedding`, ids are f32 device values and `bad` (device u32, may be
+ * NULL) receives the position of the first invalid one, 0xFFFFFFFF when all
+ * are valid.  A call's workspace (16-byte aligned) is scratch: calls that may
+ * overlap on the GPU need one each, and its contents need no preparation. */
+
+/* `count` low-rank adapters of one projection of k inputs and n outputs.
+ * Adapter i adds scales[i] * (x A_i^T) B_i^T with A_i = a[i] ([rank, k]) and
+ * B_i = b[i] ([n, rank]), both of type `dtype`.  An adapter of lower rank is
+ * stored with zeros in its remaining rank rows of A and columns of B.  a and b
+ * are aligned to their element size; 16-byte aligned with k and rank whole
+ * 16-byte runs is the fast form. */
+#define MGB_MAX_ADAPTER_RANK 256
+typedef struct mgb_adapters {
+    const void *a;       /* [count, rank, k] */
+    const void *b;       /* [count, n, rank] */
+    const float *scales; /* [count], or NULL: 1 */
+    uint64_t count, rank, k, n;
+    int32_t dtype;       /* MGB_DTYPE_* of a and b */
+} mgb_adapters;
+/* Scratch bytes of mgb_adapters_add for m rows (0 for a descriptor it refuses). */
+uint64_t mgb_adapters_workspace_bytes(const mgb_adapters *adapters, uint64_t m);
+/* y[r] = base[r] + scales[a] * (x[r] A_a^T) B_a^T with a = ids[r], for the m
+ * rows of x [m, k]; y and base are [m, n], base may be y itself (added in
+ * place) or NULL (zeros).  A row whose id is negative (-1: no adapter) gets
+ * base[r] bit for bit, as does a row with an invalid id (not a whole number
+ * below count; reported in `bad`).  Rows with the same id read its adapter
+ * together.  f32 accuracy: products accumulate in f32 from operands of at
+ * least 22 bits.  Deterministic. */
+mgb_status mgb_adapters_add(const mgb_adapters *adapters, const float *ids, const float *x,
+                            uint64_t m, const float *base, float *y, uint32_t *bad,
+                            void *workspace, uint64_t workspace_bytes, void *stream);
+/* mgb_qmatmul and then mgb_adapters_add on its y: the shared packed projection
+ * with every row's adapter beside it.  adapters->k and ->n equal k and n.  A
+ * row without an adapter equals mgb_qmatmul's bit for bit.  The workspace
+ * serves both in turn (mgb_qmatmul_adapters_workspace_bytes). */
+uint64_t mgb_qmatmul_adapters_workspace_bytes(int32_t format, uint64_t m, uint64_t n, uint64_t k,
+                                              const mgb_adapters *adapters);
+mgb_status mgb_qmatmul_adapters(int32_t format, const void *w, uint64_t n, uint64_t k,
+                                const float *x, uint64_t m, float *y, const float *addend,
+                                uint64_t addend_len, const mgb_adapters *adapters,
+                                const float *ids, uint32_t *bad, void *workspace,
+                                uint64_t workspace_bytes, void *stream);
+
+/* The packed experts of one mixture-of-experts layer (device layout, 16-byte
+ * aligned): gate and up of `gate_up_format`, stored rows [experts * ffn,
+ * hidden]; down of `down_format`, stored rows [experts * hidden, ffn], expert
+ * after expert (the stacked order of a checkpoint, so one mgb_repack per
+ * tensor).  hidden and ffn are whole blocks of their formats. */
+#define MGB_MOE_MAX_TOKENS 256
+#define MGB_MOE_MAX_EXPERTS 1024
+#define MGB_MOE_MAX_TOP_K 32
+typedef struct mgb_experts {
+    const void *gate;
+    const void *up;
+    const void *down;
+    uint64_t experts, hidden, ffn;
+    int32_t gate_up_format, down_format;
+} mgb_experts;
+/* Scratch bytes of mgb_moe_layer and mgb_moe_experts for m tokens of top_k
+ * experts each (0 for arguments they refuse), and of mgb_moe_route. */
+uint64_t mgb_moe_workspace_bytes(const mgb_experts *experts, uint64_t m, uint64_t top_k);
+uint64_t mgb_moe_route_workspace_bytes(uint64_t experts, uint64_t hidden, uint64_t m);
+/* Routing: z = x [m, hidden] * router^T (router f32 [experts, hidden]), then
+ * each token's top_k experts by z descending (equal z: the lower id first) in
+ * ids [m, top_k] and their weights in weights [m, top_k]: the softmax of z
+ * over all experts, or over the chosen ones when normalize != 0, times
+ * `scale`.  z is summed so exactly (f32 products, f64 sums) that a choice
+ * differs from the real numbers' only where they nearly tie.  A NaN z sorts
+ * last. */
+mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden, const float *x,
+                         uint64_t m, uint64_t top_k, int32_t normalize, float scale, float *ids,
+                         float *weights, void *workspace, uint64_t workspace_bytes, void *stream);
+/* y[t] = addend[t] + sum_j weights[t, j] * down_e(silu(gate_e x[t]) * up_e x[t])
+ * with e = ids[t, j], for the m <= MGB_MOE_MAX_TOKENS tokens of x [m, hidden];
+ * addend [m, hidden] may be NULL (zeros) or y.  A slot whose id is negative is
+ * unused, as is one with an invalid id (reported in `bad`).  The same id twice
+ * counts twice.  Each chosen expert's packed rows are read once for all its
+ * tokens; f32 accuracy (f32 accumulation, operands of at least 22 bits);
+ * deterministic. */
+mgb_status mgb_moe_experts(const mgb_experts *experts, const float *x, uint64_t m,
+                           const float *ids, const float *weights, uint64_t top_k,
+                           const float *addend, float *y, uint32_t *bad, void *workspace,
+                           uint64_t workspace_bytes, void *stream);
+/* The whole layer: mgb_moe_route, then mgb_moe_experts on its ids and weights
+ * (ids and weights are outputs, [m, top_k], and may be NULL). */
+mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const float *x,
+                         uint64_t m, uint64_t top_k, int32_t normalize, float scale,
+                         const float *addend, float *y, float *ids, float *weights,
+                         void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* One token per row of logits [rows, vocab] (row stride ld >= vocab values).
+ * Row parameters, f32 device arrays of `rows` values (NULL: the neutral value):
+ *   temperature  p ~ exp(logit / temperature); <= 0 or NaN: greedy (neutral: 1)
+ *   top_k        keeps the first top_k tokens; < 1 or NaN: all (neutral: 0)
+ *   top_p        keeps the shortest prefix whose share of the probability left
+ *                by top_k is at least top_p; >= 1 or NaN: all (neutral: 1)
+ *   min_p        keeps tokens with p >= min_p * the largest p; <= 0 or NaN: all
+ *                (neutral: 0)
+ *   uniform      the row's random number in [0, 1) (clamped to it; NaN: 0);
+ *                NULL: every row greedy
+ * "First" and "prefix" are in order of logit, highest first, equal logits by
+ * token index; the most likely token is always kept.  The token drawn is the
+ * first one, in index order, at which the running sum of the kept tokens'
+ * probabilities exceeds uniform * their total; greedy: the lowest index of the
+ * largest logit.  Logits of -inf or NaN are masked and never drawn; +inf logits
+ * share all probability equally.  Outputs (each may be NULL): ids [rows], the
+ * token as f32 (what mgb_embedding reads; vocab <= MGB_SAMPLE_MAX_VOCAB keeps
+ * it exact), -1 for a row with nothing left; logprob [rows], the natural
+ * logarithm of its probability among the kept tokens (-inf with nothing left);
+ * kept [rows], how many tokens were kept (u32).  Probabilities are held as
+ * 64-bit fixed-point numbers, so sums do not depend on their order. */
+#define MGB_SAMPLE_MAX_VOCAB (1u << 20)
+uint64_t mgb_sample_workspace_bytes(uint64_t rows, uint64_t vocab);
+mgb_status mgb_sample(const float *logits, uint64_t rows, uint64_t vocab, uint64_t ld,
+                      const float *temperature, const float *top_k, const float *top_p,
+                      const float *min_p, const float *uniform, float *ids, float *logprob,
+                      uint32_t *kept, void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* ---- tensor parallelism over output columns (one process per GPU) ------------------ */
 
 /* Rank g of G holds stored rows [g n/G, (g+1) n/G) of a packed weight, the

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/magnetar_b200.h"
 #include "outspec.h"
 
 namespace mgb {
@@ -60,6 +61,34 @@ cudaError_t launch_add(float *y, uint64_t len, const float *addend, uint64_t add
 cudaError_t launch_quantize_rows(const float *x, uint64_t len, int8_t *values, float *scales,
                                  int32_t *sums, cudaStream_t stream);
 cudaError_t launch_int8_rounded(const float *x, uint64_t len, float *out, cudaStream_t stream);
+
+// adapters.cu
+uint64_t adapters_scratch_bytes(const mgb_adapters &ad, uint64_t m);
+cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const float *x, uint64_t m,
+                            const float *base, float *y, uint32_t *bad, void *workspace,
+                            cudaStream_t stream);
+
+// experts.cu
+uint64_t moe_route_scratch_bytes(uint64_t experts, uint64_t hidden, uint64_t m);
+uint64_t moe_experts_scratch_bytes(const mgb_experts &ex, uint64_t m, uint64_t top_k);
+cudaError_t launch_moe_route(const float *router, uint64_t experts, uint64_t hidden,
+                             const float *x, uint64_t m, uint64_t top_k, int normalize,
+                             float scale, float *ids, float *weights, void *workspace,
+                             cudaStream_t stream);
+cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m, const float *ids,
+                               const float *weights, uint64_t top_k, const float *addend, float *y,
+                               uint32_t *bad, void *workspace, cudaStream_t stream);
+
+// sample.cu
+struct SampleArgs {
+  const float *logits;
+  uint64_t rows, vocab, ld;
+  const float *temperature, *top_k, *top_p, *min_p, *uniform;
+  float *ids, *logprob;
+  uint32_t *kept;
+};
+uint64_t sample_scratch_bytes(uint64_t rows, uint64_t vocab);
+cudaError_t launch_sample(const SampleArgs &a, void *workspace, cudaStream_t stream);
 
 int device_sms(int device);
 

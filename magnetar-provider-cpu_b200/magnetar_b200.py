@@ -32,6 +32,7 @@ FORMATS = {"q8_0": Q8_0, "q4_k": Q4_K, "q5_k": Q5_K, "q6_k": Q6_K, "iq4_nl": IQ4
 BLOCK = {Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210), IQ4_NL: (32, 18),
          Q4_0: (32, 18)}
 KERNEL_AUTO, KERNEL_GEMV, KERNEL_GEMM = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2  # MGB_DTYPE_*
 MAX_RANK = 8
 
 
@@ -97,10 +98,26 @@ class TpOut(ctypes.Structure):
                 ("wait_timeout_ms", ctypes.c_uint32)]
 
 
+class Adapters(ctypes.Structure):
+    """`mgb_adapters`: the low-rank adapters of one projection."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("count", ctypes.c_uint64), ("rank", ctypes.c_uint64), ("k", ctypes.c_uint64),
+                ("n", ctypes.c_uint64), ("dtype", ctypes.c_int32)]
+
+
+class Experts(ctypes.Structure):
+    """`mgb_experts`: the packed experts of one mixture-of-experts layer."""
+    _fields_ = [("gate", ctypes.c_void_p), ("up", ctypes.c_void_p), ("down", ctypes.c_void_p),
+                ("experts", ctypes.c_uint64), ("hidden", ctypes.c_uint64),
+                ("ffn", ctypes.c_uint64), ("gate_up_format", ctypes.c_int32),
+                ("down_format", ctypes.c_int32)]
+
+
 _lib = None
 _vp, _u64, _i32, _cp = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int32, ctypes.c_char_p
 _u64p = ctypes.POINTER(ctypes.c_uint64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
+_adp, _exp = ctypes.POINTER(Adapters), ctypes.POINTER(Experts)
 
 _SIGNATURES = {
     "mgb_last_error": ([], _cp),
@@ -148,6 +165,21 @@ _SIGNATURES = {
     "mgb_take_device_error": ([_i32, _i32p], _i32),
     "mgb_embedding": ([_i32, _vp, _u64, _u64, _i32, _vp, _u64, _i32, ctypes.c_float, _vp, _vp, _vp],
                       _i32),
+    "mgb_adapters_workspace_bytes": ([_adp, _u64], _u64),
+    "mgb_adapters_add": ([_adp, _vp, _vp, _u64, _vp, _vp, _vp, _vp, _u64, _vp], _i32),
+    "mgb_qmatmul_adapters_workspace_bytes": ([_i32, _u64, _u64, _u64, _adp], _u64),
+    "mgb_qmatmul_adapters": ([_i32, _vp, _u64, _u64, _vp, _u64, _vp, _vp, _u64, _adp, _vp, _vp,
+                              _vp, _u64, _vp], _i32),
+    "mgb_moe_workspace_bytes": ([_exp, _u64, _u64], _u64),
+    "mgb_moe_route_workspace_bytes": ([_u64, _u64, _u64], _u64),
+    "mgb_moe_route": ([_vp, _u64, _u64, _vp, _u64, _u64, _i32, ctypes.c_float, _vp, _vp, _vp,
+                       _u64, _vp], _i32),
+    "mgb_moe_experts": ([_exp, _vp, _u64, _vp, _vp, _u64, _vp, _vp, _vp, _vp, _u64, _vp], _i32),
+    "mgb_moe_layer": ([_exp, _vp, _vp, _u64, _u64, _i32, ctypes.c_float, _vp, _vp, _vp, _vp, _vp,
+                       _u64, _vp], _i32),
+    "mgb_sample_workspace_bytes": ([_u64, _u64], _u64),
+    "mgb_sample": ([_vp, _u64, _u64, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64,
+                    _vp], _i32),
     "mgb_device_alloc": ([_u64, ctypes.POINTER(_vp)], _i32),
     "mgb_device_free": ([_vp], _i32),
     "mgb_ipc_handle": ([_vp, _vp], _i32),
@@ -249,6 +281,95 @@ def take_device_error(device: int = 0) -> int:
     code = ctypes.c_int32(0)
     check(lib().mgb_take_device_error(device, ctypes.byref(code)))
     return code.value
+
+
+# ---- rows that choose: adapters, experts, sampled tokens (device pointers as ints) ------
+
+
+def adapters(a_ptr: int, b_ptr: int, count: int, rank: int, k: int, n: int, dtype: int = F32,
+             scales_ptr: int = 0) -> Adapters:
+    """`mgb_adapters`: a [count, rank, k] and b [count, n, rank] of `dtype`."""
+    return Adapters(a_ptr or None, b_ptr or None, scales_ptr or None, count, rank, k, n, dtype)
+
+
+def adapters_workspace_bytes(ad: Adapters, m: int) -> int:
+    return int(lib().mgb_adapters_workspace_bytes(ad, m))
+
+
+def adapters_add(ad: Adapters, ids_ptr: int, x_ptr: int, m: int, y_ptr: int, base_ptr: int = 0,
+                 bad_ptr: int = 0, workspace_ptr: int = 0, workspace_bytes: int = 0,
+                 stream: int = 0) -> None:
+    check(lib().mgb_adapters_add(ad, ids_ptr, x_ptr, m, base_ptr or None, y_ptr, bad_ptr or None,
+                                 workspace_ptr or None, workspace_bytes, stream or None))
+
+
+def qmatmul_adapters_workspace_bytes(fmt: int, m: int, n: int, k: int, ad: Adapters) -> int:
+    return int(lib().mgb_qmatmul_adapters_workspace_bytes(fmt, m, n, k, ad))
+
+
+def qmatmul_adapters(fmt: int, w_ptr: int, n: int, k: int, x_ptr: int, m: int, y_ptr: int,
+                     ad: Adapters, ids_ptr: int, addend_ptr: int = 0, addend_len: int = 0,
+                     bad_ptr: int = 0, workspace_ptr: int = 0, workspace_bytes: int = 0,
+                     stream: int = 0) -> None:
+    check(lib().mgb_qmatmul_adapters(fmt, w_ptr, n, k, x_ptr, m, y_ptr, addend_ptr or None,
+                                     addend_len, ad, ids_ptr, bad_ptr or None,
+                                     workspace_ptr or None, workspace_bytes, stream or None))
+
+
+def experts(gate_up_fmt: int, gate_ptr: int, up_ptr: int, down_fmt: int, down_ptr: int,
+            count: int, hidden: int, ffn: int) -> Experts:
+    """`mgb_experts`: gate and up [count * ffn, hidden], down [count * hidden, ffn], packed."""
+    return Experts(gate_ptr or None, up_ptr or None, down_ptr or None, count, hidden, ffn,
+                   gate_up_fmt, down_fmt)
+
+
+def moe_workspace_bytes(ex: Experts, m: int, top_k: int) -> int:
+    return int(lib().mgb_moe_workspace_bytes(ex, m, top_k))
+
+
+def moe_route_workspace_bytes(count: int, hidden: int, m: int) -> int:
+    return int(lib().mgb_moe_route_workspace_bytes(count, hidden, m))
+
+
+def moe_route(router_ptr: int, count: int, hidden: int, x_ptr: int, m: int, top_k: int,
+              normalize: bool, ids_ptr: int, weights_ptr: int, scale: float = 1.0,
+              workspace_ptr: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+    check(lib().mgb_moe_route(router_ptr, count, hidden, x_ptr, m, top_k, int(normalize), scale,
+                              ids_ptr, weights_ptr, workspace_ptr or None, workspace_bytes,
+                              stream or None))
+
+
+def moe_experts(ex: Experts, x_ptr: int, m: int, ids_ptr: int, weights_ptr: int, top_k: int,
+                y_ptr: int, addend_ptr: int = 0, bad_ptr: int = 0, workspace_ptr: int = 0,
+                workspace_bytes: int = 0, stream: int = 0) -> None:
+    check(lib().mgb_moe_experts(ex, x_ptr, m, ids_ptr, weights_ptr, top_k, addend_ptr or None,
+                                y_ptr, bad_ptr or None, workspace_ptr or None, workspace_bytes,
+                                stream or None))
+
+
+def moe_layer(ex: Experts, router_ptr: int, x_ptr: int, m: int, top_k: int, normalize: bool,
+              y_ptr: int, scale: float = 1.0, addend_ptr: int = 0, ids_ptr: int = 0,
+              weights_ptr: int = 0, workspace_ptr: int = 0, workspace_bytes: int = 0,
+              stream: int = 0) -> None:
+    check(lib().mgb_moe_layer(ex, router_ptr, x_ptr, m, top_k, int(normalize), scale,
+                              addend_ptr or None, y_ptr, ids_ptr or None, weights_ptr or None,
+                              workspace_ptr or None, workspace_bytes, stream or None))
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    return int(lib().mgb_sample_workspace_bytes(rows, vocab))
+
+
+def sample(logits_ptr: int, rows: int, vocab: int, ids_ptr: int, ld: int = 0,
+           temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0, min_p_ptr: int = 0,
+           uniform_ptr: int = 0, logprob_ptr: int = 0, kept_ptr: int = 0, workspace_ptr: int = 0,
+           workspace_bytes: int = 0, stream: int = 0) -> None:
+    """One token per row of logits (`ld` 0: rows are contiguous)."""
+    check(lib().mgb_sample(logits_ptr, rows, vocab, ld or vocab, temperature_ptr or None,
+                           top_k_ptr or None, top_p_ptr or None, min_p_ptr or None,
+                           uniform_ptr or None, ids_ptr or None, logprob_ptr or None,
+                           kept_ptr or None, workspace_ptr or None, workspace_bytes,
+                           stream or None))
 
 
 # ---- tensor parallelism (device pointers as ints) -------------------------------------

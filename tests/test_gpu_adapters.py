@@ -1,0 +1,278 @@
+"""Low-rank adapters (`mgb_adapters_add`, `mgb_qmatmul_adapters`) against the
+formula in 64 bits.
+
+Tolerance.  An output is base + s * sum_r b_r h_r with h_r = sum_j a_j x_j.  The
+kernels accumulate in f32 from operands of at least 22 bits, so every product
+is off by at most 2^-21 of itself and every addition by 2^-24 of the running
+sum.  With the magnitudes M = s * sum_r |b_r| sum_j |a_j x_j| an output is off
+by at most (2^-21 + (k + rank) 2^-24) M + 2 * 2^-24 (|base| + |y|) (each term
+rounded at every later addition); over a whole array the roundings are
+independent, so the 2-norm of the difference stays below 2^-19 of the result's.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import magnetar_b200 as mgb
+import synthetic
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": mgb.F32, "f16": mgb.F16, "bf16": mgb.BF16}
+
+
+@pytest.fixture(scope="module")
+def torch_cuda(cuda_device):
+    import torch
+
+    torch.cuda.set_device(cuda_device)
+    return torch
+
+
+def _torch_dtype(torch, dtype):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+
+
+def _inputs(torch, m, k, n, rank, count, dtype, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    dt = _torch_dtype(torch, dtype)
+    a = (torch.randn(count, rank, k, generator=g) / k ** 0.5).to(dt)
+    b = (torch.randn(count, n, rank, generator=g) / rank ** 0.5).to(dt)
+    scales = 0.5 + torch.rand(count, generator=g)
+    return (a, b, scales, torch.randn(m, k, generator=g), torch.randn(m, n, generator=g))
+
+
+def _call(torch, a, b, scales, dtype, ids, x, base, y=None, bad=None, stream=0, ws=None):
+    count, rank, k = a.shape
+    n, m = b.shape[1], x.shape[0]
+    ad = mgb.adapters(a.data_ptr(), b.data_ptr(), count, rank, k, n, DTYPES[dtype],
+                      scales.data_ptr() if scales is not None else 0)
+    size = mgb.adapters_workspace_bytes(ad, m)
+    if ws is None:
+        ws = torch.full((max(1, size),), 0xFF, dtype=torch.uint8, device="cuda")
+    y = torch.full((m, n), float("nan"), device="cuda") if y is None else y
+    mgb.adapters_add(ad, ids.data_ptr(), x.data_ptr(), m, y.data_ptr(),
+                     base_ptr=base.data_ptr() if base is not None else 0,
+                     bad_ptr=bad.data_ptr() if bad is not None else 0,
+                     workspace_ptr=ws.data_ptr(), workspace_bytes=size,
+                     stream=stream or torch.cuda.current_stream().cuda_stream)
+    return y
+
+
+def _expected(a, b, scales, ids, x, base):
+    """(y, magnitudes) in 64 bits."""
+    y, mag = base.double().clone(), base.double().abs() * 0
+    for row, i in enumerate(ids.tolist()):
+        if i < 0:
+            continue
+        aa, bb = a[int(i)].double(), b[int(i)].double()
+        s = float(scales[int(i)])
+        y[row] += s * (bb @ (aa @ x[row].double()))
+        mag[row] = abs(s) * (bb.abs() @ (aa.abs() @ x[row].double().abs()))
+    return y, mag
+
+
+def _check(got, want, mag, base, k, rank):
+    got = got.double().cpu()
+    e = 2.0 ** -24
+    bound = (8 + k + rank) * e * mag + 2 * e * (base.double().abs() + want.abs())
+    worst = ((got - want).abs() / bound.clamp_min(1e-300)).max()
+    assert bool(((got - want).abs() <= bound).all()), float(worst)
+    assert float((got - want).norm() / want.norm().clamp_min(1e-30)) < 2.0 ** -19
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,k,n,rank,count", [
+    (1, 1, 1, 1, 1), (1, 64, 64, 8, 2), (1, 4096, 1024, 16, 8), (3, 33, 7, 3, 2),
+    (7, 95, 130, 11, 5), (16, 256, 512, 16, 4), (17, 1000, 264, 24, 3), (40, 512, 96, 64, 40),
+    (65, 136, 1001, 5, 7), (130, 320, 200, 128, 2), (200, 64, 72, 256, 3)])
+def test_matches_the_formula(torch_cuda, dtype, m, k, n, rank, count):
+    torch = torch_cuda
+    a, b, scales, x, base = _inputs(torch, m, k, n, rank, count, dtype)
+    g = torch.Generator().manual_seed(m + k)
+    ids = torch.randint(-1, count, (m,), generator=g).float()
+    want, mag = _expected(a, b, scales, ids, x, base)
+    dev = [t.cuda() for t in (a, b, scales, ids, x, base)]
+    y = _call(torch, *dev[:3], dtype, *dev[3:])
+    _check(y, want, mag, base, k, rank)
+    none = (ids < 0).nonzero()[:, 0]
+    assert torch.equal(y.cpu()[none], base[none])  # bit for bit
+    # the same call twice: the same bits
+    assert torch.equal(_call(torch, *dev[:3], dtype, *dev[3:]), y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [70, 300, 1500])
+@pytest.mark.parametrize("order", ["prompts", "alternating", "one", "none"])
+def test_many_rows(torch_cuda, dtype, m, order):
+    """Prompts of consecutive rows, rows that take turns, one adapter, none."""
+    torch = torch_cuda
+    k, n, rank, count = 264, 328, 16, 6
+    a, b, scales, x, base = _inputs(torch, m, k, n, rank, count, dtype)
+    at = torch.arange(m)
+    ids = {"prompts": torch.bucketize(at, torch.tensor([5, 33, m // 2, m - 1])) - 1,
+           "alternating": at % (count + 1) - 1, "one": at * 0 + 3, "none": at * 0 - 1}[order].float()
+    want, mag = _expected(a, b, scales, ids, x, base)
+    dev = [t.cuda() for t in (a, b, scales, ids, x, base)]
+    y = _call(torch, *dev[:3], dtype, *dev[3:])
+    _check(y, want, mag, base, k, rank)
+    # in place: base is y
+    z = dev[5].clone()
+    assert torch.equal(_call(torch, *dev[:3], dtype, *dev[3:5], z, y=z), y)
+
+
+def test_no_base_and_no_scales(torch_cuda):
+    torch = torch_cuda
+    a, b, _, x, base = _inputs(torch, 9, 128, 64, 8, 3, "bf16")
+    ids = torch.tensor([0, 1, 2, -1, 2, 2, 0, -7.5, 1.0])  # any negative id: no adapter
+    one = torch.ones(3)
+    want, mag = _expected(a, b, one, ids, x, base * 0)
+    y = _call(torch, a.cuda(), b.cuda(), None, "bf16", ids.cuda(), x.cuda(), None)
+    _check(y, want, mag, base * 0, 128, 8)
+    assert bool((y[3] == 0).all()) and bool((y[7] == 0).all())
+
+
+@pytest.mark.parametrize("m", [9, 150])
+def test_invalid_ids_are_reported_and_skipped(torch_cuda, m):
+    torch = torch_cuda
+    a, b, scales, x, base = _inputs(torch, m, 96, 64, 8, 4, "f32")
+    dev = [t.cuda() for t in (a, b, scales)]
+    xd, based = x.cuda(), base.cuda()
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for wrong in (4.0, 1e9, 0.5, float("nan"), float("inf")):
+        ids = torch.arange(m).float() % 4
+        ids[7], ids[5] = wrong, wrong
+        y = _call(torch, *dev, "f32", ids.cuda(), xd, based, bad=bad)
+        assert int(bad) == 5
+        want, mag = _expected(a, b, scales, torch.where(ids == torch.arange(m) % 4, ids, -1.0), x, base)
+        _check(y, want, mag, base, 96, 8)
+        assert torch.equal(y[5].cpu(), base[5]) and torch.equal(y[7].cpu(), base[7])
+    ids = (torch.arange(m).float() % 5 - 1)
+    _call(torch, *dev, "f32", ids.cuda(), xd, based, bad=bad)
+    assert int(bad) == -1  # 0xFFFFFFFF
+
+
+def test_nan_stays_in_its_row(torch_cuda):
+    """A row's NaN or infinity reaches that row alone, and an unused adapter's none."""
+    torch = torch_cuda
+    for m in (6, 96):
+        a, b, scales, x, base = _inputs(torch, m, 128, 64, 16, 3, "bf16")
+        a[2], b[2] = float("nan"), float("inf")
+        x[1, 3] = float("nan")
+        ids = torch.zeros(m)
+        ids[2::2] = 1
+        y = _call(torch, *[t.cuda() for t in (a, b, scales)], "bf16", ids.cuda(), x.cuda(), base.cuda()).cpu()
+        assert bool(y[1].isnan().all())
+        rest = torch.arange(m) != 1
+        assert bool(y[rest].isfinite().all())
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_unaligned_buffers(torch_cuda, dtype, offset):
+    """Every buffer starts `offset` elements past an aligned address."""
+    torch = torch_cuda
+    for m in (5, 90):
+        k, n, rank, count = 128, 96, 16, 3
+        parts = _inputs(torch, m, k, n, rank, count, dtype)
+        ids = torch.arange(m).float() % (count + 1) - 1
+        want, mag = _expected(*parts[:3], ids, *parts[3:])
+
+        def off(t):
+            buf = torch.empty(t.numel() + offset, dtype=t.dtype, device="cuda")
+            buf[offset:] = t.flatten().cuda()
+            return buf[offset:].view(t.shape)
+
+        y = off(torch.zeros(m, n))
+        _call(torch, *[off(t) for t in parts[:3]], dtype, off(ids), off(parts[3]), off(parts[4]), y=y)
+        _check(y, want, mag, parts[4], k, rank)
+
+
+def test_rows_behind_the_last_are_left(torch_cuda):
+    torch = torch_cuda
+    for m in (5, 90):
+        a, b, scales, x, base = _inputs(torch, m + 3, 128, 72, 8, 3, "f16")
+        ids = torch.zeros(m + 3)
+        y = torch.full((m + 3, 72), 7.0, device="cuda")
+        _call(torch, *[t.cuda() for t in (a, b, scales)], "f16", ids.cuda(), x[:m].cuda(), base.cuda(), y=y)
+        assert bool((y[m:] == 7.0).all())
+
+
+@pytest.mark.parametrize("m", [4, 120])
+def test_large_and_small_activations(torch_cuda, m):
+    """Rows of very different magnitude (f32's range is kept)."""
+    torch = torch_cuda
+    a, b, scales, x, base = _inputs(torch, m, 256, 64, 16, 3, "bf16")
+    x *= 10.0 ** torch.linspace(-20, 20, m)[:, None]
+    ids = torch.arange(m).float() % 3
+    want, mag = _expected(a, b, scales, ids, x, base * 0)
+    y = _call(torch, *[t.cuda() for t in (a, b, scales)], "bf16", ids.cuda(), x.cuda(), None)
+    got = y.double().cpu()
+    assert bool(((got - want).abs() <= (8 + 256 + 16) * 2.0 ** -24 * mag + 2.0 ** -23 * want.abs()).all())
+    rows = (got - want).norm(dim=1) / want.norm(dim=1)
+    assert float(rows.max()) < 2.0 ** -19
+
+
+@pytest.mark.parametrize("fmt,m,n,k", [(mgb.Q4_K, 1, 96, 512), (mgb.Q4_K, 2, 300, 1024),
+                                       (mgb.Q8_0, 5, 64, 96), (mgb.Q6_K, 33, 520, 512),
+                                       (mgb.IQ4_NL, 140, 256, 256)])
+def test_beside_a_packed_projection(torch_cuda, fmt, m, n, k):
+    """The projection's y plus the adapters', bit for bit the two calls; rows
+    without an adapter are the projection's."""
+    torch = torch_cuda
+    stream = torch.cuda.current_stream().cuda_stream
+    src = torch.from_numpy(synthetic.packed_weights(fmt, n, k, seed=5)).cuda()
+    w = torch.empty(mgb.packed_bytes(fmt, n, k), dtype=torch.uint8, device="cuda")
+    mgb.repack(fmt, src.data_ptr(), n, k, w.data_ptr(), stream)
+    a, b, scales, x, _ = (t.cuda() for t in _inputs(torch, m, k, n, 16, 4, "bf16"))
+    bias = torch.randn(n, device="cuda")
+    ids = (torch.arange(m, device="cuda") % 5 - 1).float()
+    ad = mgb.adapters(a.data_ptr(), b.data_ptr(), 4, 16, k, n, mgb.BF16, scales.data_ptr())
+    size = mgb.qmatmul_adapters_workspace_bytes(fmt, m, n, k, ad)
+    ws = torch.empty(max(1, size), dtype=torch.uint8, device="cuda")
+    y = torch.full((m, n), float("nan"), device="cuda")
+    mgb.qmatmul_adapters(fmt, w.data_ptr(), n, k, x.data_ptr(), m, y.data_ptr(), ad, ids.data_ptr(),
+                         addend_ptr=bias.data_ptr(), addend_len=n, workspace_ptr=ws.data_ptr(),
+                         workspace_bytes=size, stream=stream)
+    plain = torch.full((m, n), float("nan"), device="cuda")
+    mgb.qmatmul(fmt, w.data_ptr(), n, k, x.data_ptr(), m, plain.data_ptr(), bias.data_ptr(), n,
+                ws.data_ptr(), size, stream)
+    torch.cuda.synchronize()
+    assert torch.equal(y[ids < 0], plain[ids < 0])
+    both = _call(torch, a, b, scales, "bf16", ids, x, plain)
+    assert torch.equal(y, both)
+    assert m < 2 or not torch.equal(y, plain)
+    assert mgb.take_device_error(0) == 0
+
+
+def test_other_stream_and_graph(torch_cuda):
+    """On a side stream, and captured and replayed with new inputs; two graphs
+    with a workspace each do not disturb one another."""
+    torch = torch_cuda
+    for m in (3, 100):
+        a, b, scales, x, base = (t.cuda() for t in _inputs(torch, m, 128, 96, 16, 4, "f16"))
+        ids = (torch.arange(m, device="cuda") % 5 - 1).float()
+        want = _call(torch, a, b, scales, "f16", ids, x, base)
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        y = torch.empty_like(base)
+        with torch.cuda.stream(side):
+            _call(torch, a, b, scales, "f16", ids, x, base, y=y, ws=torch.empty(1 << 20, dtype=torch.uint8, device="cuda"))
+        side.synchronize()
+        assert torch.equal(y, want)
+        graphs = []
+        for _ in range(2):
+            gx, gy = x.clone(), torch.empty_like(base)
+            ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                _call(torch, a, b, scales, "f16", ids, gx, base, y=gy, ws=ws)
+            graphs.append((graph, gx, gy, ws))
+        graphs[0][1].mul_(2)
+        for graph, *_ in graphs * 3:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[1][2], want)
+        assert torch.equal(graphs[0][2], _call(torch, a, b, scales, "f16", ids, x * 2, base))
