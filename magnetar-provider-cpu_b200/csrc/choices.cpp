@@ -81,6 +81,9 @@ mgb_status check_experts(const mgb_experts *ex, uint64_t m, uint64_t top_k) {
   if (!top_k || top_k > MGB_MOE_MAX_TOP_K)
     return fail(MGB_INVALID_ARGUMENT, "top_k %llu, expected 1 to %d", (unsigned long long)top_k,
                 MGB_MOE_MAX_TOP_K);
+  // the kernels address activations (4 bytes a value) with 32-bit offsets
+  if (m * top_k * (ex->hidden > ex->ffn ? ex->hidden : ex->ffn) >= (1ull << 30))
+    return fail(MGB_INVALID_ARGUMENT, "tokens * top_k * sizes reach 2^30 values");
   return MGB_OK;
 }
 
@@ -176,12 +179,10 @@ uint64_t mgb_moe_route_workspace_bytes(uint64_t experts, uint64_t hidden, uint64
   return round16(moe_route_scratch_bytes(experts, hidden, m));
 }
 
-// mgb_moe_layer: the experts' scratch, then the routing's, then ids and weights.
+// The experts' scratch, then room for mgb_moe_layer's ids and weights.
 uint64_t mgb_moe_workspace_bytes(const mgb_experts *experts, uint64_t m, uint64_t top_k) {
   if (check_experts(experts, m, top_k) != MGB_OK) return 0;
-  return round16(moe_experts_scratch_bytes(*experts, m, top_k)) +
-         round16(moe_route_scratch_bytes(experts->experts, experts->hidden, m)) +
-         2 * round16(m * top_k * 4);
+  return round16(moe_experts_scratch_bytes(*experts, m, top_k)) + 2 * round16(m * top_k * 4);
 }
 
 mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden, const float *x,
@@ -195,7 +196,7 @@ mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden,
     s = check_workspace(workspace, workspace_bytes, moe_route_scratch_bytes(experts, hidden, m));
   if (s != MGB_OK) return s;
   cudaError_t e = launch_moe_route(router, experts, hidden, x, m, top_k, normalize != 0, scale, ids,
-                                   weights, workspace, static_cast<cudaStream_t>(stream));
+                                   weights, nullptr, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "routing launch");
 }
 
@@ -208,7 +209,7 @@ mgb_status mgb_moe_experts(const mgb_experts *experts, const float *x, uint64_t 
     s = check_workspace(workspace, workspace_bytes, moe_experts_scratch_bytes(*experts, m, top_k));
   if (s != MGB_OK) return s;
   cudaError_t e = launch_moe_experts(*experts, x, m, ids, weights, top_k, addend, y, bad, workspace,
-                                     static_cast<cudaStream_t>(stream));
+                                     false, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "expert launch");
 }
 
@@ -221,18 +222,18 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
   if (s == MGB_OK)
     s = check_workspace(workspace, workspace_bytes, mgb_moe_workspace_bytes(experts, m, top_k));
   if (s != MGB_OK) return s;
-  uint8_t *route = static_cast<uint8_t *>(workspace) +
-                   round16(moe_experts_scratch_bytes(*experts, m, top_k));
-  uint8_t *own = route + round16(moe_route_scratch_bytes(experts->experts, experts->hidden, m));
+  uint8_t *own = static_cast<uint8_t *>(workspace) +
+                 round16(moe_experts_scratch_bytes(*experts, m, top_k));
   if (!ids) ids = reinterpret_cast<float *>(own);
   if (!weights) weights = reinterpret_cast<float *>(own + round16(m * top_k * 4));
   s = check_experts_call(experts, x, m, ids, weights, top_k, addend, y);
   if (s != MGB_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_moe_route(router, experts->experts, experts->hidden, x, m, top_k,
-                                   normalize != 0, scale, ids, weights, route, st);
+                                   normalize != 0, scale, ids, weights, experts, workspace, st);
   if (e != cudaSuccess) return cuda_fail(e, "routing launch");
-  e = launch_moe_experts(*experts, x, m, ids, weights, top_k, addend, y, nullptr, workspace, st);
+  e = launch_moe_experts(*experts, x, m, ids, weights, top_k, addend, y, nullptr, workspace, true,
+                         st);
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "expert launch");
 }
 

@@ -1,0 +1,6 @@
+// The expert products over Q5_K weights.
+#include "experts_launch.cuh"
+
+namespace mgb {
+template cudaError_t launch_moe_product<Q5_K>(const moe::Args &, bool, int, int, cudaStream_t);
+}  // namespace mgb

@@ -68,16 +68,18 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
                             const float *base, float *y, uint32_t *bad, void *workspace,
                             cudaStream_t stream);
 
-// experts.cu
+// experts.cu.  With pack_for (the experts of mgb_moe_layer, `workspace` theirs)
+// the routing kernel also packs the activations for the products.
 uint64_t moe_route_scratch_bytes(uint64_t experts, uint64_t hidden, uint64_t m);
 uint64_t moe_experts_scratch_bytes(const mgb_experts &ex, uint64_t m, uint64_t top_k);
 cudaError_t launch_moe_route(const float *router, uint64_t experts, uint64_t hidden,
                              const float *x, uint64_t m, uint64_t top_k, int normalize,
-                             float scale, float *ids, float *weights, void *workspace,
-                             cudaStream_t stream);
+                             float scale, float *ids, float *weights, const mgb_experts *pack_for,
+                             void *workspace, cudaStream_t stream);
+// packed: x is in the workspace's packets already (launch_moe_route with pack_for)
 cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m, const float *ids,
                                const float *weights, uint64_t top_k, const float *addend, float *y,
-                               uint32_t *bad, void *workspace, cudaStream_t stream);
+                               uint32_t *bad, void *workspace, bool packed, cudaStream_t stream);
 
 // sample.cu
 struct SampleArgs {
