@@ -376,8 +376,8 @@ mgb_status mgb_quantize_rows(const float *x, uint64_t len, int8_t *values, float
 /* Operators in which every activation row of a batch picks what it meets: the
  * low-rank adapter added to a shared projection, the experts of a mixture, the
  * next token.  No counterparts on the reference's packed path.  Device
- * pointers of the current device throughout; work is queued on `stream` and
- * nothing is allocated, synchronised or kept between calls.  As in
+ * pointers of the current device throughout; work is queued on `stream`,
+ * nothing is synchronised and nothing kept between calls.  As in
  * `mgb_embedding`, ids are f32 device values and `bad` (device u32, may be
  * NULL) receives the position of the first invalid one, 0xFFFFFFFF when all
  * are valid.  A call's workspace (16-byte aligned) is scratch: calls that may
@@ -429,6 +429,7 @@ mgb_status mgb_qmatmul_adapters(int32_t format, const void *w, uint64_t n, uint6
 #define MGB_MOE_MAX_TOKENS 256
 #define MGB_MOE_MAX_EXPERTS 1024
 #define MGB_MOE_MAX_TOP_K 32
+#define MGB_MOE_MAX_WIDTH (1u << 18) /* hidden and ffn */
 typedef struct mgb_experts {
     const void *gate;
     const void *up;
@@ -455,8 +456,11 @@ mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden,
  * addend [m, hidden] may be NULL (zeros) or y.  A slot whose id is negative is
  * unused, as is one with an invalid id (reported in `bad`).  The same id twice
  * counts twice.  Each chosen expert's packed rows are read once for all its
- * tokens; f32 accuracy (f32 accumulation, operands of at least 22 bits);
- * deterministic. */
+ * tokens; f32 accuracy: weights enter exactly,
+ * activations with at least 22 bits (values below 2^-27 of their row's largest:
+ * 2^-40 of the largest), sums in f32.  Deterministic.  The first call on a
+ * device allocates its error word (see mgb_take_device_error), as mgb_qmatmul's
+ * does: make it before any stream capture. */
 mgb_status mgb_moe_experts(const mgb_experts *experts, const float *x, uint64_t m,
                            const float *ids, const float *weights, uint64_t top_k,
                            const float *addend, float *y, uint32_t *bad, void *workspace,

@@ -70,7 +70,7 @@ mgb_status check_experts(const mgb_experts *ex, uint64_t m, uint64_t top_k) {
   if (!ex->experts || ex->experts > MGB_MOE_MAX_EXPERTS)
     return fail(MGB_INVALID_ARGUMENT, "%llu experts, expected 1 to %d",
                 (unsigned long long)ex->experts, MGB_MOE_MAX_EXPERTS);
-  if (ex->hidden > (1u << 24) || ex->ffn > (1u << 24) || too_large(ex->experts, ex->hidden, ex->ffn))
+  if (ex->hidden > MGB_MOE_MAX_WIDTH || ex->ffn > MGB_MOE_MAX_WIDTH || too_large(ex->experts, ex->hidden, ex->ffn))
     return fail(MGB_INVALID_ARGUMENT, "expert sizes are too large");
   mgb_status s = check_packed_shape(ex->gate_up_format, ex->experts * ex->ffn, ex->hidden);
   if (s == MGB_OK) s = check_packed_shape(ex->down_format, ex->experts * ex->hidden, ex->ffn);
@@ -81,9 +81,11 @@ mgb_status check_experts(const mgb_experts *ex, uint64_t m, uint64_t top_k) {
   if (!top_k || top_k > MGB_MOE_MAX_TOP_K)
     return fail(MGB_INVALID_ARGUMENT, "top_k %llu, expected 1 to %d", (unsigned long long)top_k,
                 MGB_MOE_MAX_TOP_K);
-  // the kernels address activations (4 bytes a value) with 32-bit offsets
-  if (m * top_k * (ex->hidden > ex->ffn ? ex->hidden : ex->ffn) >= (1ull << 30))
-    return fail(MGB_INVALID_ARGUMENT, "tokens * top_k * sizes reach 2^30 values");
+  // blocks of 128 rows by 256 columns are counted in 32 bits
+  const uint64_t blocks = (ex->hidden / 128 + 1) * (ex->ffn / 128 + 1);
+  if (m * top_k * blocks >= (1ull << 31))
+    return fail(MGB_INVALID_ARGUMENT, "expert sizes are too large for %llu tokens",
+                (unsigned long long)m);
   return MGB_OK;
 }
 
@@ -107,7 +109,7 @@ mgb_status check_route(const float *router, uint64_t experts, uint64_t hidden, c
   if (!experts || experts > MGB_MOE_MAX_EXPERTS)
     return fail(MGB_INVALID_ARGUMENT, "%llu experts, expected 1 to %d", (unsigned long long)experts,
                 MGB_MOE_MAX_EXPERTS);
-  if (!hidden || hidden > (1u << 24)) return fail(MGB_INVALID_ARGUMENT, "hidden %llu is out of range", (unsigned long long)hidden);
+  if (!hidden || hidden > MGB_MOE_MAX_WIDTH) return fail(MGB_INVALID_ARGUMENT, "hidden %llu is out of range", (unsigned long long)hidden);
   if (m > MGB_MOE_MAX_TOKENS)
     return fail(MGB_INVALID_ARGUMENT, "%llu tokens, at most %d are taken in one call",
                 (unsigned long long)m, MGB_MOE_MAX_TOKENS);
@@ -118,6 +120,13 @@ mgb_status check_route(const float *router, uint64_t experts, uint64_t hidden, c
   if (!aligned(router, 4) || !aligned(x, 4))
     return fail(MGB_INVALID_ARGUMENT, "a device pointer is not aligned to its element size");
   return MGB_OK;
+}
+
+// The device error word of the current device (bounded waits that give up).
+int *error_word() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return device_error_flag(dev);
 }
 
 uint64_t round16(uint64_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -173,7 +182,7 @@ mgb_status mgb_qmatmul_adapters(int32_t format, const void *w, uint64_t n, uint6
 }
 
 uint64_t mgb_moe_route_workspace_bytes(uint64_t experts, uint64_t hidden, uint64_t m) {
-  if (!experts || experts > MGB_MOE_MAX_EXPERTS || !hidden || hidden > (1u << 24) ||
+  if (!experts || experts > MGB_MOE_MAX_EXPERTS || !hidden || hidden > MGB_MOE_MAX_WIDTH ||
       m > MGB_MOE_MAX_TOKENS)
     return 0;
   return round16(moe_route_scratch_bytes(experts, hidden, m));
@@ -209,7 +218,7 @@ mgb_status mgb_moe_experts(const mgb_experts *experts, const float *x, uint64_t 
     s = check_workspace(workspace, workspace_bytes, moe_experts_scratch_bytes(*experts, m, top_k));
   if (s != MGB_OK) return s;
   cudaError_t e = launch_moe_experts(*experts, x, m, ids, weights, top_k, addend, y, bad, workspace,
-                                     false, static_cast<cudaStream_t>(stream));
+                                     false, error_word(), static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "expert launch");
 }
 
@@ -233,7 +242,7 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
                                    normalize != 0, scale, ids, weights, experts, workspace, st);
   if (e != cudaSuccess) return cuda_fail(e, "routing launch");
   e = launch_moe_experts(*experts, x, m, ids, weights, top_k, addend, y, nullptr, workspace, true,
-                         st);
+                         error_word(), st);
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "expert launch");
 }
 

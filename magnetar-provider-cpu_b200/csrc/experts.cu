@@ -1,10 +1,10 @@
 // A mixture-of-experts layer over packed experts, for a few tokens:
 //   z = x R^T;  (e_j, w_j) = the top_k of z and their softmax weights;
 //   y = addend + sum_j w_j D_ej (silu(G_ej x) * (U_ej x)).
-// Four launches, each a programmatic dependent of the one before: routing (a
-// cluster per token, which also packs the token's activations), gate and up,
-// down, and the weighted sum over a token's slots.  The two products are in
-// experts.cuh.
+// Five launches, each a programmatic dependent of the one before: routing (a
+// cluster per token, which also packs the token's activations), gate and up, h
+// (a cluster per slot, packed again), down, and the weighted sum over a token's
+// slots.  The two products are in experts.cuh.
 #include <cooperative_groups.h>
 
 #include "experts.cuh"
@@ -17,36 +17,44 @@ using moe::expert_of;
 constexpr int ROUTE_CTAS = 8;  // of a token's cluster
 constexpr int ROUTE_THREADS = 256;
 
-// The token's activations in packets for weights of format fmt: run by run over
-// the warps `first`, first + step, ...
-__device__ __forceinline__ void pack_token(int fmt, const float *x, int token,
-                                           int hidden, int first, int step, uint8_t *packets,
-                                           float2 *meta) {
-  const int lane = threadIdx.x & 31, runs = hidden / RUN;
-  for (int r = first; r < runs; r += step) {
-    const size_t at = (size_t)token * runs + r;
-    moe::write_packet(fmt, moe::ld_f32(x + (size_t)token * hidden + r * RUN + lane), lane,
-                      packets + at * moe::PACKET, meta + at);
-  }
+// Packs row `row` of x for weights of format fmt: the runs first, first + step,
+// ... by this CTA's warps (first, step count warps).  Every CTA finds the row's
+// largest magnitude itself.
+template <int CTA_THREADS>
+__device__ __forceinline__ void pack_row(int fmt, const float *x, uint64_t row, int cols, int first,
+                                         int step, const moe::Packed16 &o) {
+  __shared__ float most[CTA_THREADS / 32];
+  const int lane = threadIdx.x & 31;
+  const float *xr = x + row * cols;
+  float mx = 0.f;
+#pragma unroll 4
+  for (int j = threadIdx.x; j < cols; j += CTA_THREADS) mx = fmaxf(mx, fabsf(xr[j]));
+#pragma unroll
+  for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  if (lane == 0) most[threadIdx.x >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < CTA_THREADS / 32; ++w) mx = fmaxf(mx, most[w]);
+  const int k = moe::scale_exponent(mx);
+  for (int r = first; r < cols / RUN; r += step)
+    moe::pack_run16(fmt, o, row, cols, r, k, lane, [&](int i) { return xr[r * RUN + i]; });
+  if (first == 0 && lane == 0) o.scale[row] = moe::pow2(-k);
 }
 
 __global__ void __launch_bounds__(256)
-    mgb_moe_pack_kernel(int fmt, const float *x, int hidden, uint8_t *packets,
-                        float2 *meta) {
+    mgb_moe_pack_kernel(int fmt, const float *x, int cols, moe::Packed16 o) {
   moe::grid_wait();
   moe::grid_dependents();
-  pack_token(fmt, x, blockIdx.y, hidden, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8,
-             packets, meta);
+  pack_row<256>(fmt, x, blockIdx.y, cols, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8, o);
 }
 
-// One cluster per token: its warps take the experts' logits and, with
-// `packets`, the token's runs; the first CTA's first warp then picks.  A logit
-// is a sum of f32 products in chains of hidden / 128 a lane, joined in f64.
+// One cluster per token: its warps take the experts' logits and, with `pack`,
+// the token's runs; the first CTA's first warp then picks.  A logit is a sum of
+// f32 products in chains of hidden / 128 a lane, joined in f64.
 __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREADS)
     mgb_moe_route_kernel(const float *__restrict__ router, int experts, int hidden,
                          const float *x, int top_k, int normalize, float scale, float *ids,
-                         float *weights, int fmt,
-                         uint8_t *packets, float2 *meta) {
+                         float *weights, bool pack, int fmt, moe::Packed16 packed) {
   __shared__ double z[MGB_MOE_MAX_EXPERTS];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank();
@@ -64,25 +72,25 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
     if (wide) {
 #pragma unroll 4
       for (int j = lane * 4; j < hidden; j += 128) {
-        const uint4 a = moe::ld_v4(xr + j);
+        const float4 a = *reinterpret_cast<const float4 *>(xr + j);
         const float4 b = __ldg(reinterpret_cast<const float4 *>(r + j));
-        s[0] = fmaf(__uint_as_float(a.x), b.x, s[0]);
-        s[1] = fmaf(__uint_as_float(a.y), b.y, s[1]);
-        s[2] = fmaf(__uint_as_float(a.z), b.z, s[2]);
-        s[3] = fmaf(__uint_as_float(a.w), b.w, s[3]);
+        s[0] = fmaf(a.x, b.x, s[0]);
+        s[1] = fmaf(a.y, b.y, s[1]);
+        s[2] = fmaf(a.z, b.z, s[2]);
+        s[3] = fmaf(a.w, b.w, s[3]);
       }
     } else {
       for (int j = lane; j < hidden; j += 128)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if (j + 32 * c < hidden) s[c] = fmaf(moe::ld_f32(xr + j + 32 * c), r[j + 32 * c], s[c]);
+          if (j + 32 * c < hidden) s[c] = fmaf(xr[j + 32 * c], r[j + 32 * c], s[c]);
     }
     double d = ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) zs[e] = d;
   }
-  if (packets) pack_token(fmt, x, token, hidden, warp, WARPS, packets, meta);
+  if (pack) pack_row<ROUTE_THREADS>(fmt, x, token, hidden, warp, WARPS, packed);
   cluster.sync();
   if (rank || threadIdx.x >= 32) return;
 
@@ -124,64 +132,188 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
     weights[(size_t)token * top_k + lane] = (float)(mine / (normalize ? sum : total) * (double)scale);
 }
 
-// y = addend + the weighted slots of a token, in slot order.
-__global__ void __launch_bounds__(256)
-    mgb_moe_combine_kernel(const float *out, const float *ids, const float *weights, int experts,
-                           int hidden, int top_k, const float *addend, float *y) {
+// How the parts of a product are found: what its kernel left and the shapes.
+struct Parts {
+  const float *out;
+  const int32_t *place, *share;
+  int tiles, nb, width;  // row tiles of a pass, stages of a row, values of a result row
+};
+
+// The parts of row tile `tile` of a slot's pass.
+__device__ __forceinline__ int tile_parts(const Parts &p, int place, int share, int tile) {
+  return moe::parts_of((place >> 16) * p.tiles + tile, p.nb, share);
+}
+// The sum of n parts of value c of a slot; the first two (all there are in most
+// tiles) are loaded together.
+__device__ __forceinline__ float part_sum(const Parts &p, int place, int used, int n, int c) {
+  const float *at = p.out + (uint64_t)(place & 0xFFFF) * p.width + c;
+  const uint64_t step = (uint64_t)used * p.width;
+  float s = at[0];
+  if (n > 1) s += at[step];
+  for (int i = 2; i < n; ++i) s += at[i * step];
+  return s;
+}
+
+// h = silu(gate) * up of one slot, packed for the down projection: a cluster per
+// slot, which finds the row's largest magnitude together.
+constexpr int H_CTAS = 8;
+constexpr int H_THREADS = 512;
+__global__ void __cluster_dims__(H_CTAS, 1, 1) __launch_bounds__(H_THREADS)
+    mgb_moe_h_kernel(const Parts p, int ffn, int fmt, moe::Packed16 o) {
+  extern __shared__ float h[];  // this CTA's runs
+  __shared__ float most[H_THREADS / 32];
+  __shared__ float cta_most;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), slot = blockIdx.x / H_CTAS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   moe::grid_wait();
   moe::grid_dependents();
-  const int token = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
-  if (c >= hidden) return;  // hidden is a multiple of 32
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  const int place = p.place[slot];
+  if (place < 0) return;  // the whole cluster
+  const int share = p.share[0], used = p.share[1];
+  const int runs = ffn / RUN, per = (runs + H_CTAS - 1) / H_CTAS;
+  const int r0 = min(runs, rank * per), r1 = min(runs, r0 + per);
+  const int tiles1 = p.tiles / 2;
+  float mx = 0.f;
+  for (int r = r0 + warp; r < r1; r += H_THREADS / 32) {  // a warp's run lies in one tile
+    const int tile = r * RUN / moe::TILE, f = r * RUN + lane;
+    const int ng = tile_parts(p, place, share, tile), nu = tile_parts(p, place, share, tiles1 + tile);
+    const float g = part_sum(p, place, used, ng, f), u = part_sum(p, place, used, nu, ffn + f);
+    const float v = g / (1.f + expf(-g)) * u;
+    h[f - r0 * RUN] = v;
+    mx = fmaxf(mx, fabsf(v));
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  if (lane == 0) most[warp] = mx;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < H_THREADS / 32; ++w) mx = fmaxf(mx, most[w]);
+    cta_most = mx;
+  }
+  cluster.sync();
+  mx = 0.f;
+  for (int r = 0; r < H_CTAS; ++r) mx = fmaxf(mx, *cluster.map_shared_rank(&cta_most, r));
+  const int k = moe::scale_exponent(mx);
+  for (int r = r0 + warp; r < r1; r += H_THREADS / 32)
+    moe::pack_run16(fmt, o, slot, ffn, r, k, lane, [&](int i) { return h[(r - r0) * RUN + i]; });
+  if (rank == 0 && threadIdx.x == 0) o.scale[slot] = moe::pow2(-k);
+  cluster.sync();  // the others' reads of cta_most are done
+}
+
+// y = addend + the weighted slots of a token, in slot order.
+__global__ void __launch_bounds__(256)
+    mgb_moe_combine_kernel(const Parts p, const float *weights, int hidden, int top_k,
+                           const float *addend, float *y) {
+  moe::grid_wait();
+  moe::grid_dependents();
+  const int token = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= hidden) return;
+  const int share = p.share[0], used = p.share[1];
+  float a = 0.f;
+#pragma unroll 4
   for (int j = 0; j < top_k; ++j) {
-    const size_t slot = (size_t)token * top_k + j;
-    if (expert_of(moe::ld_f32(ids + slot), experts) < 0) continue;
-    const float w = moe::ld_f32(weights + slot);
-    const uint4 v = moe::ld_v4(out + slot * hidden + c);
-    a[0] = fmaf(w, __uint_as_float(v.x), a[0]);
-    a[1] = fmaf(w, __uint_as_float(v.y), a[1]);
-    a[2] = fmaf(w, __uint_as_float(v.z), a[2]);
-    a[3] = fmaf(w, __uint_as_float(v.w), a[3]);
+    const int place = p.place[token * top_k + j];
+    if (place < 0) continue;
+    const int n = tile_parts(p, place, share, c / moe::TILE);
+    a = fmaf(weights[token * top_k + j], part_sum(p, place, used, n, c), a);
   }
   const size_t at = (size_t)token * hidden + c;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[at + i] = addend ? addend[at + i] + a[i] : a[i];
+  y[at] = addend ? addend[at] + a : a;
 }
 
 uint64_t moe_route_scratch_bytes(uint64_t, uint64_t, uint64_t) { return 0; }
 
-// The products' scratch: x and h in packets with their run factors, the slots'
-// outputs.
+static int current_sms() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return device_sms(dev);
+}
+
+// Tokens of one expert in a pass over its rows: m is the most it can have.
+static int pass_tokens(int fmt, uint64_t m) {
+  const int t = m <= 8 ? 8 : m <= 16 ? 16 : 32;
+  return t < moe::max_tokens(fmt) ? t : moe::max_tokens(fmt);
+}
+
+static cudaError_t moe_product(int fmt, const moe::Args *a, int tokens, int sms, int *ctas_per_sm,
+                               cudaStream_t stream) {
+  switch (fmt) {
+    case Q4_K: return launch_moe_product<Q4_K>(a, tokens, sms, ctas_per_sm, stream);
+    case Q5_K: return launch_moe_product<Q5_K>(a, tokens, sms, ctas_per_sm, stream);
+    case Q6_K: return launch_moe_product<Q6_K>(a, tokens, sms, ctas_per_sm, stream);
+    case Q8_0: return launch_moe_product<Q8_0>(a, tokens, sms, ctas_per_sm, stream);
+    case IQ4_NL: return launch_moe_product<IQ4_NL>(a, tokens, sms, ctas_per_sm, stream);
+    default: return launch_moe_product<Q4_0>(a, tokens, sms, ctas_per_sm, stream);
+  }
+}
+
+// Result rows of a product: parts times used slots.  A tile is cut into more
+// than two parts only where few passes share the CTAs: P parts need a share
+// below nb / (P - 2) stages, so passes below ctas / (tiles (P - 2)).
+static uint64_t part_rows(uint64_t slots, uint64_t tokens, uint64_t tiles, uint64_t ctas) {
+  uint64_t most = 2 * slots;
+  for (uint64_t P = 3; P <= moe::MAX_PARTS + 1; ++P) {
+    const uint64_t rows = tokens * (ctas / (tiles * (P - 2)) + 1);
+    const uint64_t need = P * (slots < rows ? slots : rows);
+    most = most > need ? most : need;
+  }
+  return most;
+}
+
+// The products' scratch.
 struct MoeScratch {
-  uint64_t x, x_meta, h, h_meta, out, total;
-  MoeScratch(const mgb_experts &ex, uint64_t m, uint64_t top_k) {
+  uint64_t x_hi, x_lo, x_sums, x_scale, h_hi, h_lo, h_sums, h_scale, place[2], share[2], out, total;
+  MoeScratch(const mgb_experts &ex, uint64_t m, uint64_t top_k, int sms) {
     const uint64_t slots = m * top_k;
-    // in order, each 128-byte aligned
     uint64_t at = 0;
-    auto take = [&](uint64_t bytes) {
+    auto take = [&](uint64_t bytes) {  // in order, each 128-byte aligned
       const uint64_t r = at;
       at += (bytes + 127) / 128 * 128;
       return r;
     };
-    x = take(m * ex.hidden * 4);
-    x_meta = take(m * (ex.hidden / RUN) * 8);
-    h = take(slots * ex.ffn * 4);
-    h_meta = take(slots * (ex.ffn / RUN) * 8);
-    out = take(slots * ex.hidden * 4);
+    x_hi = take(m * ex.hidden * 2);
+    x_lo = take(m * ex.hidden * 2);
+    x_sums = take(m * (ex.hidden / 256) * 32);
+    x_scale = take(m * 4);
+    h_hi = take(slots * ex.ffn * 2);
+    h_lo = take(slots * ex.ffn * 2);
+    h_sums = take(slots * (ex.ffn / 256) * 32);
+    h_scale = take(slots * 4);
+    for (int i = 0; i < 2; ++i) place[i] = take(slots * 4), share[i] = take(8);
+    // the second product's results take the first one's place
+    auto rows = [&](int fmt, uint64_t tiles) {
+      const int tokens = pass_tokens(fmt, m);
+      int per_sm = 0;
+      moe_product(fmt, nullptr, tokens, sms, &per_sm, nullptr);
+      return part_rows(slots, tokens, tiles, (uint64_t)sms * per_sm);
+    };
+    const uint64_t a = rows(ex.gate_up_format, 2 * ceil_div(ex.ffn, moe::TILE)) * 2 * ex.ffn;
+    const uint64_t b = rows(ex.down_format, ceil_div(ex.hidden, moe::TILE)) * ex.hidden;
+    out = take((a > b ? a : b) * 4);
     total = at;
+  }
+  moe::Packed16 x(uint8_t *ws) const {
+    return {reinterpret_cast<__half *>(ws + x_hi), reinterpret_cast<__half *>(ws + x_lo),
+            reinterpret_cast<__half *>(ws + x_sums), reinterpret_cast<float *>(ws + x_scale)};
+  }
+  moe::Packed16 h(uint8_t *ws) const {
+    return {reinterpret_cast<__half *>(ws + h_hi), reinterpret_cast<__half *>(ws + h_lo),
+            reinterpret_cast<__half *>(ws + h_sums), reinterpret_cast<float *>(ws + h_scale)};
   }
 };
 
 uint64_t moe_experts_scratch_bytes(const mgb_experts &ex, uint64_t m, uint64_t top_k) {
-  return MoeScratch(ex, m, top_k).total;
+  return m ? MoeScratch(ex, m, top_k, current_sms()).total : 0;
 }
 
 template <typename... P, typename... A>
-static cudaError_t launch_chained(void (*kern)(P...), dim3 grid, dim3 block, cudaStream_t stream,
-                                  A... args) {
+static cudaError_t launch_chained(void (*kern)(P...), dim3 grid, dim3 block, uint32_t smem,
+                                  cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -196,100 +328,73 @@ cudaError_t launch_moe_route(const float *router, uint64_t experts, uint64_t hid
                              float scale, float *ids, float *weights, const mgb_experts *pack_for,
                              void *workspace, cudaStream_t stream) {
   if (!m) return cudaSuccess;
-  uint8_t *packets = nullptr;
-  float2 *meta = nullptr;
-  int fmt = 0;
-  if (pack_for) {  // the products of mgb_moe_layer follow, with this workspace
-    const MoeScratch s(*pack_for, m, top_k);
-    packets = static_cast<uint8_t *>(workspace) + s.x;
-    meta = reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + s.x_meta);
-    fmt = pack_for->gate_up_format;
-  }
-  return launch_chained(mgb_moe_route_kernel, dim3((unsigned)m * ROUTE_CTAS), dim3(ROUTE_THREADS),
+  moe::Packed16 packed = {};
+  if (pack_for)  // the products of mgb_moe_layer follow, with this workspace
+    packed = MoeScratch(*pack_for, m, top_k, current_sms()).x(static_cast<uint8_t *>(workspace));
+  return launch_chained(mgb_moe_route_kernel, dim3((unsigned)m * ROUTE_CTAS), dim3(ROUTE_THREADS), 0,
                         stream, router, (int)experts, (int)hidden, x, (int)top_k, normalize, scale,
-                        ids, weights, fmt, packets, meta);
-}
-
-static cudaError_t moe_product(int fmt, const moe::Args &a, bool gate_up, int nt, int sms,
-                               cudaStream_t stream) {
-  switch (fmt) {
-    case Q4_K: return launch_moe_product<Q4_K>(a, gate_up, nt, sms, stream);
-    case Q5_K: return launch_moe_product<Q5_K>(a, gate_up, nt, sms, stream);
-    case Q6_K: return launch_moe_product<Q6_K>(a, gate_up, nt, sms, stream);
-    case Q8_0: return launch_moe_product<Q8_0>(a, gate_up, nt, sms, stream);
-    case IQ4_NL: return launch_moe_product<IQ4_NL>(a, gate_up, nt, sms, stream);
-    default: return launch_moe_product<Q4_0>(a, gate_up, nt, sms, stream);
-  }
-}
-
-// Warps that share a tile's columns: as many as there are stages of a row (every
-// warp then streams its own piece of it), and more, one of them idle, where the
-// tiles would not cover the SMs.
-static int column_slices(int fmt, int rows, int cols, int row_unit, int most, uint64_t slots,
-                         int experts, int sms) {
-  const int stage = fmt == Q4_K || fmt == Q4_0 || fmt == IQ4_NL ? 256 : 128;
-  const int stages = (cols + stage - 1) / stage;
-  const uint64_t used = slots < (uint64_t)experts ? slots : (uint64_t)experts;
-  int ks = 1;
-  while (ks < most) {
-    const uint64_t tiles = used * ceil_div(rows, row_unit * (moe::WARPS / ks));
-    if (ks * 2 <= stages || (ks < stages && tiles < (uint64_t)sms)) ks *= 2;
-    else break;
-  }
-  return ks;
+                        ids, weights, pack_for != nullptr, pack_for ? pack_for->gate_up_format : 0,
+                        packed);
 }
 
 cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m, const float *ids,
                                const float *weights, uint64_t top_k, const float *addend, float *y,
-                               uint32_t *bad, void *workspace, bool packed, cudaStream_t stream) {
+                               uint32_t *bad, void *workspace, bool packed, int *err,
+                               cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   if (bad) e = cudaMemsetAsync(bad, 0xFF, sizeof(uint32_t), stream);
   if (e != cudaSuccess || !m) return e;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int sms = device_sms(dev);
-  const MoeScratch s(ex, m, top_k);
+  const int sms = current_sms();
+  const MoeScratch s(ex, m, top_k, sms);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   const int hidden = (int)ex.hidden, ffn = (int)ex.ffn, slots = (int)(m * top_k);
-  // tokens of one expert in a pass over its rows: m is the most it can have
-  const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
   if (!packed) {
-    e = launch_chained(mgb_moe_pack_kernel, dim3((unsigned)ceil_div(hidden / RUN, 8), (unsigned)m),
-                       dim3(256), stream, ex.gate_up_format, x, hidden, ws + s.x,
-                       reinterpret_cast<float2 *>(ws + s.x_meta));
+    e = launch_chained(mgb_moe_pack_kernel, dim3((unsigned)ceil_div(hidden / RUN, 32), (unsigned)m),
+                       dim3(256), 0, stream, ex.gate_up_format, x, hidden, s.x(ws));
     if (e != cudaSuccess) return e;
   }
   moe::Args a = {};
   a.w0 = static_cast<const uint8_t *>(ex.gate);
   a.w1 = static_cast<const uint8_t *>(ex.up);
-  a.packets = ws + s.x;
-  a.meta = reinterpret_cast<const float2 *>(ws + s.x_meta);
+  a.act = s.x(ws);
   a.ids = ids;
-  a.h_packets = ws + s.h;
-  a.h_meta = reinterpret_cast<float2 *>(ws + s.h_meta);
+  a.out = reinterpret_cast<float *>(ws + s.out);
+  a.place = reinterpret_cast<int32_t *>(ws + s.place[0]);
+  a.share = reinterpret_cast<int32_t *>(ws + s.share[0]);
   a.bad = bad;
+  a.err = err;
   a.experts = (int)ex.experts;
+  a.matrices = 2;
   a.rows = ffn;
   a.cols = hidden;
   a.slots = slots;
   a.act_div = (int)top_k;
-  a.ks = column_slices(ex.gate_up_format, ffn, hidden, 16, 8, slots, a.experts, sms);
-  a.down_fmt = ex.down_format;
-  e = moe_product(ex.gate_up_format, a, true, nt, sms, stream);
+  e = moe_product(ex.gate_up_format, &a, pass_tokens(ex.gate_up_format, m), sms, nullptr, stream);
+  if (e != cudaSuccess) return e;
+  const Parts gu{a.out, a.place, a.share, 2 * (int)ceil_div(ffn, moe::TILE), (int)ceil_div(hidden, moe::stage_cols(ex.gate_up_format)), 2 * ffn};
+  const uint32_t h_smem = (uint32_t)ceil_div(ffn / RUN, H_CTAS) * RUN * 4;
+  if (h_smem > 48 * 1024) {
+    e = cudaFuncSetAttribute(mgb_moe_h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h_smem);
+    if (e != cudaSuccess) return e;
+  }
+  e = launch_chained(mgb_moe_h_kernel, dim3((unsigned)slots * H_CTAS), dim3(H_THREADS), h_smem, stream, gu,
+                     ffn, ex.down_format, s.h(ws));
   if (e != cudaSuccess) return e;
   a.w0 = a.w1 = static_cast<const uint8_t *>(ex.down);
-  a.packets = ws + s.h;
-  a.meta = reinterpret_cast<const float2 *>(ws + s.h_meta);
-  a.out = reinterpret_cast<float *>(ws + s.out);
+  a.act = s.h(ws);
+  a.place = reinterpret_cast<int32_t *>(ws + s.place[1]);
+  a.share = reinterpret_cast<int32_t *>(ws + s.share[1]);
+  a.bad = nullptr;
+  a.matrices = 1;
   a.rows = hidden;
   a.cols = ffn;
   a.act_div = 1;
-  a.ks = column_slices(ex.down_format, hidden, ffn, 32, 16, slots, a.experts, sms);
-  e = moe_product(ex.down_format, a, false, nt, sms, stream);
+  e = moe_product(ex.down_format, &a, pass_tokens(ex.down_format, m), sms, nullptr, stream);
   if (e != cudaSuccess) return e;
-  return launch_chained(mgb_moe_combine_kernel, dim3((unsigned)ceil_div(hidden, 1024), (unsigned)m),
-                        dim3(256), stream, static_cast<const float *>(a.out), ids, weights,
-                        a.experts, hidden, (int)top_k, addend, y);
+  const Parts dn{a.out, a.place, a.share, (int)ceil_div(hidden, moe::TILE), 
+                 (int)ceil_div(ffn, moe::stage_cols(ex.down_format)), hidden};
+  return launch_chained(mgb_moe_combine_kernel, dim3((unsigned)ceil_div(hidden, 256), (unsigned)m),
+                        dim3(256), 0, stream, dn, weights, hidden, (int)top_k, addend, y);
 }
 
 }  // namespace mgb

@@ -1,18 +1,36 @@
 // Launches of the packed expert products of one format.
 #pragma once
 
+#include <atomic>
+
 #include "experts.cuh"
 
 namespace mgb {
 
-template <int FMT, bool GATE_UP, int NT>
-static cudaError_t launch_moe_one(const moe::Args &a, int sms, cudaStream_t stream) {
-  const uint32_t smem = moe::WARPS * moe::warp_bytes<FMT>() + moe::plan_bytes(a.experts, a.slots);
-  auto *kern = moe::mgb_moe_product_kernel<FMT, GATE_UP, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <int FMT, int T>
+static cudaError_t launch_moe_one(const moe::Args *args, int sms, int *ctas_per_sm,
+                                  cudaStream_t stream) {
+  using X = moe::Shape<FMT, T>;
+  if (ctas_per_sm) *ctas_per_sm = X::CTAS;
+  if (!args) return cudaSuccess;
+  const moe::Args &a = *args;
+  auto *kern = moe::mgb_moe_product_kernel<FMT, T>;
+  // at least what keeps CTAs for which there is no TMEM off the SM
+  uint32_t smem = X::FIXED + moe::plan_bytes(a.experts, a.slots);
+  constexpr uint32_t least = 228 * 1024 / (512 / X::TMEM + 1);
+  if (smem < least) smem = least;
+  // the opt-in is an attribute of the function on a device: once each
+  static std::atomic<uint64_t> opted{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (!(opted.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+    if (e != cudaSuccess) return e;
+    opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)sms);
+  cfg.gridDim = dim3((unsigned)(sms * X::CTAS));
   cfg.blockDim = dim3(moe::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -25,15 +43,12 @@ static cudaError_t launch_moe_one(const moe::Args &a, int sms, cudaStream_t stre
 }
 
 template <int FMT>
-cudaError_t launch_moe_product(const moe::Args &a, bool gate_up, int nt, int sms,
+cudaError_t launch_moe_product(const moe::Args *a, int tokens, int sms, int *ctas_per_sm,
                                cudaStream_t stream) {
-  if (gate_up)
-    return nt == 1   ? launch_moe_one<FMT, true, 1>(a, sms, stream)
-           : nt == 2 ? launch_moe_one<FMT, true, 2>(a, sms, stream)
-                     : launch_moe_one<FMT, true, 4>(a, sms, stream);
-  return nt == 1   ? launch_moe_one<FMT, false, 1>(a, sms, stream)
-         : nt == 2 ? launch_moe_one<FMT, false, 2>(a, sms, stream)
-                   : launch_moe_one<FMT, false, 4>(a, sms, stream);
+  if (tokens == 8) return launch_moe_one<FMT, 8>(a, sms, ctas_per_sm, stream);
+  if constexpr (moe::max_tokens(FMT) > 16)
+    if (tokens == 32) return launch_moe_one<FMT, 32>(a, sms, ctas_per_sm, stream);
+  return launch_moe_one<FMT, 16>(a, sms, ctas_per_sm, stream);
 }
 
 }  // namespace mgb

@@ -79,7 +79,8 @@ cudaError_t launch_moe_route(const float *router, uint64_t experts, uint64_t hid
 // packed: x is in the workspace's packets already (launch_moe_route with pack_for)
 cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m, const float *ids,
                                const float *weights, uint64_t top_k, const float *addend, float *y,
-                               uint32_t *bad, void *workspace, bool packed, cudaStream_t stream);
+                               uint32_t *bad, void *workspace, bool packed, int *err,
+                               cudaStream_t stream);
 
 // sample.cu
 struct SampleArgs {
