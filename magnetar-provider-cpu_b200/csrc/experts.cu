@@ -154,10 +154,27 @@ __device__ __forceinline__ float part_sum(const Parts &p, int place, int used, i
   return s;
 }
 
+// Four values (c and the rows' widths are multiples of 32).
+__device__ __forceinline__ float4 part_sum4(const Parts &p, int place, int used, int n, int c) {
+  const float *at = p.out + (uint64_t)(place & 0xFFFF) * p.width + c;
+  const uint64_t step = (uint64_t)used * p.width;
+  float4 s = *reinterpret_cast<const float4 *>(at);
+  for (int i = 1; i < n; ++i) {
+    const float4 v = *reinterpret_cast<const float4 *>(at + i * step);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  return s;
+}
+
 // h = silu(gate) * up of one slot, packed for the down projection: a cluster per
 // slot, which finds the row's largest magnitude together.
 constexpr int H_CTAS = 8;
-constexpr int H_THREADS = 512;
+constexpr int H_THREADS = 256;
+// Runs of a CTA: whole row tiles.
+__host__ __device__ inline int h_runs(int ffn) {
+  const int per = (ffn / RUN + H_CTAS - 1) / H_CTAS;
+  return (per + 3) & ~3;
+}
 __global__ void __cluster_dims__(H_CTAS, 1, 1) __launch_bounds__(H_THREADS)
     mgb_moe_h_kernel(const Parts p, int ffn, int fmt, moe::Packed16 o) {
   extern __shared__ float h[];  // this CTA's runs
@@ -171,17 +188,23 @@ __global__ void __cluster_dims__(H_CTAS, 1, 1) __launch_bounds__(H_THREADS)
   const int place = p.place[slot];
   if (place < 0) return;  // the whole cluster
   const int share = p.share[0], used = p.share[1];
-  const int runs = ffn / RUN, per = (runs + H_CTAS - 1) / H_CTAS;
+  const int runs = ffn / RUN, per = h_runs(ffn);
   const int r0 = min(runs, rank * per), r1 = min(runs, r0 + per);
   const int tiles1 = p.tiles / 2;
   float mx = 0.f;
-  for (int r = r0 + warp; r < r1; r += H_THREADS / 32) {  // a warp's run lies in one tile
-    const int tile = r * RUN / moe::TILE, f = r * RUN + lane;
+  // a warp's four runs (r0 is a multiple of four) lie in one row tile
+  for (int r = r0 + 4 * warp; r < r1; r += H_THREADS / 8) {
+    const int tile = r * RUN / moe::TILE, f = r * RUN + 4 * lane;
+    if (f >= r1 * RUN) continue;
     const int ng = tile_parts(p, place, share, tile), nu = tile_parts(p, place, share, tiles1 + tile);
-    const float g = part_sum(p, place, used, ng, f), u = part_sum(p, place, used, nu, ffn + f);
-    const float v = g / (1.f + expf(-g)) * u;
-    h[f - r0 * RUN] = v;
-    mx = fmaxf(mx, fabsf(v));
+    const float4 g = part_sum4(p, place, used, ng, f), u = part_sum4(p, place, used, nu, ffn + f);
+    float4 v;
+    v.x = g.x / (1.f + expf(-g.x)) * u.x;
+    v.y = g.y / (1.f + expf(-g.y)) * u.y;
+    v.z = g.z / (1.f + expf(-g.z)) * u.z;
+    v.w = g.w / (1.f + expf(-g.w)) * u.w;
+    *reinterpret_cast<float4 *>(h + f - r0 * RUN) = v;
+    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
@@ -372,7 +395,7 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   e = moe_product(ex.gate_up_format, &a, pass_tokens(ex.gate_up_format, m), sms, nullptr, stream);
   if (e != cudaSuccess) return e;
   const Parts gu{a.out, a.place, a.share, 2 * (int)ceil_div(ffn, moe::TILE), (int)ceil_div(hidden, moe::stage_cols(ex.gate_up_format)), 2 * ffn};
-  const uint32_t h_smem = (uint32_t)ceil_div(ffn / RUN, H_CTAS) * RUN * 4;
+  const uint32_t h_smem = (uint32_t)h_runs(ffn) * RUN * 4;
   if (h_smem > 48 * 1024) {
     e = cudaFuncSetAttribute(mgb_moe_h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h_smem);
     if (e != cudaSuccess) return e;

@@ -115,6 +115,27 @@ __device__ __forceinline__ void grid_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// A bounded wait for phase `parity` that leaves the issue slots to the warps with
+// work: each try suspends the warp for up to half a millisecond (the default
+// limit is so short that the polls of waiting warps took a third of the issue
+// slots).  Gives up, and records it, after about two seconds.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, int *err) {
+  for (int i = 0; i < 4096; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(500000u)
+        : "memory");
+    if (ok) return true;
+    if (err && *(volatile int *)err != 0) return false;
+  }
+  record_error(err, ERR_WAIT_TIMEOUT);
+  return false;
+}
+
 // D[tmem] (+)= A[tmem] (f16, 128 rows x 16) * B[smem] (f16, K-major)
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
@@ -555,7 +576,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
         cp_async_wait<X::B_DEPTH - 2>();
         fence_proxy_async_smem();  // this lane's copies, for the tensor core's reads
         __syncwarp();
-        ok = __all_sync(0xffffffffu, mbar_wait(full, q & 1, p.err));
+        ok = __all_sync(0xffffffffu, wait_phase(full, q & 1, p.err));
         if (!ok) break;
         if (lane == 0) {
           fence_after();
@@ -595,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
     }
     cp_async_wait<0>();
     // the last MMAs have been performed before TMEM goes back
-    if (q > 0) mbar_wait(done, (q - 1) & 1, p.err);
+    if (q > 0) wait_phase(done, (q - 1) & 1, p.err);
     __syncwarp();
   } else {
     // ---------------- weights ----------------
@@ -680,7 +701,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
 
     // waits for step q - 1 and adds its results
     auto collect = [&]() {
-      ok = __all_sync(0xffffffffu, mbar_wait(done, (q - 1) & 1, p.err));
+      ok = __all_sync(0xffffffffu, wait_phase(done, (q - 1) & 1, p.err));
       if (!ok) return;
       fence_after();
       if (KF && !stage_end) return;
