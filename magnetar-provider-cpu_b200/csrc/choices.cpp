@@ -43,7 +43,7 @@ mgb_status check_adapters(const mgb_adapters *ad, uint64_t m) {
     return fail(MGB_INVALID_ARGUMENT, "adapter rank %llu is above %d", (unsigned long long)ad->rank,
                 MGB_MAX_ADAPTER_RANK);
   // ids are f32: whole numbers up to 2^24 are exact
-  if (ad->count > (1u << 24) || m > (1ull << 31) || ad->k > (1u << 30) || ad->n > (1u << 30) ||
+  if (ad->count > (1u << 24) || m > (1u << 24) || ad->k > (1u << 30) || ad->n > (1u << 30) ||
       too_large(ad->count, ad->rank, ad->k) || too_large(ad->count, ad->rank, ad->n) ||
       too_large(m, ad->k) || too_large(m, ad->n))
     return fail(MGB_INVALID_ARGUMENT, "adapter sizes are too large");
