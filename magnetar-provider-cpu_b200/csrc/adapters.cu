@@ -6,18 +6,20 @@
 // and then an eighth of the outputs (two chained launches cost one row 9.8 us
 // against PLACEHOLDER).
 //
-// Rows are grouped by adapter into tiles of up to 16, the M of mma.sync
-// m16n8k8 (tf32 operands, f32 accumulation), so that an adapter is read once
-// for its rows whatever their order, and one row alone costs no more than its
-// adapter's bytes.  The products are bound by those bytes or, with many rows,
-// by base and y; arithmetic intensity never exceeds a few hundred operations a
-// byte, far from what tcgen05 is for.
+// Rows are grouped by adapter into tiles of up to 64, so that an adapter is read
+// once for its rows whatever their order, and one row alone costs no more than
+// its adapter's bytes.  16 rows are the M of mma.sync m16n8k8 (tf32 operands, f32
+// accumulation).  The products are bound by the adapters' bytes or, with many
+// rows, by base and y: rank operations a value, far from what tcgen05 is for.
 //
 // f32 accuracy from tf32: x and h are held as hi + lo, two tf32 terms (22 bits);
 // f16 and bf16 factors are tf32 numbers as they are, f32 factors are split too.
 // The order of a product's K is free, so a lane takes runs of neighbouring
 // values of its row: every load is 16 bytes where the buffers allow it.
 #include <cooperative_groups.h>
+
+#include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -27,7 +29,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int ROWS = 16;          // of a tile
+constexpr int M = 16;             // rows of an MMA
+constexpr int MOST_ROWS = 64;     // of a tile
 constexpr int INLINE_ROWS = 128;  // up to here every CTA plans for itself
 constexpr int BUCKETS = 4096;     // of the planning kernel's sort
 constexpr int CTAS = 8;           // of a cluster
@@ -54,6 +57,7 @@ struct Params {
   uint32_t *bad;
   uint64_t count;
   int m, k, n, rank;
+  int tile_rows;     // rows of a tile: 16, 32 or 64
   bool wide_a, wide_b, wide_x, wide_y;  // 16-byte loads are aligned
 };
 
@@ -72,7 +76,7 @@ struct SmallPlan {
   int ntiles;
 };
 
-// Rows sorted by (id, row), tiles of up to 16 rows of one id.
+// Rows sorted by (id, row), tiles of up to tile_rows rows of one id.
 __device__ void plan_small(const Params &p, SmallPlan &s, bool report) {
   const int i = threadIdx.x;
   if (i == 0) s.ntiles = 0;
@@ -95,14 +99,14 @@ __device__ void plan_small(const Params &p, SmallPlan &s, bool report) {
       same += o == id;
     }
     s.order[pos] = (int16_t)i;
-    s.head[pos] = nth % ROWS == 0;
+    s.head[pos] = nth % p.tile_rows == 0;
   }
   __syncthreads();
-  if (i < p.m && nth % ROWS == 0) {
+  if (i < p.m && nth % p.tile_rows == 0) {
     int t = 0;
     for (int j = 0; j < pos; ++j) t += s.head[j];
-    s.tiles[t] = Tile{pos, min(ROWS, same - nth), id};
-    if (pos + min(ROWS, same - nth) == p.m) s.ntiles = t + 1;
+    s.tiles[t] = Tile{pos, min(p.tile_rows, same - nth), id};
+    if (pos + min(p.tile_rows, same - nth) == p.m) s.ntiles = t + 1;
   }
   __syncthreads();
 }
@@ -128,7 +132,7 @@ __device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {  
 }
 
 // One CTA: rows by bucket (the adapter, modulo 4,095; the last bucket holds the
-// rows without one), then tiles of up to 16 neighbours of one adapter.  Which
+// rows without one), then tiles of up to tile_rows neighbours of one adapter.  Which
 // tile a row lands in does not affect its result.
 __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) {
   __shared__ int at[BUCKETS];
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
   __syncthreads();
   for (int r = threadIdx.x; r < p.m; r += 1024) p.order[atomicAdd(&at[bucket(id_of(r))], 1)] = r;
   __syncthreads();
-  // run heads, then tile heads (every 16th of a run)
+  // run heads, then tile heads (every tile_rows-th row of a run)
   if (threadIdx.x == 0) s_carry[0] = 0, s_carry[1] = 0;
   __syncthreads();
   for (int p0 = 0; p0 < p.m; p0 += 1024) {
@@ -180,7 +184,7 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
     __syncthreads();
     for (int w = 0; w < warp; ++w) start = max(start, sums[w]);
     start = max(start, s_carry[0]);
-    const bool tile = i < p.m && (i - start) % ROWS == 0;
+    const bool tile = i < p.m && (i - start) % p.tile_rows == 0;
     int total;
     const int t = s_carry[1] + block_scan(tile, sums, total);
     __syncthreads();
@@ -197,13 +201,13 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
 
 // The CTA's tile and its rows (row[i] of lanes' tokens, absent ones repeat the
 // first); false: no such tile.
-__device__ __forceinline__ bool find_tile(const Params &p, int t, SmallPlan &plan, int (&rows)[ROWS],
+__device__ __forceinline__ bool find_tile(const Params &p, int t, SmallPlan &plan, int (&rows)[MOST_ROWS],
                                           bool report, Tile &tile) {
   const bool small = p.m <= INLINE_ROWS;
   if (small) plan_small(p, plan, report);
   if (t >= (small ? plan.ntiles : *p.ntiles)) return false;
   tile = small ? plan.tiles[t] : p.tiles[t];
-  if (threadIdx.x < ROWS) {
+  if (threadIdx.x < MOST_ROWS) {
     const int i = tile.start + (threadIdx.x < tile.len ? threadIdx.x : 0);
     rows[threadIdx.x] = small ? plan.order[i] : p.order[i];
   }
@@ -277,37 +281,97 @@ __device__ __forceinline__ void load_values(const T *at, int left, bool wide, fl
   }
 }
 
+// N neighbouring values in pairs as they are stored (16-bit types), or one by one.
+template <typename T, int N>
+struct Pairs {
+  static constexpr int REGS = sizeof(T) == 4 ? N : N / 2;
+  uint32_t r[REGS];
+  __device__ __forceinline__ void load(const T *at, int left, bool wide) {
+    if (wide && left >= N) {
+      if constexpr (REGS >= 4) {
+#pragma unroll
+        for (int i = 0; i < REGS / 4; ++i) {
+          const uint4 v = reinterpret_cast<const uint4 *>(at)[i];
+          r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
+        }
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(at);
+        r[0] = v.x, r[1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < REGS; ++i) r[i] = 0;
+      T *d = reinterpret_cast<T *>(r);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) d[i] = at[i];
+    }
+  }
+  // values 2 s and 2 s + 1
+  __device__ __forceinline__ float2 pair(int s) const {
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(r[2 * s]), __uint_as_float(r[2 * s + 1]));
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return make_float2(__uint_as_float(r[s] << 16), __uint_as_float(r[s] & 0xFFFF0000u));
+    else return __half22float2(*reinterpret_cast<const __half2 *>(&r[s]));
+  }
+};
+
 // ---- the kernel --------------------------------------------------------------------------------
-//
-// RC: ranks of a pass (a lane of the second product: RC / 4 neighbours, K of
-// RC / 8 MMAs).  Shared memory: the warps' sums of a pass, then the whole h
-// (`red`), and this CTA's part of h (`part`).
-template <int RC>
-__host__ __device__ constexpr uint32_t red_floats() {
-  return WARPS * ROWS * (RC + 4);
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// RC: ranks of a pass (a lane of the second product: RC / 4 neighbours, K of
+// RC / 8 MMAs).  Shared memory: h as MMA operands (hi and lo, [rows / 16][ranks /
+// 8][lane][4]), then in turn this CTA's part of h ([rows][ranks + 4]) and, where
+// the buffers allow 16-byte copies (WIDE), a ring of B's rows for every warp.
 template <typename T, int RC>
-__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, 2)
+struct Shared {
+  static constexpr uint32_t ROW = RC * sizeof(T) + 16;  // neighbouring rows in different banks
+  static constexpr uint32_t STAGE = COLS * ROW;
+  static constexpr int DEPTH = 2;
+  static constexpr uint32_t RING = WARPS * DEPTH * STAGE;
+};
+__host__ __device__ inline int h_width(int rank, int rc) { return (rank + rc - 1) / rc * rc; }
+__host__ __device__ inline uint32_t h_bytes(int tile_rows, int width) { return tile_rows * width * 8; }
+__host__ __device__ inline uint32_t part_bytes(int tile_rows, int width) {
+  return tile_rows * (width + 4) * 4;
+}
+
+template <typename T, int RC, bool WIDE>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
     mgb_adapter_kernel(const Params p) {
-  extern __shared__ __align__(16) float red[];
+  using SM = Shared<T, RC>;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ SmallPlan plan;
-  __shared__ int rows[ROWS];
+  __shared__ int rows[MOST_ROWS];
   cg::cluster_group cluster = cg::this_cluster();
   const int cta = (int)cluster.block_rank();
-  const int width = (p.rank + RC - 1) / RC * RC;  // ranks in whole passes
-  float *part = red + max(red_floats<RC>(), (uint32_t)ROWS * (width + 4));  // [ROWS][width]
+  const int width = h_width(p.rank, RC), stride = width + 4;
+  uint4 *hs = reinterpret_cast<uint4 *>(smem);  // [rows / 16][width / 8][hi, lo][lane]
+  float *part = reinterpret_cast<float *>(smem + h_bytes(p.tile_rows, width));
   grid_wait();
   grid_dependents();
   Tile tile;
   // (the whole cluster has one tile)
   if (!find_tile(p, blockIdx.x / CTAS, plan, rows, blockIdx.x == 0, tile)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int mts = (tile.len + M - 1) / M;  // blocks of 16 rows
 
-  // h = s A x: this CTA's eighth of k, in groups of 32 that its warps take in turn
   if (tile.id >= 0) {
+    // h = s A x.  This CTA's eighth of k in groups of 32; a warp takes one block of
+    // rows (of 1, 2 or 4) and every kparts-th group
+    const int split_m = mts > 2 ? 4 : mts, kparts = WARPS / split_m;
+    const int mt = warp % split_m, kp = warp / split_m;
     const T *a = static_cast<const T *>(p.a) + (uint64_t)tile.id * p.rank * p.k;
-    const float *x0 = p.x + (uint64_t)rows[g] * p.k, *x1 = p.x + (uint64_t)rows[g + 8] * p.k;
+    const float *x0 = p.x + (uint64_t)rows[mt * M + g] * p.k, *x1 = p.x + (uint64_t)rows[mt * M + g + 8] * p.k;
     const int groups = (p.k + 31) / 32, per = (groups + CTAS - 1) / CTAS;
     const int g0 = min(groups, cta * per), g1 = min(groups, g0 + per);
     for (int r0 = 0; r0 < p.rank; r0 += RC) {
@@ -316,144 +380,220 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, 2)
       for (int n = 0; n < RC / 8; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-      for (int q = g0 + warp; q < g1; q += WARPS) {
-        const int k0 = q * 32 + t * 8, left = p.k - k0;  // this lane's 8 values: K of four MMAs
-        float v0[8], v1[8];
-        load_values<8>(x0 + k0, left, p.wide_x, v0);
-        load_values<8>(x1 + k0, left, p.wide_x, v1);
-        uint32_t hi[4][4], lo[4][4];
+      if (mt < mts)
+        for (int q = g0 + kp; q < g1; q += kparts) {
+          const int k0 = q * 32 + t * 8, left = p.k - k0;  // this lane's 8 values: K of four MMAs
+          float v0[8], v1[8];
+          load_values<8>(x0 + k0, left, p.wide_x, v0);
+          load_values<8>(x1 + k0, left, p.wide_x, v1);
+          uint32_t hi[4][4], lo[4][4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          split(v0[2 * s], hi[s][0], lo[s][0]);
-          split(v1[2 * s], hi[s][1], lo[s][1]);
-          split(v0[2 * s + 1], hi[s][2], lo[s][2]);
-          split(v1[2 * s + 1], hi[s][3], lo[s][3]);
+          for (int s = 0; s < 4; ++s) {
+            split(v0[2 * s], hi[s][0], lo[s][0]);
+            split(v1[2 * s], hi[s][1], lo[s][1]);
+            split(v0[2 * s + 1], hi[s][2], lo[s][2]);
+            split(v1[2 * s + 1], hi[s][3], lo[s][3]);
+          }
+#pragma unroll
+          for (int n = 0; n < RC / 8; ++n) {
+            const int r = r0 + n * 8 + g;
+            if (r0 + n * 8 >= p.rank) break;
+            float w[8];
+            load_values<8>(a + (uint64_t)min(r, p.rank - 1) * p.k + k0, r < p.rank ? left : 0, p.wide_a, w);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) multiply<T>(acc[n], hi[s], lo[s], w[2 * s], w[2 * s + 1]);
+          }
         }
+      // the warps' sums, in order
+      for (int k = 0; k < kparts; ++k) {
+        if (kp == k && mt < mts)
 #pragma unroll
-        for (int n = 0; n < RC / 8; ++n) {
-          const int r = r0 + n * 8 + g;
-          if (r0 + n * 8 >= p.rank) break;
-          float w[8];
-          load_values<8>(a + (uint64_t)min(r, p.rank - 1) * p.k + k0, r < p.rank ? left : 0, p.wide_a, w);
+          for (int n = 0; n < RC / 8; ++n)
 #pragma unroll
-          for (int s = 0; s < 4; ++s) multiply<T>(acc[n], hi[s], lo[s], w[2 * s], w[2 * s + 1]);
-        }
+            for (int i = 0; i < 4; ++i) {
+              float *at = part + (mt * M + g + 8 * (i >> 1)) * stride + r0 + n * 8 + 2 * t + (i & 1);
+              *at = k ? *at + acc[n][i] : acc[n][i];
+            }
+        __syncthreads();
       }
-#pragma unroll
-      for (int n = 0; n < RC / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          red[(warp * ROWS + g + 8 * (i >> 1)) * (RC + 4) + n * 8 + 2 * t + (i & 1)] = acc[n][i];
-      __syncthreads();
-      for (int i = threadIdx.x; i < ROWS * RC; i += 32 * WARPS) {
-        const int row = i / RC, c = i % RC;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) s += red[(w * ROWS + row) * (RC + 4) + c];
-        part[row * width + r0 + c] = s;
-      }
-      __syncthreads();
     }
     cluster.sync();
-    // the whole h, summed over the CTAs in order, in `red` ([ROWS][width + 4])
+    // the whole h, summed over the CTAs in order, as operands: lane (g, t) of step
+    // 8 q + s multiplies ranks q RC + t RC / 4 + 2 s and the next
     const float scale = p.scales ? p.scales[tile.id] : 1.f;
-    for (int i = threadIdx.x; i < ROWS * width; i += 32 * WARPS) {
-      float v[CTAS], s = 0.f;
+    const int steps = width / 8;
+    for (int i = threadIdx.x; i < mts * steps * 32; i += 32 * WARPS) {
+      const int l = i & 31, step = (i >> 5) % steps, b = (i >> 5) / steps;
+      const int r = step / (RC / 8) * RC + (l & 3) * (RC / 4) + 2 * (step % (RC / 8));
+      const float *at = part + (b * M + (l >> 2)) * stride + r;
+      float2 v0 = make_float2(0.f, 0.f), v1 = v0;
 #pragma unroll
-      for (int c = 0; c < CTAS; ++c) v[c] = cluster.map_shared_rank(part, c)[i];
-#pragma unroll
-      for (int c = 0; c < CTAS; ++c) s += v[c];
-      red[i / width * (width + 4) + i % width] = s * scale;
+      for (int c = 0; c < CTAS; ++c) {
+        const float *o = cluster.map_shared_rank(at, c);
+        const float2 u0 = *reinterpret_cast<const float2 *>(o), u1 = *reinterpret_cast<const float2 *>(o + 8 * stride);
+        v0.x += u0.x, v0.y += u0.y, v1.x += u1.x, v1.y += u1.y;
+      }
+      uint4 hi, lo;
+      split(v0.x * scale, hi.x, lo.x);
+      split(v1.x * scale, hi.y, lo.y);
+      split(v0.y * scale, hi.z, lo.z);
+      split(v1.y * scale, hi.w, lo.w);
+      hs[(b * steps + step) * 64 + l] = hi;
+      hs[(b * steps + step) * 64 + 32 + l] = lo;
     }
-    __syncthreads();
-    cluster.barrier_arrive();  // (waited for before this CTA's part may go)
+    cluster.sync();  // h is complete, and no CTA reads another's part any more
   }
 
   // y = base + B h: blocks of 32 outputs.  A warp's four MMA column blocks are
-  // interleaved so that a lane ends up with 8 neighbouring outputs of a row.
-  constexpr int PER = RC / 4, STEPS = RC / 8;
+  // interleaved so that a lane ends up with 8 neighbouring outputs of a row: column
+  // g of block n is output 8 (g / 2) + 2 n + g % 2.
+  constexpr int PER = RC / 4, STEPS = RC / 8, CHUNKS = RC * sizeof(T) / 16, NEXT = CTAS * WARPS * COLS;
   const T *b = static_cast<const T *>(p.b) + (uint64_t)max(tile.id, 0) * p.n * p.rank;
-  uint32_t hi[STEPS][4], lo[STEPS][4];
-  auto load_h = [&](int r0) {
-    const float *h0 = red + g * (width + 4) + r0 + t * PER, *h1 = h0 + 8 * (width + 4);
+  const int passes = tile.id >= 0 ? width / RC : 0, steps = width / 8;
+  uint8_t *ring = smem + h_bytes(p.tile_rows, width) + warp * SM::DEPTH * SM::STAGE;
+  // WIDE: a warp's copies of B (a pass of a block a stage) run DEPTH ahead
+  int fc = (cta * WARPS + warp) * COLS, fp = 0, fslot = 0, slot = 0;
+  auto fetch = [&]() {
+    if (fc < p.n && passes) {
+      uint8_t *st = ring + fslot * SM::STAGE;
+      const int have = (p.rank - fp * RC) * (int)sizeof(T);  // bytes of a row in this pass
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      split(h0[2 * s], hi[s][0], lo[s][0]);
-      split(h1[2 * s], hi[s][1], lo[s][1]);
-      split(h0[2 * s + 1], hi[s][2], lo[s][2]);
-      split(h1[2 * s + 1], hi[s][3], lo[s][3]);
-    }
-  };
-  if (tile.id >= 0 && p.rank <= RC) load_h(0);
-  for (int c0 = (cta * WARPS + warp) * COLS; c0 < p.n; c0 += CTAS * WARPS * COLS) {
-    // lane (g, t) ends with rows g and g + 8, outputs c0 + 8 t .. + 7
-    const int c = c0 + 8 * t;
-    const bool wide = p.wide_y && c + 8 <= p.n;
-    float4 old[2][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (wide && p.base && g + 8 * h < tile.len)
-          old[h][q] = *reinterpret_cast<const float4 *>(p.base + (uint64_t)rows[g + 8 * h] * p.n + c + 4 * q);
-        else old[h][q] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float acc[4][4];
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-    if (tile.id >= 0)
-      for (int r0 = 0; r0 < p.rank; r0 += RC) {
-        if (p.rank > RC) load_h(r0);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          // MMA column g of block n: the outputs 8 (g / 2) + 2 n + g % 2
-          const int col = c0 + 8 * (g >> 1) + 2 * n + (g & 1);
-          float w[PER];
-          load_values<PER>(b + (uint64_t)min(col, p.n - 1) * p.rank + r0 + t * PER,
-                           col < p.n ? p.rank - r0 - t * PER : 0, p.wide_b, w);
-#pragma unroll
-          for (int s = 0; s < STEPS; ++s) multiply<T>(acc[n], hi[s], lo[s], w[2 * s], w[2 * s + 1]);
-        }
+      for (int i = 0; i < CHUNKS; ++i) {
+        const int q = i * 32 + lane, row = q / CHUNKS, c = q % CHUNKS;
+        const bool in = c * 16 < have;  // (zeros behind the last rank)
+        if (fc + row < p.n)
+          cp_async16(st + row * SM::ROW + c * 16,
+                     reinterpret_cast<const uint8_t *>(b + (uint64_t)(fc + row) * p.rank + fp * RC) +
+                         (in ? c * 16 : 0), in ? 16 : 0);
       }
+      fslot = fslot + 1 == SM::DEPTH ? 0 : fslot + 1;
+      if (++fp == passes) fp = 0, fc += NEXT;
+    }
+    cp_async_commit();
+  };
+  if (WIDE)
+#pragma unroll
+    for (int i = 0; i < SM::DEPTH; ++i) fetch();
+  // base (after the first pass: y) of lane (g, t)'s outputs c .. c + 7, c = c0 + 8 t,
+  // of rows g and g + 8 of a block of rows; loaded one block ahead
+  struct Old {
+    float v[2][8];
+  };
+  auto load_old = [&](Old &o, int c0, int q, int mt) {
+    const float *from = q ? p.y : p.base;
+    const int c = c0 + 8 * t;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = g + 8 * h;
-      if (row >= tile.len || c >= p.n) continue;
-      const uint64_t at = (uint64_t)rows[row] * p.n + c;
-      float v[8];
+      const int row = mt * M + g + 8 * h;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) v[2 * n] = acc[n][2 * h], v[2 * n + 1] = acc[n][2 * h + 1];
-      if (wide) {
+      for (int i = 0; i < 8; ++i) o.v[h][i] = 0.f;
+      if (!from || row >= tile.len) continue;
+      const float *at = from + (uint64_t)rows[row] * p.n + c;
+      if (p.wide_y && c + 8 <= p.n) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const float4 s = old[h][q];
-          *reinterpret_cast<float4 *>(p.y + at + 4 * q) =
-              tile.id < 0 ? s
-                          : make_float4(s.x + v[4 * q], s.y + v[4 * q + 1], s.z + v[4 * q + 2], s.w + v[4 * q + 3]);
+        for (int i = 0; i < 2; ++i) {
+          const float4 v = *reinterpret_cast<const float4 *>(at + 4 * i);
+          o.v[h][4 * i] = v.x, o.v[h][4 * i + 1] = v.y, o.v[h][4 * i + 2] = v.z, o.v[h][4 * i + 3] = v.w;
         }
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c + i < p.n) {
-            const float s = p.base ? p.base[at + i] : 0.f;
-            p.y[at + i] = tile.id < 0 ? s : s + v[i];
+          if (c + i < p.n) o.v[h][i] = at[i];
+      }
+    }
+  };
+  Old next;
+  int c0 = (cta * WARPS + warp) * COLS;
+  if (c0 < p.n) load_old(next, c0, 0, 0);
+  for (; c0 < p.n; c0 += NEXT) {
+    const int c = c0 + 8 * t;
+    const bool wide = p.wide_y && c + 8 <= p.n;
+    for (int q = 0; q < max(passes, 1); ++q) {
+      Pairs<T, PER> w[4];
+      if (passes) {
+        if (WIDE) {
+          cp_async_wait<SM::DEPTH - 1>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int col = 8 * (g >> 1) + 2 * n + (g & 1);
+          if (WIDE)
+            w[n].load(reinterpret_cast<const T *>(ring + slot * SM::STAGE + col * SM::ROW) + t * PER, PER, true);
+          else
+            w[n].load(b + (uint64_t)min(c0 + col, p.n - 1) * p.rank + q * RC + t * PER,
+                      c0 + col < p.n ? p.rank - q * RC - t * PER : 0, p.wide_b);
+        }
+        if (WIDE) {
+          __syncwarp();
+          slot = slot + 1 == SM::DEPTH ? 0 : slot + 1;
+          fetch();
+        }
+      }
+      const bool add = q || p.base;  // (more than one pass: the sums so far are in y)
+      for (int mt = 0; mt < mts; ++mt) {
+        const Old old = next;
+        if (mt + 1 < mts) load_old(next, c0, q, mt + 1);
+        else if (q + 1 < passes && mts > 1) load_old(next, c0, q + 1, 0);  // (one block: not written yet)
+        else if (q + 1 >= passes && c0 + NEXT < p.n) load_old(next, c0 + NEXT, 0, 0);
+        float acc[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        if (passes)
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) {
+            const uint4 *f = hs + (mt * steps + q * STEPS + s) * 64 + lane;
+            const uint4 h0 = f[0], l0 = f[32];
+            const uint32_t hi[4] = {h0.x, h0.y, h0.z, h0.w}, lo[4] = {l0.x, l0.y, l0.z, l0.w};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const float2 v = w[n].pair(s);
+              multiply<T>(acc[n], hi, lo, v.x, v.y);
+            }
           }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (mt * M + g + 8 * h >= tile.len) continue;
+          float v[8];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              v[2 * n + e] = !passes ? old.v[h][2 * n + e]
+                             : add   ? old.v[h][2 * n + e] + acc[n][2 * h + e]
+                                     : acc[n][2 * h + e];
+          float *y = p.y + (uint64_t)rows[mt * M + g + 8 * h] * p.n + c;
+          if (wide) {
+            *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4 *>(y + 4) = make_float4(v[4], v[5], v[6], v[7]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < p.n) y[i] = v[i];
+          }
+        }
+        if (mts == 1 && q + 1 < passes) load_old(next, c0, q + 1, 0);
       }
     }
   }
-  if (tile.id >= 0) cluster.barrier_wait();
+  if (WIDE) cp_async_wait<0>();
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The most tiles m rows can make.
-uint64_t tile_bound(uint64_t m, uint64_t count) {
+uint64_t tile_bound(uint64_t m, uint64_t count, uint64_t tile_rows) {
   // an adapter's last tile may be short; above the sort's buckets neighbours may
   // alternate
-  const uint64_t most = count < BUCKETS - 1 || m <= INLINE_ROWS ? m / ROWS + count + 1 : m;
+  const uint64_t most = count < BUCKETS - 1 || m <= INLINE_ROWS ? m / tile_rows + count + 1 : m;
   return most < m ? most : m;
 }
+
+// Rows of a tile: h of 64 rows as operands takes 512 bytes a rank of shared
+// memory, which two CTAs an SM allow up to rank 64.
+int tile_rows_of(uint64_t rank) { return rank <= 64 ? 64 : rank <= 128 ? 32 : 16; }
 
 // The sort's scratch (rows up to INLINE_ROWS need none of it).
 struct Scratch {
@@ -467,7 +607,7 @@ struct Scratch {
     };
     const uint64_t planned = m > INLINE_ROWS ? m : 0;
     order = take(planned * 4);
-    tiles = take(planned ? tile_bound(m, ad.count) * sizeof(Tile) : 0);
+    tiles = take(planned ? tile_bound(m, ad.count, tile_rows_of(ad.rank)) * sizeof(Tile) : 0);
     ntiles = take(4);
     total = at;
   }
@@ -488,24 +628,36 @@ cudaError_t launch_chained(void (*kern)(Params), unsigned grid, int threads, uin
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <typename T, int RC>
+template <typename T, int RC, bool WIDE>
 cudaError_t launch_rc(const Params &p, unsigned tiles, cudaStream_t stream) {
-  const uint32_t width = (uint32_t)ceil_div(p.rank, RC) * RC;
-  const uint32_t whole = ROWS * (width + 4);
-  const uint32_t smem = ((red_floats<RC>() > whole ? red_floats<RC>() : whole) + ROWS * width) * 4;
-  auto *kern = mgb_adapter_kernel<T, RC>;
-  if (RC == 64) {  // the others stay below what needs no opt-in
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+  const int width = h_width(p.rank, RC);
+  uint32_t smem = part_bytes(p.tile_rows, width);
+  if (WIDE && smem < Shared<T, RC>::RING) smem = Shared<T, RC>::RING;
+  smem += h_bytes(p.tile_rows, width);
+  auto *kern = mgb_adapter_kernel<T, RC, WIDE>;
+  if (smem > 40 * 1024) {  // (with the static part above 48 KB) the opt-in is an attribute of the function on a device: once each
+    static std::atomic<uint64_t> opted{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (!(opted.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024);
+      if (e != cudaSuccess) return e;
+      opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+    }
   }
   return launch_chained(kern, tiles * CTAS, 32 * WARPS, smem, stream, p);
 }
 
 template <typename T>
 cudaError_t launch_t(const Params &p, unsigned tiles, cudaStream_t stream) {
-  return p.rank <= 16   ? launch_rc<T, 16>(p, tiles, stream)
-         : p.rank <= 32 ? launch_rc<T, 32>(p, tiles, stream)
-                        : launch_rc<T, 64>(p, tiles, stream);
+  if (p.wide_b && p.wide_y)
+    return p.rank <= 16   ? launch_rc<T, 16, true>(p, tiles, stream)
+           : p.rank <= 32 ? launch_rc<T, 32, true>(p, tiles, stream)
+                          : launch_rc<T, 64, true>(p, tiles, stream);
+  return p.rank <= 16   ? launch_rc<T, 16, false>(p, tiles, stream)
+         : p.rank <= 32 ? launch_rc<T, 32, false>(p, tiles, stream)
+                        : launch_rc<T, 64, false>(p, tiles, stream);
 }
 
 }  // namespace
@@ -534,6 +686,7 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
   p.k = (int)ad.k;
   p.n = (int)ad.n;
   p.rank = (int)ad.rank;
+  p.tile_rows = tile_rows_of(ad.rank);
   const Scratch s(ad, m);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   p.order = reinterpret_cast<int32_t *>(ws + s.order);
@@ -548,7 +701,7 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
     e = launch_chained(mgb_adapter_plan_kernel, 1, 1024, 0, stream, p);
     if (e != cudaSuccess) return e;
   }
-  const unsigned tiles = (unsigned)tile_bound(m, ad.count);
+  const unsigned tiles = (unsigned)tile_bound(m, ad.count, p.tile_rows);
   if (ad.dtype == MGB_DTYPE_F32) return launch_t<float>(p, tiles, stream);
   if (ad.dtype == MGB_DTYPE_F16) return launch_t<__half>(p, tiles, stream);
   return launch_t<__nv_bfloat16>(p, tiles, stream);
