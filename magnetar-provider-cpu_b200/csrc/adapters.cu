@@ -1,10 +1,12 @@
 // Low-rank adapters of many requests beside a shared projection:
 //   y[r] = base[r] + s_a * (x[r] A_a^T) B_a^T,  a = ids[r],
 // in two products: h[r] = s_a * A_a x[r] (rank values a row), y[r] = base[r] +
-// B_a h[r], by one launch: a cluster of 8 CTAs takes one group of rows, each CTA
-// an eighth of k for h, which they exchange through distributed shared memory,
-// and then an eighth of the outputs (two chained launches cost one row 9.8 us
-// against PLACEHOLDER).
+// B_a h[r].  Up to 128 rows, where launches count, one launch does both: a
+// cluster takes one group of rows, each of its CTAs a slice of k for h, which
+// they exchange through distributed shared memory, and then a slice of the
+// outputs.  More rows take three chained launches (grouping, h, y) and hand h over
+// through global memory: at 64 rows a group the exchange of 8 CTAs' parts by
+// remote reads of shared memory alone took 47 us of 187 (2,048 rows, rank 64).
 //
 // Rows are grouped by adapter into tiles of up to 64, so that an adapter is read
 // once for its rows whatever their order, and one row alone costs no more than
@@ -33,7 +35,7 @@ constexpr int M = 16;             // rows of an MMA
 constexpr int MOST_ROWS = 64;     // of a tile
 constexpr int INLINE_ROWS = 128;  // up to here every CTA plans for itself
 constexpr int BUCKETS = 4096;     // of the planning kernel's sort
-constexpr int CTAS = 8;           // of a cluster
+constexpr int MOST_CTAS = 8;      // of a cluster
 constexpr int WARPS = 8;          // of a CTA
 constexpr int COLS = 32;          // outputs of a warp at a time
 
@@ -50,7 +52,7 @@ struct Tile {
 struct Params {
   const void *a, *b;
   const float *scales, *ids, *x, *base;
-  float *y;
+  float *y, *h;      // h: [splits][m, sorted][h_width] (m > INLINE_ROWS)
   int32_t *order;    // [m]: the rows by adapter (m > INLINE_ROWS)
   Tile *tiles;       // and their tiles
   int32_t *ntiles;
@@ -58,6 +60,7 @@ struct Params {
   uint64_t count;
   int m, k, n, rank;
   int tile_rows;     // rows of a tile: 16, 32 or 64
+  int splits;        // slices of k (the CTAs of a cluster, or of the grid)
   bool wide_a, wide_b, wide_x, wide_y;  // 16-byte loads are aligned
 };
 
@@ -132,20 +135,27 @@ __device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {  
 }
 
 // One CTA: rows by bucket (the adapter, modulo 4,095; the last bucket holds the
-// rows without one), then tiles of up to tile_rows neighbours of one adapter.  Which
-// tile a row lands in does not affect its result.
+// rows without one), then tiles of up to tile_rows neighbours of one adapter.
+// Up to CACHED rows the ids and the order stay in shared memory.
+constexpr int CACHED = 4096;
 __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) {
   __shared__ int at[BUCKETS];
+  __shared__ int ids[CACHED];      // by row, then by sorted position
+  __shared__ uint16_t sorted[CACHED];
   __shared__ int sums[32], s_carry[2];
   grid_wait();
   grid_dependents();
+  const bool cached = p.m <= CACHED;
   for (int b = threadIdx.x; b < BUCKETS; b += 1024) at[b] = 0;
   __syncthreads();
-  auto id_of = [&](int r) { return adapter_of(p.ids[r], p.count); };
   auto bucket = [&](int id) { return id < 0 ? BUCKETS - 1 : id % (BUCKETS - 1); };
   for (int r = threadIdx.x; r < p.m; r += 1024) {
-    const int id = id_of(r);
-    if (id == -2 && p.bad) atomicMin(p.bad, (uint32_t)r);
+    int id = adapter_of(p.ids[r], p.count);
+    if (id == -2) {
+      if (p.bad) atomicMin(p.bad, (uint32_t)r);
+      id = -1;
+    }
+    if (cached) ids[r] = id;
     atomicAdd(&at[bucket(id)], 1);
   }
   __syncthreads();
@@ -158,8 +168,29 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
     for (int i = 0; i < 4; ++i) at[4 * threadIdx.x + i] = s, s += c[i];
   }
   __syncthreads();
-  for (int r = threadIdx.x; r < p.m; r += 1024) p.order[atomicAdd(&at[bucket(id_of(r))], 1)] = r;
-  __syncthreads();
+  // in row order, a warp after the other: where a row lands decides in which order
+  // its sums are taken
+  for (int r0 = 0; r0 < p.m; r0 += 1024) {
+    const int r = r0 + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int id = r >= p.m ? -1 : cached ? ids[r] : max(adapter_of(p.ids[r], p.count), -1);
+    const int b = r < p.m ? bucket(id) : BUCKETS;
+    const uint32_t same = __match_any_sync(0xffffffffu, b);
+    for (int w = 0; w < 32 && r0 + 32 * w < p.m; ++w) {
+      if (warp == w) {  // (the whole warp)
+        const int i = r < p.m ? at[b] + __popc(same & ((1u << lane) - 1)) : 0;
+        __syncwarp();
+        if (r < p.m) {
+          p.order[i] = r;
+          if (cached) sorted[i] = (uint16_t)r;
+          if ((same >> lane) == 1u) at[b] = i + 1;  // the last of its bucket
+        }
+      }
+      __syncthreads();
+    }
+  }
+  auto id_at = [&](int i) {
+    return cached ? ids[sorted[i]] : max(adapter_of(p.ids[p.order[i]], p.count), -1);
+  };
   // run heads, then tile heads (every tile_rows-th row of a run)
   if (threadIdx.x == 0) s_carry[0] = 0, s_carry[1] = 0;
   __syncthreads();
@@ -167,8 +198,8 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
     const int i = p0 + threadIdx.x;
     int id = -3, prev = -3;
     if (i < p.m) {
-      id = max(id_of(p.order[i]), -1);
-      if (i) prev = max(id_of(p.order[i - 1]), -1);
+      id = id_at(i);
+      if (i) prev = id_at(i - 1);
     }
     const bool head = i < p.m && id != prev;
     // the run's start: an inclusive maximum of the head positions
@@ -345,116 +376,103 @@ __host__ __device__ inline uint32_t part_bytes(int tile_rows, int width) {
   return tile_rows * (width + 4) * 4;
 }
 
-template <typename T, int RC, bool WIDE>
-__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
-    mgb_adapter_kernel(const Params p) {
-  using SM = Shared<T, RC>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ SmallPlan plan;
-  __shared__ int rows[MOST_ROWS];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cta = (int)cluster.block_rank();
-  const int width = h_width(p.rank, RC), stride = width + 4;
-  uint4 *hs = reinterpret_cast<uint4 *>(smem);  // [rows / 16][width / 8][hi, lo][lane]
-  float *part = reinterpret_cast<float *>(smem + h_bytes(p.tile_rows, width));
-  grid_wait();
-  grid_dependents();
-  Tile tile;
-  // (the whole cluster has one tile)
-  if (!find_tile(p, blockIdx.x / CTAS, plan, rows, blockIdx.x == 0, tile)) return;
+// part = A x over groups g0 .. g1 of 32 of k, by the whole CTA.  A warp takes one
+// block of rows (of 1, 2 or 4) and every kparts-th group.
+template <typename T, int RC>
+__device__ __forceinline__ void shrink(const Params &p, const Tile &tile, const int (&rows)[MOST_ROWS],
+                                       int g0, int g1, int width, float *part) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int mts = (tile.len + M - 1) / M;  // blocks of 16 rows
-
-  if (tile.id >= 0) {
-    // h = s A x.  This CTA's eighth of k in groups of 32; a warp takes one block of
-    // rows (of 1, 2 or 4) and every kparts-th group
-    const int split_m = mts > 2 ? 4 : mts, kparts = WARPS / split_m;
-    const int mt = warp % split_m, kp = warp / split_m;
-    const T *a = static_cast<const T *>(p.a) + (uint64_t)tile.id * p.rank * p.k;
-    const float *x0 = p.x + (uint64_t)rows[mt * M + g] * p.k, *x1 = p.x + (uint64_t)rows[mt * M + g + 8] * p.k;
-    const int groups = (p.k + 31) / 32, per = (groups + CTAS - 1) / CTAS;
-    const int g0 = min(groups, cta * per), g1 = min(groups, g0 + per);
-    for (int r0 = 0; r0 < p.rank; r0 += RC) {
-      float acc[RC / 8][4];
+  const int mts = (tile.len + M - 1) / M, stride = width + 4;
+  const int split_m = mts > 2 ? 4 : mts, kparts = WARPS / split_m;
+  const int mt = warp % split_m, kp = warp / split_m;
+  const T *a = static_cast<const T *>(p.a) + (uint64_t)tile.id * p.rank * p.k;
+  const float *x0 = p.x + (uint64_t)rows[mt * M + g] * p.k, *x1 = p.x + (uint64_t)rows[mt * M + g + 8] * p.k;
+  for (int r0 = 0; r0 < p.rank; r0 += RC) {
+    float acc[RC / 8][4];
 #pragma unroll
-      for (int n = 0; n < RC / 8; ++n)
+    for (int n = 0; n < RC / 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-      if (mt < mts)
-        for (int q = g0 + kp; q < g1; q += kparts) {
-          const int k0 = q * 32 + t * 8, left = p.k - k0;  // this lane's 8 values: K of four MMAs
-          float v0[8], v1[8];
-          load_values<8>(x0 + k0, left, p.wide_x, v0);
-          load_values<8>(x1 + k0, left, p.wide_x, v1);
-          uint32_t hi[4][4], lo[4][4];
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+    if (mt < mts)
+      for (int q = g0 + kp; q < g1; q += kparts) {
+        const int k0 = q * 32 + t * 8, left = p.k - k0;  // this lane's 8 values: K of four MMAs
+        float v0[8], v1[8];
+        Pairs<T, 8> w[RC / 8];
+        load_values<8>(x0 + k0, left, p.wide_x, v0);
+        load_values<8>(x1 + k0, left, p.wide_x, v1);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            split(v0[2 * s], hi[s][0], lo[s][0]);
-            split(v1[2 * s], hi[s][1], lo[s][1]);
-            split(v0[2 * s + 1], hi[s][2], lo[s][2]);
-            split(v1[2 * s + 1], hi[s][3], lo[s][3]);
-          }
+        for (int n = 0; n < RC / 8; ++n) {
+          const int r = r0 + n * 8 + g;
+          w[n].load(a + (uint64_t)min(r, p.rank - 1) * p.k + k0, r < p.rank ? left : 0, p.wide_a);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          uint32_t hi[4], lo[4];
+          split(v0[2 * s], hi[0], lo[0]);
+          split(v1[2 * s], hi[1], lo[1]);
+          split(v0[2 * s + 1], hi[2], lo[2]);
+          split(v1[2 * s + 1], hi[3], lo[3]);
 #pragma unroll
           for (int n = 0; n < RC / 8; ++n) {
-            const int r = r0 + n * 8 + g;
-            if (r0 + n * 8 >= p.rank) break;
-            float w[8];
-            load_values<8>(a + (uint64_t)min(r, p.rank - 1) * p.k + k0, r < p.rank ? left : 0, p.wide_a, w);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) multiply<T>(acc[n], hi[s], lo[s], w[2 * s], w[2 * s + 1]);
+            const float2 v = w[n].pair(s);
+            multiply<T>(acc[n], hi, lo, v.x, v.y);
           }
         }
-      // the warps' sums, in order
-      for (int k = 0; k < kparts; ++k) {
-        if (kp == k && mt < mts)
-#pragma unroll
-          for (int n = 0; n < RC / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float *at = part + (mt * M + g + 8 * (i >> 1)) * stride + r0 + n * 8 + 2 * t + (i & 1);
-              *at = k ? *at + acc[n][i] : acc[n][i];
-            }
-        __syncthreads();
       }
-    }
-    cluster.sync();
-    // the whole h, summed over the CTAs in order, as operands: lane (g, t) of step
-    // 8 q + s multiplies ranks q RC + t RC / 4 + 2 s and the next
-    const float scale = p.scales ? p.scales[tile.id] : 1.f;
-    const int steps = width / 8;
-    for (int i = threadIdx.x; i < mts * steps * 32; i += 32 * WARPS) {
-      const int l = i & 31, step = (i >> 5) % steps, b = (i >> 5) / steps;
-      const int r = step / (RC / 8) * RC + (l & 3) * (RC / 4) + 2 * (step % (RC / 8));
-      const float *at = part + (b * M + (l >> 2)) * stride + r;
-      float2 v0 = make_float2(0.f, 0.f), v1 = v0;
+    // the warps' sums, in order
+    for (int k = 0; k < kparts; ++k) {
+      if (kp == k && mt < mts)
 #pragma unroll
-      for (int c = 0; c < CTAS; ++c) {
-        const float *o = cluster.map_shared_rank(at, c);
-        const float2 u0 = *reinterpret_cast<const float2 *>(o), u1 = *reinterpret_cast<const float2 *>(o + 8 * stride);
-        v0.x += u0.x, v0.y += u0.y, v1.x += u1.x, v1.y += u1.y;
-      }
-      uint4 hi, lo;
-      split(v0.x * scale, hi.x, lo.x);
-      split(v1.x * scale, hi.y, lo.y);
-      split(v0.y * scale, hi.z, lo.z);
-      split(v1.y * scale, hi.w, lo.w);
-      hs[(b * steps + step) * 64 + l] = hi;
-      hs[(b * steps + step) * 64 + 32 + l] = lo;
+        for (int n = 0; n < RC / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float *at = part + (mt * M + g + 8 * (i >> 1)) * stride + r0 + n * 8 + 2 * t + (i & 1);
+            *at = k ? *at + acc[n][i] : acc[n][i];
+          }
+      __syncthreads();
     }
-    cluster.sync();  // h is complete, and no CTA reads another's part any more
   }
+}
 
-  // y = base + B h: blocks of 32 outputs.  A warp's four MMA column blocks are
-  // interleaved so that a lane ends up with 8 neighbouring outputs of a row: column
-  // g of block n is output 8 (g / 2) + 2 n + g % 2.
-  constexpr int PER = RC / 4, STEPS = RC / 8, CHUNKS = RC * sizeof(T) / 16, NEXT = CTAS * WARPS * COLS;
+// h as operands: lane (g, t) of step q RC / 8 + s multiplies ranks q RC + t RC / 4 +
+// 2 s and the next.  sum(row, r): h of the tile's row at ranks r and r + 1.
+template <int RC, typename F>
+__device__ __forceinline__ void h_operands(uint4 *hs, int mts, int width, const F &sum) {
+  const int steps = width / 8;
+  for (int i = threadIdx.x; i < mts * steps * 32; i += 32 * WARPS) {
+    const int l = i & 31, step = (i >> 5) % steps, b = (i >> 5) / steps;
+    const int r = step / (RC / 8) * RC + (l & 3) * (RC / 4) + 2 * (step % (RC / 8));
+    const float2 v0 = sum(b * M + (l >> 2), r), v1 = sum(b * M + (l >> 2) + 8, r);
+    uint4 hi, lo;
+    split(v0.x, hi.x, lo.x);
+    split(v1.x, hi.y, lo.y);
+    split(v0.y, hi.z, lo.z);
+    split(v1.y, hi.w, lo.w);
+    hs[(b * steps + step) * 64 + l] = hi;
+    hs[(b * steps + step) * 64 + 32 + l] = lo;
+  }
+}
+
+// y = base + B h for the blocks of 32 outputs first, first + step, ... of this
+// warp.  Its four MMA column blocks are interleaved so that a lane ends up with 8
+// neighbouring outputs of a row: column g of block n is output 8 (g / 2) + 2 n +
+// g % 2.
+template <typename T, int RC, bool WIDE>
+__device__ __forceinline__ void expand(const Params &p, const Tile &tile, const int (&rows)[MOST_ROWS],
+                                       const uint4 *hs, int width, uint8_t *ring, int first, int end,
+                                       int step) {
+  using SM = Shared<T, RC>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int mts = (tile.len + M - 1) / M;
+  constexpr int PER = RC / 4, STEPS = RC / 8, CHUNKS = RC * sizeof(T) / 16;
+  const int NEXT = step * COLS, last = min(p.n, end * COLS);
   const T *b = static_cast<const T *>(p.b) + (uint64_t)max(tile.id, 0) * p.n * p.rank;
   const int passes = tile.id >= 0 ? width / RC : 0, steps = width / 8;
-  uint8_t *ring = smem + h_bytes(p.tile_rows, width) + warp * SM::DEPTH * SM::STAGE;
+  ring += (threadIdx.x >> 5) * SM::DEPTH * SM::STAGE;
   // WIDE: a warp's copies of B (a pass of a block a stage) run DEPTH ahead
-  int fc = (cta * WARPS + warp) * COLS, fp = 0, fslot = 0, slot = 0;
+  int fc = first * COLS, fp = 0, fslot = 0, slot = 0;
   auto fetch = [&]() {
-    if (fc < p.n && passes) {
+    if (fc < last && passes) {
       uint8_t *st = ring + fslot * SM::STAGE;
       const int have = (p.rank - fp * RC) * (int)sizeof(T);  // bytes of a row in this pass
 #pragma unroll
@@ -503,9 +521,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, sizeo
     }
   };
   Old next;
-  int c0 = (cta * WARPS + warp) * COLS;
-  if (c0 < p.n) load_old(next, c0, 0, 0);
-  for (; c0 < p.n; c0 += NEXT) {
+  int c0 = first * COLS;
+  if (c0 < last) load_old(next, c0, 0, 0);
+  for (; c0 < last; c0 += NEXT) {
     const int c = c0 + 8 * t;
     const bool wide = p.wide_y && c + 8 <= p.n;
     for (int q = 0; q < max(passes, 1); ++q) {
@@ -535,7 +553,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, sizeo
         const Old old = next;
         if (mt + 1 < mts) load_old(next, c0, q, mt + 1);
         else if (q + 1 < passes && mts > 1) load_old(next, c0, q + 1, 0);  // (one block: not written yet)
-        else if (q + 1 >= passes && c0 + NEXT < p.n) load_old(next, c0 + NEXT, 0, 0);
+        else if (q + 1 >= passes && c0 + NEXT < last) load_old(next, c0 + NEXT, 0, 0);
         float acc[4][4];
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -581,6 +599,98 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(32 * WARPS, sizeo
   if (WIDE) cp_async_wait<0>();
 }
 
+// Both products of one tile by a cluster of `splits` CTAs.
+template <typename T, int RC, bool WIDE>
+__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapter_kernel(const Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ SmallPlan plan;
+  __shared__ int rows[MOST_ROWS];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cta = (int)cluster.block_rank(), ctas = p.splits, warp = threadIdx.x >> 5;
+  const int width = h_width(p.rank, RC);
+  uint4 *hs = reinterpret_cast<uint4 *>(smem);
+  float *part = reinterpret_cast<float *>(smem + h_bytes(p.tile_rows, width));
+  grid_wait();
+  grid_dependents();
+  Tile tile;
+  // (the whole cluster has one tile)
+  if (!find_tile(p, blockIdx.x / ctas, plan, rows, blockIdx.x == 0, tile)) return;
+  if (tile.id >= 0) {
+    const int groups = (p.k + 31) / 32, per = (groups + ctas - 1) / ctas;
+    const int g0 = min(groups, cta * per), g1 = min(groups, g0 + per);
+    shrink<T, RC>(p, tile, rows, g0, g1, width, part);
+    cluster.sync();
+    const float scale = p.scales ? p.scales[tile.id] : 1.f;
+    h_operands<RC>(hs, (tile.len + M - 1) / M, width, [&](int row, int r) {
+      float2 s = make_float2(0.f, 0.f);
+      if (row >= tile.len) return s;
+      for (int c = 0; c < ctas; ++c) {  // in order
+        const float2 u = *reinterpret_cast<const float2 *>(
+            cluster.map_shared_rank(part + row * (width + 4) + r, c));
+        s.x += u.x, s.y += u.y;
+      }
+      return make_float2(s.x * scale, s.y * scale);
+    });
+    cluster.sync();  // h is complete, and no CTA reads another's part any more
+  }
+  expand<T, RC, WIDE>(p, tile, rows, hs, width, smem + h_bytes(p.tile_rows, width), cta * WARPS + warp,
+                      (p.n + COLS - 1) / COLS, ctas * WARPS);
+}
+
+// The two products apart, for grouped rows: CTA (slice of k, tile), and CTA
+// (slice of the outputs, tile).
+template <typename T, int RC>
+__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapter_h_kernel(const Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ SmallPlan plan;
+  __shared__ int rows[MOST_ROWS];
+  const int width = h_width(p.rank, RC);
+  float *part = reinterpret_cast<float *>(smem);
+  grid_wait();
+  grid_dependents();
+  Tile tile;
+  const int split = blockIdx.x % p.splits;
+  if (!find_tile(p, blockIdx.x / p.splits, plan, rows, false, tile) || tile.id < 0) return;
+  const int groups = (p.k + 31) / 32, per = (groups + p.splits - 1) / p.splits;
+  const int g0 = min(groups, split * per), g1 = min(groups, g0 + per);
+  shrink<T, RC>(p, tile, rows, g0, g1, width, part);
+  const float scale = p.scales ? p.scales[tile.id] : 1.f;
+  float *h = p.h + ((uint64_t)split * p.m + tile.start) * width;
+  for (int i = threadIdx.x; i < tile.len * width; i += 32 * WARPS)
+    h[i] = part[i / width * (width + 4) + i % width] * scale;
+}
+constexpr int Y_BLOCKS = 2;  // blocks of 32 outputs of a warp, with 16 rows a block of rows
+template <typename T, int RC, bool WIDE>
+__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
+    mgb_adapter_y_kernel(const Params p, int slices) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ SmallPlan plan;
+  __shared__ int rows[MOST_ROWS];
+  const int width = h_width(p.rank, RC), warp = threadIdx.x >> 5;
+  uint4 *hs = reinterpret_cast<uint4 *>(smem);
+  grid_wait();
+  grid_dependents();
+  Tile tile;
+  const int slice = blockIdx.x % slices;
+  if (!find_tile(p, blockIdx.x / slices, plan, rows, false, tile)) return;
+  if (tile.id >= 0) {
+    h_operands<RC>(hs, (tile.len + M - 1) / M, width, [&](int row, int r) {
+      float2 s = make_float2(0.f, 0.f);
+      if (row >= tile.len) return s;
+      const float *at = p.h + (uint64_t)(tile.start + row) * width + r;
+      for (int c = 0; c < p.splits; ++c) {  // in order
+        const float2 u = *reinterpret_cast<const float2 *>(at + (uint64_t)c * p.m * width);
+        s.x += u.x, s.y += u.y;
+      }
+      return s;
+    });
+    __syncthreads();
+  }
+  const int blocks = (p.n + COLS - 1) / COLS, per = (blocks + slices - 1) / slices;
+  expand<T, RC, WIDE>(p, tile, rows, hs, width, smem + h_bytes(p.tile_rows, width), slice * per + warp,
+                      min(blocks, (slice + 1) * per), WARPS);
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The most tiles m rows can make.
@@ -595,10 +705,27 @@ uint64_t tile_bound(uint64_t m, uint64_t count, uint64_t tile_rows) {
 // memory, which two CTAs an SM allow up to rank 64.
 int tile_rows_of(uint64_t rank) { return rank <= 64 ? 64 : rank <= 128 ? 32 : 16; }
 
-// The sort's scratch (rows up to INLINE_ROWS need none of it).
+int pass_ranks(uint64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
+
+// Slices of k.  A cluster: as many CTAs as keep all clusters on the SMs at once
+// (two CTAs each), so that 64 rows of 64 adapters do not run in two waves.  The
+// grid: enough for two CTAs an SM, at least a group of 32 a warp.
+int k_splits(const mgb_adapters &ad, uint64_t m, int sms) {
+  const uint64_t tiles = tile_bound(m, ad.count, tile_rows_of(ad.rank));
+  if (m <= INLINE_ROWS) {
+    int s = MOST_CTAS;
+    while (s > 1 && tiles * s > 2 * (uint64_t)sms) s /= 2;
+    return s;
+  }
+  const uint64_t want = ceil_div(2 * (uint64_t)sms, tiles), most = ceil_div(ceil_div(ad.k, 32), WARPS);
+  const uint64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+}
+
+// Grouped rows' scratch (up to INLINE_ROWS rows need none of it).
 struct Scratch {
-  uint64_t order, tiles, ntiles, total;
-  Scratch(const mgb_adapters &ad, uint64_t m) {
+  uint64_t order, tiles, ntiles, h, total;
+  Scratch(const mgb_adapters &ad, uint64_t m, int splits) {
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
       const uint64_t r = at;
@@ -609,61 +736,92 @@ struct Scratch {
     order = take(planned * 4);
     tiles = take(planned ? tile_bound(m, ad.count, tile_rows_of(ad.rank)) * sizeof(Tile) : 0);
     ntiles = take(4);
+    h = take((uint64_t)splits * planned * h_width((int)ad.rank, pass_ranks(ad.rank)) * 4);
     total = at;
   }
 };
 
-cudaError_t launch_chained(void (*kern)(Params), unsigned grid, int threads, uint32_t smem,
-                           cudaStream_t stream, const Params &p) {
+int current_sms() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return device_sms(dev);
+}
+
+// A programmatic dependent launch, in clusters of `cluster` CTAs.
+template <typename... A>
+cudaError_t launch_chained(void (*kern)(A...), unsigned grid, int threads, uint32_t smem, int cluster,
+                           cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Lets a kernel use its dynamic shared memory: an attribute of the function on a
+// device, set once each.
+template <typename K>
+cudaError_t opt_in(K kern, std::atomic<uint64_t> &opted) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || opted.load(std::memory_order_relaxed) >> (dev & 63) & 1) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024);
+  if (e == cudaSuccess) opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+  return e;
 }
 
 template <typename T, int RC, bool WIDE>
-cudaError_t launch_rc(const Params &p, unsigned tiles, cudaStream_t stream) {
+cudaError_t launch_rc(const Params &p, unsigned tiles, int sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> opted[3];
   const int width = h_width(p.rank, RC);
-  uint32_t smem = part_bytes(p.tile_rows, width);
-  if (WIDE && smem < Shared<T, RC>::RING) smem = Shared<T, RC>::RING;
-  smem += h_bytes(p.tile_rows, width);
-  auto *kern = mgb_adapter_kernel<T, RC, WIDE>;
-  if (smem > 40 * 1024) {  // (with the static part above 48 KB) the opt-in is an attribute of the function on a device: once each
-    static std::atomic<uint64_t> opted{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (!(opted.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024);
-      if (e != cudaSuccess) return e;
-      opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
-    }
+  const uint32_t h = h_bytes(p.tile_rows, width), part = part_bytes(p.tile_rows, width);
+  const uint32_t ring = WIDE ? Shared<T, RC>::RING : 0;
+  cudaError_t e;
+  if (p.m <= INLINE_ROWS) {
+    if ((e = opt_in(mgb_adapter_kernel<T, RC, WIDE>, opted[0])) != cudaSuccess) return e;
+    return launch_chained(mgb_adapter_kernel<T, RC, WIDE>, tiles * p.splits, 32 * WARPS,
+                          h + (part > ring ? part : ring), p.splits, stream, p);
   }
-  return launch_chained(kern, tiles * CTAS, 32 * WARPS, smem, stream, p);
+  if ((e = opt_in(mgb_adapter_h_kernel<T, RC>, opted[1])) != cudaSuccess) return e;
+  if ((e = opt_in(mgb_adapter_y_kernel<T, RC, WIDE>, opted[2])) != cudaSuccess) return e;
+  e = launch_chained(mgb_adapter_h_kernel<T, RC>, tiles * p.splits, 32 * WARPS, part, 1, stream, p);
+  if (e != cudaSuccess) return e;
+  // slices of the outputs: a few blocks a warp, and the SMs covered
+  const uint64_t blocks = ceil_div(p.n, COLS);
+  uint64_t slices = ceil_div(blocks, WARPS * Y_BLOCKS);
+  const uint64_t cover = ceil_div(2 * (uint64_t)sms, tiles), most = ceil_div(blocks, WARPS);
+  if (slices < cover) slices = cover < most ? cover : most;
+  const uint64_t fit = 0x7FFFFFFFull / tiles;  // CTAs of a grid
+  if (slices > fit) slices = fit;
+  return launch_chained(mgb_adapter_y_kernel<T, RC, WIDE>, (unsigned)(tiles * slices), 32 * WARPS, h + ring,
+                        1, stream, p, (int)slices);
 }
 
 template <typename T>
-cudaError_t launch_t(const Params &p, unsigned tiles, cudaStream_t stream) {
+cudaError_t launch_t(const Params &p, unsigned tiles, int sms, cudaStream_t stream) {
+  const int rc = pass_ranks(p.rank);
   if (p.wide_b && p.wide_y)
-    return p.rank <= 16   ? launch_rc<T, 16, true>(p, tiles, stream)
-           : p.rank <= 32 ? launch_rc<T, 32, true>(p, tiles, stream)
-                          : launch_rc<T, 64, true>(p, tiles, stream);
-  return p.rank <= 16   ? launch_rc<T, 16, false>(p, tiles, stream)
-         : p.rank <= 32 ? launch_rc<T, 32, false>(p, tiles, stream)
-                        : launch_rc<T, 64, false>(p, tiles, stream);
+    return rc == 16   ? launch_rc<T, 16, true>(p, tiles, sms, stream)
+           : rc == 32 ? launch_rc<T, 32, true>(p, tiles, sms, stream)
+                      : launch_rc<T, 64, true>(p, tiles, sms, stream);
+  return rc == 16   ? launch_rc<T, 16, false>(p, tiles, sms, stream)
+         : rc == 32 ? launch_rc<T, 32, false>(p, tiles, sms, stream)
+                    : launch_rc<T, 64, false>(p, tiles, sms, stream);
 }
 
 }  // namespace
 
 uint64_t adapters_scratch_bytes(const mgb_adapters &ad, uint64_t m) {
-  return m ? Scratch(ad, m).total : 0;
+  return m ? Scratch(ad, m, k_splits(ad, m, current_sms())).total : 0;
 }
 
 cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const float *x, uint64_t m,
@@ -687,24 +845,27 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
   p.n = (int)ad.n;
   p.rank = (int)ad.rank;
   p.tile_rows = tile_rows_of(ad.rank);
-  const Scratch s(ad, m);
+  const int sms = current_sms();
+  p.splits = k_splits(ad, m, sms);
+  const Scratch s(ad, m, p.splits);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   p.order = reinterpret_cast<int32_t *>(ws + s.order);
   p.tiles = reinterpret_cast<Tile *>(ws + s.tiles);
   p.ntiles = reinterpret_cast<int32_t *>(ws + s.ntiles);
+  p.h = reinterpret_cast<float *>(ws + s.h);
   const uint64_t per = ad.dtype == MGB_DTYPE_F32 ? 4 : 8;  // values in 16 bytes
   p.wide_a = aligned16(ad.a) && ad.k % per == 0;
   p.wide_b = aligned16(ad.b) && ad.rank % per == 0;
   p.wide_x = aligned16(x) && ad.k % 4 == 0;
   p.wide_y = aligned16(y) && aligned16(base) && ad.n % 4 == 0;
   if (m > INLINE_ROWS) {
-    e = launch_chained(mgb_adapter_plan_kernel, 1, 1024, 0, stream, p);
+    e = launch_chained(mgb_adapter_plan_kernel, 1, 1024, 0, 1, stream, p);
     if (e != cudaSuccess) return e;
   }
   const unsigned tiles = (unsigned)tile_bound(m, ad.count, p.tile_rows);
-  if (ad.dtype == MGB_DTYPE_F32) return launch_t<float>(p, tiles, stream);
-  if (ad.dtype == MGB_DTYPE_F16) return launch_t<__half>(p, tiles, stream);
-  return launch_t<__nv_bfloat16>(p, tiles, stream);
+  if (ad.dtype == MGB_DTYPE_F32) return launch_t<float>(p, tiles, sms, stream);
+  if (ad.dtype == MGB_DTYPE_F16) return launch_t<__half>(p, tiles, sms, stream);
+  return launch_t<__nv_bfloat16>(p, tiles, sms, stream);
 }
 
 }  // namespace mgb
