@@ -61,8 +61,10 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
   const int token = blockIdx.x / ROUTE_CTAS;
   const int warp = rank * (ROUTE_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   constexpr int WARPS = ROUTE_CTAS * ROUTE_THREADS / 32;
+  cluster.barrier_arrive();  // (the first CTA has started before its memory is written)
   moe::grid_wait();
   moe::grid_dependents();
+  cluster.barrier_wait();
   double *zs = cluster.map_shared_rank(z, 0);
   const float *xr = x + (size_t)token * hidden;
   const bool wide = hidden % 4 == 0 && ((uintptr_t)router & 15) == 0 && ((uintptr_t)x & 15) == 0;

@@ -5,18 +5,32 @@
 // monotonic, -0 as +0; 0 for -inf and NaN, which are masked).  Every cut keeps
 // a prefix of the tokens sorted by (key descending, index ascending), so what
 // is kept is described by a key tau and how many tokens of key tau (the lowest
-// indices) stay: no sort is needed, only the search for tau.  It is searched
-// by histograms over key ranges, 2,048 bins a level, of counts (top-k) or of
-// probability mass (top-p).
+// indices) stay: no sort of the vocabulary is needed, only the search for tau.
+//
+// A row is read once: a cluster of CTAs holds it in shared memory (a few CTAs an
+// SM, so that one row's loads overlap another's arithmetic), and the CTAs agree
+// on one number after another through distributed shared memory.
+//  - Small top_k: every CTA finds its own candidates (the bins of a histogram of
+//    the distance to its largest logit that hold its first top_k tokens), the
+//    first CTA sorts them all and does the rest: one cluster barrier a row.
+//  - Otherwise tau is searched by histograms of counts (top-k) or of mass (top-p)
+//    over ever smaller key ranges: first by distance to the largest logit, where
+//    tokens spread evenly over the bins, then by key.
 //
 // Mass.  A token's weight is 2^((logit - max) log2(e) / T) as a 64-bit integer
 // in units of 2^-43: integer sums are the same in every order, so atomics and
 // any split of a row give the same token, and a border is only missed where
 // weights round (2^-31 relative).  2^20 tokens of weight 1 stay below 2^63.
+#include <cooperative_groups.h>
+
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
 namespace mgb {
+
+namespace cg = cooperative_groups;
 
 constexpr int ONE_BITS = 43;  // weight 1
 
@@ -90,243 +104,542 @@ struct Weigh {
   }
 };
 
-constexpr int BINS = 2048;
-constexpr int THREADS = 1024;
+constexpr int BINS = 1024;
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int MOST_CTAS = 8;      // of a cluster
+constexpr int LIST = 1024;        // candidates the first CTA sorts
+constexpr int MOST_TOP_K = THREADS;  // of the candidate path
+constexpr uint32_t LOWEST = 0x00800000u;  // the key of the lowest finite value
+constexpr float BIN_SCALE = 16.f;    // bins of the distance to the largest logit
 
-struct Found {
-  uint32_t key;
-  uint64_t above;  // count or mass of the keys above it
+// The bin of a live logit by its distance to the largest one: monotonic.
+__device__ __forceinline__ int distance_bin(float top, float v) {
+  const int b = (int)((top - v) * BIN_SCALE);  // (saturates)
+  return b < BINS - 1 ? b : BINS - 1;
+}
+
+struct Shared {
+  unsigned long long hist[BINS];        // counts or masses; the sort's buffer
+  unsigned long long list[LIST];        // first CTA: its cluster's candidates / histogram
+  unsigned long long scan[WARPS];
+  // what the CTAs tell each other, by rank
+  unsigned long long top[MOST_CTAS];    // (key, ~index) of the largest logit
+  unsigned long long mass[MOST_CTAS], cut_mass[MOST_CTAS];
+  uint32_t live[MOST_CTAS], found[MOST_CTAS], ties[MOST_CTAS], count[MOST_CTAS];
+  // the first CTA's answers
+  unsigned long long above;
+  uint32_t lo, hi;
+  // of the CTA
+  unsigned long long warp_mass[WARPS];
+  uint32_t warp_ties[WARPS], warp_count[WARPS], taken, bin;
 };
 
-// The largest key in [lo, hi] at which the count (MASS: the mass) of the keys
-// from hi down to it reaches `target` (>= 1, at most what [lo, hi] holds).
+__device__ __forceinline__ unsigned long long block_max(unsigned long long v, Shared &s) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const unsigned long long u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = v > u ? v : u;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) v = v > s.scan[w] ? v : s.scan[w];
+  return v;
+}
+
+// Inclusive sum over the CTA's threads.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, Shared &s,
+                                                         unsigned long long &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) s.scan[warp] = v;
+  __syncthreads();
+  total = 0;
+  unsigned long long before = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += s.scan[w];
+    total += s.scan[w];
+  }
+  return before + v;
+}
+
+// The first bin at which the running sum of hist reaches target, and the sum
+// before it; all threads (sums of `hist`, which 4 bins a thread).
+__device__ __forceinline__ void find_bin(const unsigned long long *hist, unsigned long long target,
+                                         Shared &s, int &bin, unsigned long long &before) {
+  unsigned long long c[BINS / THREADS], v = 0, total;
+#pragma unroll
+  for (int i = 0; i < BINS / THREADS; ++i) c[i] = hist[threadIdx.x * (BINS / THREADS) + i], v += c[i];
+  unsigned long long run = block_scan(v, s, total) - v;
+#pragma unroll
+  for (int i = 0; i < BINS / THREADS; ++i) {
+    if (run < target && run + c[i] >= target)
+      s.bin = threadIdx.x * (BINS / THREADS) + i, s.above = run;
+    run += c[i];
+  }
+  __syncthreads();
+  bin = (int)s.bin;
+  before = s.above;
+}
+
+struct Row {
+  const float *v;      // this CTA's part of the row
+  uint32_t first, n;   // index of its first token, tokens
+  float top;           // the row's largest logit
+  uint32_t top_key;
+};
+
+// The largest key in [lo, hi] at which the count (MASS: the mass) of the keys from
+// hi down to it reaches `target` (>= 1, at most what [lo, hi] holds); above: the
+// count or mass of the keys over it.  The whole cluster.
 template <bool MASS>
-__device__ Found find_key(const float *__restrict__ row, uint32_t vocab, uint32_t lo, uint32_t hi,
-                          uint64_t target, const Weigh &weigh, uint64_t *hist) {
-  __shared__ uint64_t s_above, s_warp[THREADS / 32];
-  __shared__ uint32_t s_bin;
-  uint64_t above = 0;
+__device__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t hi, unsigned long long target,
+                             const Weigh &weigh, Shared &s, cg::cluster_group &cluster,
+                             unsigned long long &above) {
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  bool linear = !__isinff(row.top);
+  above = 0;
   while (lo < hi) {
     int shift = 0;
     while (((hi - lo) >> shift) >= BINS) ++shift;
-    for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0;
-    __syncthreads();
-    for (uint32_t t = threadIdx.x; t < vocab; t += THREADS) {
-      const float v = row[t];
+    for (int i = threadIdx.x; i < BINS; i += THREADS) {
+      s.hist[i] = 0;
+      if (rank == 0 && ctas > 1) s.list[i] = 0;  // the cluster's histogram
+    }
+    cluster.sync();
+    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
+      const float v = row.v[i];
       const uint32_t key = key_of(v);
-      if (key < lo || key > hi || !key) continue;
-      atomicAdd((unsigned long long *)&hist[(hi - key) >> shift], MASS ? weigh(v) : 1ull);
+      if (key < lo || key > hi) continue;
+      const int b = linear ? distance_bin(row.top, v) : (int)((hi - key) >> shift);
+      atomicAdd(&s.hist[b], MASS ? (unsigned long long)weigh(v) : 1ull);
     }
     __syncthreads();
-    // inclusive sums from the highest bin; two bins a thread
-    const uint64_t a = hist[2 * threadIdx.x], b = hist[2 * threadIdx.x + 1];
-    uint64_t s = a + b;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += up;
+    if (ctas > 1) {
+      unsigned long long *all = cluster.map_shared_rank(s.list, 0);
+      for (int i = threadIdx.x; i < BINS; i += THREADS)
+        if (s.hist[i]) atomicAdd(&all[i], s.hist[i]);
+      cluster.sync();
     }
-    if (lane == 31) s_warp[warp] = s;
-    __syncthreads();
-    uint64_t before = above;
-    for (int w = 0; w < warp; ++w) before += s_warp[w];
-    const uint64_t end = before + s, start = end - a - b;
-    if (start < target && end >= target) {
-      const bool second = start + a < target;
-      s_bin = 2 * threadIdx.x + second;
-      s_above = second ? start + a : start;
-    }
-    __syncthreads();
-    above = s_above;
-    const uint32_t bin = s_bin;
-    hi = hi - (bin << shift);
-    const uint32_t width = (1u << shift) - 1;
-    lo = hi - lo > width ? hi - width : lo;
-    __syncthreads();
-  }
-  return {hi, above};
-}
-
-template <typename T>
-__device__ T block_sum(T v, T *scratch) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T s = 0;
-  for (int w = 0; w < THREADS / 32; ++w) s += scratch[w];
-  return s;
-}
-
-__global__ void __launch_bounds__(THREADS) mgb_sample_kernel(const SampleArgs p) {
-  __shared__ uint64_t hist[BINS];
-  __shared__ uint64_t scratch[THREADS / 32], seg_mass[THREADS / 32];
-  __shared__ uint32_t seg_ties[THREADS / 32], s_low;
-  __shared__ uint32_t s_max;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t vocab = (uint32_t)p.vocab;
-  for (uint64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    const float *row = p.logits + r * p.ld;
-    __syncthreads();
-    if (threadIdx.x == 0) s_max = 0, s_low = 0xFFFFFFFFu;
-    __syncthreads();
-    uint32_t mx = 0;
-    uint64_t live = 0;
-    for (uint32_t t = threadIdx.x; t < vocab; t += THREADS) {
-      const uint32_t key = key_of(row[t]);
-      mx = max(mx, key);
-      live += key != 0;
-    }
-    atomicMax(&s_max, mx);
-    live = block_sum(live, scratch);
-    const uint32_t top = s_max;
-    if (!top) {
-      if (threadIdx.x == 0) {
-        if (p.ids) p.ids[r] = -1.f;
-        if (p.logprob) p.logprob[r] = __int_as_float(0xff800000);
-        if (p.kept) p.kept[r] = 0;
-      }
-      continue;
-    }
-    const float temp = p.temperature ? p.temperature[r] : 1.f;
-    if (!(temp > 0.f) || !p.uniform) {
-      for (uint32_t t = threadIdx.x; t < vocab; t += THREADS)
-        if (key_of(row[t]) == top) {
-          atomicMin(&s_low, t);
-          break;
+    if (rank == 0) {
+      int bin;
+      unsigned long long before;
+      find_bin(ctas > 1 ? s.list : s.hist, target - above, s, bin, before);
+      if (threadIdx.x < (unsigned)ctas) {
+        uint32_t nlo = lo, nhi = hi;
+        if (linear) {
+          // bins fall as keys grow: the keys of the bin, by bisection
+          auto edge = [&](int b) {  // the smallest key in [lo, hi] whose bin is at most b
+            uint32_t l = lo, h = hi;
+            while (l < h) {
+              const uint32_t m = l + (h - l) / 2;
+              if (distance_bin(row.top, value_of(m)) <= b) h = m;
+              else l = m + 1;
+            }
+            return l;
+          };
+          nlo = edge(bin);
+          nhi = bin ? edge(bin - 1) - 1 : hi;
+        } else {
+          nhi = hi - ((uint32_t)bin << shift);
+          const uint32_t width = (1u << shift) - 1;
+          nlo = nhi - lo > width ? nhi - width : lo;
         }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        if (p.ids) p.ids[r] = (float)s_low;
-        if (p.logprob) p.logprob[r] = 0.f;
-        if (p.kept) p.kept[r] = 1;
+        Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
+        o->lo = nlo;
+        o->hi = nhi;
+        o->above = above + before;
       }
-      continue;
     }
-    Weigh weigh;
-    weigh.top = value_of(top);
-    // 1 / T stays finite
-    const double c = fmin(1.4426950408889634 / (double)temp, 1e30);
+    cluster.sync();
+    lo = s.lo;
+    hi = s.hi;
+    above = s.above;
+    linear = false;
+  }
+  __syncthreads();
+  return hi;
+}
+
+__device__ __forceinline__ void answer(const SampleArgs &p, uint64_t r, float id, float logprob,
+                                       uint32_t kept) {
+  if (p.ids) p.ids[r] = id;
+  if (p.logprob) p.logprob[r] = logprob;
+  if (p.kept) p.kept[r] = kept;
+}
+
+// One row a cluster.  STAGED: each CTA's part of the row is in its shared memory;
+// otherwise (vocabularies that do not fit) it is read from global memory again.
+template <bool STAGED>
+__global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs p, uint32_t chunk) {
+  __shared__ Shared s;
+  extern __shared__ __align__(16) float data[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t r = blockIdx.x / ctas;
+  const uint32_t vocab = (uint32_t)p.vocab;
+  cluster.barrier_arrive();  // (waited for before another CTA's memory is touched: it has started)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  Row row;
+  row.first = min(vocab, rank * chunk);
+  row.n = min(chunk, vocab - row.first);
+  const float *src = p.logits + r * p.ld + row.first;
+  const float temp = p.temperature ? p.temperature[r] : 1.f;
+  const bool greedy = !(temp > 0.f) || !p.uniform;
+  const float kf = p.top_k ? p.top_k[r] : 0.f;
+
+  // the CTA's largest (key, ~index) and live tokens; the row comes in once
+  unsigned long long best = 0;
+  uint32_t live = 0;
+  auto see = [&](float v, uint32_t i) {
+    const uint32_t key = key_of(v);
+    live += key != 0;
+    const unsigned long long c = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (row.first + i));
+    if (key && c > best) best = c;
+  };
+  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    const uint32_t n4 = row.n / 4;
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < n4; i += THREADS) {
+      const float4 v = reinterpret_cast<const float4 *>(src)[i];
+      if (STAGED) reinterpret_cast<float4 *>(data)[i] = v;
+      see(v.x, 4 * i);
+      see(v.y, 4 * i + 1);
+      see(v.z, 4 * i + 2);
+      see(v.w, 4 * i + 3);
+    }
+    for (uint32_t i = 4 * n4 + threadIdx.x; i < row.n; i += THREADS) {
+      const float v = src[i];
+      if (STAGED) data[i] = v;
+      see(v, i);
+    }
+  } else {
+#pragma unroll 8
+    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
+      const float v = src[i];
+      if (STAGED) data[i] = v;
+      see(v, i);
+    }
+  }
+  row.v = STAGED ? data : src;
+  best = block_max(best, s);
+  {
+    unsigned long long total;
+    block_scan(live, s, total);
+    live = (uint32_t)total;
+  }
+
+  cluster.barrier_wait();
+
+  // small top_k: this CTA's candidates, to the first CTA's list
+  const uint32_t room = LIST / ctas;
+  const bool few = !greedy && kf >= 1.f && kf < (float)MOST_TOP_K + 1.f && kf < (float)room + 1.f;
+  uint32_t found = 0xFFFFFFFFu;  // none sent
+  if (few) {
+    const uint32_t k = (uint32_t)kf;
+    const float top = value_of((uint32_t)(best >> 32));
+    int last = BINS;
+    if (threadIdx.x == 0) s.taken = 0;
+    if (live > room && !__isinff(top)) {
+      for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
+        const float v = row.v[i];
+        // (the last bins do not matter: k <= room < live)
+        if (key_of(v)) atomicAdd(&s.hist[distance_bin(top, v)], 1ull);
+      }
+      __syncthreads();
+      unsigned long long before;
+      find_bin(s.hist, k, s, last, before);
+      found = (uint32_t)(before + s.hist[last]);
+    } else {
+      found = live;
+      __syncthreads();
+    }
+    if (found <= room) {
+      unsigned long long *list = cluster.map_shared_rank(s.list, 0) + rank * room;
+      for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
+        const float v = row.v[i];
+        const uint32_t key = key_of(v);
+        if (key && (last == BINS || distance_bin(top, v) <= last))
+          list[atomicAdd(&s.taken, 1u)] =
+              ((unsigned long long)key << 32) | (0xFFFFFFFFu - (row.first + i));
+      }
+    }
+  }
+  if (threadIdx.x < (unsigned)ctas) {
+    Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
+    o->top[rank] = best;
+    o->live[rank] = live;
+    o->found[rank] = found;
+  }
+  cluster.sync();
+  bool listed = few;
+  best = 0, live = 0;
+  for (int c = 0; c < ctas; ++c) {
+    best = best > s.top[c] ? best : s.top[c];
+    live += s.live[c];
+    listed = listed && s.found[c] <= room;
+  }
+  row.top_key = (uint32_t)(best >> 32);
+  if (!row.top_key || greedy) {
+    if (rank == 0 && threadIdx.x == 0) {
+      if (!row.top_key) answer(p, r, -1.f, __int_as_float(0xff800000), 0);
+      else answer(p, r, (float)(0xFFFFFFFFu - (uint32_t)best), 0.f, 1);
+    }
+    return;
+  }
+  row.top = value_of(row.top_key);
+  Weigh weigh;
+  weigh.top = row.top;
+  {
+    const double c = fmin(1.4426950408889634 / (double)temp, 1e30);  // 1 / T stays finite
     weigh.chi = (float)c;
     weigh.clo = (float)(c - (double)weigh.chi);
+  }
+  const float pf = p.top_p ? p.top_p[r] : 1.f, mf = p.min_p ? p.min_p[r] : 0.f;
+  const float uf = p.uniform[r];
+  const double u = uf > 0.f ? (double)fminf(uf, 0.99999994f) : 0.0;
+  const unsigned long long least =
+      mf > 0.f ? (unsigned long long)ceil((double)fminf(mf, 1.f) * (double)(1ull << ONE_BITS)) : 0;
+  auto mass_target = [&](unsigned long long total) {  // of top-p, in [1, total]
+    const double want = ceil((double)fmaxf(pf, 0.f) * (double)total);
+    const unsigned long long t = want < 1.0 ? 1ull : (unsigned long long)want;
+    return t < total ? t : total;
+  };
 
-    // top-k
-    uint32_t tau = 1;  // every live key
-    uint64_t ties = vocab;
-    const float kf = p.top_k ? p.top_k[r] : 0.f;
-    if (kf >= 1.f && floorf(kf) < (float)live) {
-      const uint64_t k = (uint64_t)kf;
-      const Found f = find_key<false>(row, vocab, 1, top, k, weigh, hist);
-      tau = f.key;
-      ties = k - f.above;
+  if (listed) {
+    // ---- the first CTA sorts the candidates, best first, and does the rest
+    if (rank) return;
+    uint32_t n = 0;
+    for (int c = 0; c < ctas; ++c) {
+      for (uint32_t i = threadIdx.x; i < s.found[c]; i += THREADS) s.hist[n + i] = s.list[c * room + i];
+      n += s.found[c];
     }
-    // top-p
-    const float pf = p.top_p ? p.top_p[r] : 1.f;
-    if (pf < 1.f) {
-      uint64_t gt = 0;
-      for (uint32_t t = threadIdx.x; t < vocab; t += THREADS) {
-        const float v = row[t];
-        const uint32_t key = key_of(v);
-        if (key > tau || (key == tau && tau == 1)) gt += weigh(v);
+    uint32_t size = 2;
+    while (size < n) size <<= 1;
+    for (uint32_t i = n + threadIdx.x; i < size; i += THREADS) s.hist[i] = 0;
+    __syncthreads();
+    for (uint32_t k = 2; k <= size; k <<= 1)
+      for (uint32_t j = k >> 1; j; j >>= 1) {
+        for (uint32_t i = threadIdx.x; i < size / 2; i += THREADS) {
+          const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
+          const unsigned long long x = s.hist[a], y = s.hist[b];
+          if ((x < y) == ((a & k) == 0)) s.hist[a] = y, s.hist[b] = x;
+        }
+        __syncthreads();
       }
-      uint64_t total = block_sum(gt, scratch);
-      if (tau > 1) total += ties * weigh(value_of(tau));
-      const double want = ceil((double)fmaxf(pf, 0.f) * (double)total);
-      uint64_t target = want < 1.0 ? 1 : (uint64_t)want;
-      if (target > total) target = total;
-      const Found f = find_key<true>(row, vocab, tau, top, target, weigh, hist);
-      const uint64_t w = weigh(value_of(f.key));
-      const uint64_t need = w ? (target - f.above + w - 1) / w : 1;
-      ties = f.key == tau ? min(ties, need) : need;
-      tau = f.key;
+    const uint32_t i = threadIdx.x;
+    n = min(n, (uint32_t)kf);  // <= THREADS
+    const unsigned long long mine = i < n ? s.hist[i] : 0;
+    const uint32_t key = (uint32_t)(mine >> 32), token = 0xFFFFFFFFu - (uint32_t)mine;
+    const unsigned long long w = i < n ? weigh(value_of(key)) : 0;
+    unsigned long long total;
+    const unsigned long long sum = block_scan(w, s, total);
+    if (pf < 1.f) n = __syncthreads_count(i < n && sum - w < mass_target(total));
+    n = __syncthreads_count(i < n && (w >= least || key == row.top_key));
+    s.list[i] = w;
+    if (i + 1 == n) s.above = sum;  // the kept total
+    __syncthreads();
+    total = s.above;
+    unsigned long long target = (unsigned long long)(u * (double)total);
+    if (target >= total) target = total - 1;
+    if (i < n) {
+      unsigned long long upto = 0;  // the kept mass of the tokens up to this one
+      for (uint32_t j = 0; j < n; ++j)
+        if ((uint32_t)s.hist[j] >= (uint32_t)mine) upto += s.list[j];
+      if (upto > target && upto - w <= target)
+        answer(p, r, (float)token, (float)(log((double)w) - log((double)total)), n);
     }
-    const float mf = p.min_p ? p.min_p[r] : 0.f;
-    const uint64_t least =
-        mf > 0.f ? (uint64_t)ceil((double)fminf(mf, 1.f) * (double)(1ull << ONE_BITS)) : 0;
-    if (tau == 1) ties = 0, tau = 0;  // no cut: every live key is above tau
-    if (tau && tau != top && weigh(value_of(tau)) < least) ties = 0;
-    const uint64_t wt = tau ? weigh(value_of(tau)) : 0;
+    return;
+  }
 
-    // one contiguous segment a warp: kept mass and ties
-    const uint32_t seg = (vocab + THREADS / 32 - 1) / (THREADS / 32);
-    const uint32_t s0 = min(vocab, warp * seg), s1 = min(vocab, s0 + seg);
-    uint64_t mass = 0, count = 0;
-    uint32_t tied = 0;
-    for (uint32_t t = s0 + lane; t < s1; t += 32) {
-      const float v = row[t];
+  // ---- the cuts: everything above tau, and `ties` tokens of key tau
+  uint32_t tau = 0;
+  unsigned long long ties = 0, above;
+  if (kf >= 1.f && floorf(kf) < (float)live) {
+    const unsigned long long k = (unsigned long long)kf;
+    tau = find_key<false>(row, LOWEST, row.top_key, k, weigh, s, cluster, above);
+    ties = k - above;
+  }
+  if (pf < 1.f) {
+    unsigned long long gt = 0, total;
+    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
+      const float v = row.v[i];
+      if (key_of(v) > tau) gt += weigh(v);
+    }
+    block_scan(gt, s, total);
+    if (threadIdx.x < (unsigned)ctas) cluster.map_shared_rank(&s, threadIdx.x)->cut_mass[rank] = total;
+    cluster.sync();
+    total = ties * (tau ? weigh(value_of(tau)) : 0);
+    for (int c = 0; c < ctas; ++c) total += s.cut_mass[c];
+    const unsigned long long target = mass_target(total);
+    const uint32_t key = find_key<true>(row, tau ? tau : LOWEST, row.top_key, target, weigh, s, cluster, above);
+    const unsigned long long w = weigh(value_of(key));
+    const unsigned long long need = w ? (target - above + w - 1) / w : 1;
+    ties = key == tau && ties < need ? ties : need;
+    tau = key;
+  }
+  const unsigned long long wt = tau ? weigh(value_of(tau)) : 0;
+  if (tau && tau != row.top_key && wt < least) ties = 0;
+
+  // ---- kept mass and ties of every warp's stretch of the CTA's part
+  const uint32_t stretch = (row.n + WARPS - 1) / WARPS;
+  const uint32_t s0 = min(row.n, warp * stretch), s1 = min(row.n, s0 + stretch);
+  auto kept = [&](float v, uint32_t key) {  // the weight of a token above tau, if it stays
+    const unsigned long long w = weigh(v);
+    return w >= least || key == row.top_key ? w : 0;
+  };
+  {
+    unsigned long long mass = 0;
+    uint32_t tied = 0, count = 0;
+    for (uint32_t i = s0 + lane; i < s1; i += 32) {
+      const float v = row.v[i];
       const uint32_t key = key_of(v);
-      if (!key || key < tau) continue;
-      if (key == tau) {
+      if (key > tau) {
+        const unsigned long long w = weigh(v);
+        const bool in = w >= least || key == row.top_key;
+        mass += in ? w : 0;
+        count += in;
+      } else if (key && key == tau) {
         ++tied;
-        continue;
       }
-      const uint64_t w = weigh(v);
-      if (w < least && key != top) continue;
-      mass += w;
-      ++count;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       mass += __shfl_xor_sync(0xffffffffu, mass, o);
       tied += __shfl_xor_sync(0xffffffffu, tied, o);
+      count += __shfl_xor_sync(0xffffffffu, count, o);
     }
-    if (lane == 0) seg_mass[warp] = mass, seg_ties[warp] = tied;
-    count = block_sum(count, scratch);
-    uint64_t total = 0, before = 0, mine = 0, mine_ties = 0, left = ties;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      const uint64_t take = min(left, (uint64_t)seg_ties[w]);
-      if (w == warp) before = total, mine = seg_mass[w] + take * wt, mine_ties = take;
-      left -= take;
-      total += seg_mass[w] + take * wt;
+    __syncthreads();
+    if (lane == 0) s.warp_mass[warp] = mass, s.warp_ties[warp] = tied, s.warp_count[warp] = count;
+    __syncthreads();
+    if (threadIdx.x < (unsigned)ctas) {
+      Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
+      unsigned long long m = 0;
+      uint32_t t = 0, c = 0;
+      for (int w = 0; w < WARPS; ++w) m += s.warp_mass[w], t += s.warp_ties[w], c += s.warp_count[w];
+      o->mass[rank] = m;
+      o->ties[rank] = t;
+      o->count[rank] = c;
     }
-    const float uf = p.uniform[r];
-    const double u = uf > 0.f ? (double)fminf(uf, 0.99999994f) : 0.0;
-    uint64_t target = (uint64_t)(u * (double)total);  // the first running sum above it
-    if (target >= total) target = total - 1;
-    if (before <= target && target < before + mine) {
-      uint64_t run = before;
-      uint32_t tie_run = 0;
-      for (uint32_t t0 = s0; t0 < s1; t0 += 32) {
-        const uint32_t t = t0 + lane;
-        const float v = t < s1 ? row[t] : 0.f;
-        const uint32_t key = t < s1 ? key_of(v) : 0;
-        const bool tie = key && key == tau;
-        const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-        uint64_t w = 0;
-        if (tie) w = tie_run + __popc(tie_mask & ((1u << lane) - 1)) < mine_ties ? wt : 0;
-        else if (key > tau) {
-          w = weigh(v);
-          if (w < least && key != top) w = 0;
-        }
-        tie_run += __popc(tie_mask);
-        uint64_t s = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t up = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += up;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, w && run + s > target);
-        if (hit) {
-          if (lane == __ffs(hit) - 1) {
-            if (p.ids) p.ids[r] = (float)t;
-            if (p.logprob) p.logprob[r] = (float)(log((double)w) - log((double)total));
-          }
+  }
+  cluster.sync();  // (the last one: nothing remote is touched after it)
+  unsigned long long total = 0, before = 0, left = ties;
+  uint32_t count = 0, mine_ties = 0;
+  for (int c = 0; c < ctas; ++c) {
+    if (c == rank) {  // this warp's place in the order
+      unsigned long long l = left;
+      before = total;
+      for (int w = 0; w < WARPS; ++w) {
+        const unsigned long long take = l < s.warp_ties[w] ? l : s.warp_ties[w];
+        if (w == warp) {
+          mine_ties = (uint32_t)take;
           break;
         }
-        run += __shfl_sync(0xffffffffu, s, 31);
+        before += s.warp_mass[w] + take * wt;
+        l -= take;
       }
     }
-    if (threadIdx.x == 0 && p.kept) p.kept[r] = (uint32_t)(count + (ties - left));
+    const unsigned long long take = left < s.ties[c] ? left : s.ties[c];
+    total += s.mass[c] + take * wt;
+    count += s.count[c] + (uint32_t)take;
+    left -= take;
+  }
+  unsigned long long target = (unsigned long long)(u * (double)total);  // the first sum above it
+  if (target >= total) target = total - 1;
+  if (before > target || target >= before + s.warp_mass[warp] + mine_ties * wt) return;
+  unsigned long long run = before;
+  uint32_t tie_run = 0;
+  for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
+    const uint32_t i = i0 + lane;
+    const float v = i < s1 ? row.v[i] : 0.f;
+    const uint32_t key = i < s1 ? key_of(v) : 0;
+    const bool tie = key && key == tau;
+    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
+    unsigned long long w = 0;
+    if (tie) w = tie_run + __popc(tie_mask & ((1u << lane) - 1)) < mine_ties ? wt : 0;
+    else if (key > tau) w = kept(v, key);
+    tie_run += __popc(tie_mask);
+    unsigned long long sum = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, w && run + sum > target);
+    if (hit) {
+      if (lane == __ffs(hit) - 1)
+        answer(p, r, (float)(row.first + i), (float)(log((double)w) - log((double)total)), count);
+      return;
+    }
+    run += __shfl_sync(0xffffffffu, sum, 31);
   }
 }
 
 uint64_t sample_scratch_bytes(uint64_t, uint64_t) { return 0; }
 
 cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
-  mgb_sample_kernel<<<(unsigned)(a.rows < 65535 ? a.rows : 65535), THREADS, 0, stream>>>(a);
-  return cudaGetLastError();
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const int sms = device_sms(dev);
+  // CTAs of a row: parts of up to 16,384 tokens (64 KB: three CTAs an SM), and,
+  // with few rows, as many as leave each 2,048
+  uint32_t ctas = 1;
+  while (ctas < MOST_CTAS && (ceil_div(a.vocab, ctas) > 16384 ||
+                              (a.rows * ctas * 2 <= (uint64_t)sms && ceil_div(a.vocab, 2 * ctas) >= 2048)))
+    ctas *= 2;
+  const uint32_t chunk = (uint32_t)(ceil_div(ceil_div(a.vocab, ctas), 4) * 4);
+  const bool staged = chunk <= 48 * 1024;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = staged ? chunk * 4 : 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  auto *kern = staged ? mgb_sample_kernel<true> : mgb_sample_kernel<false>;
+  if (staged) {  // the opt-in is an attribute of the function on a device: once each
+    static std::atomic<uint64_t> opted{0};
+    if (!(opted.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 196608);
+      if (e != cudaSuccess) return e;
+      opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+    }
+  }
+  // a grid holds 2^31 - 1 CTAs
+  const uint64_t most = 0x7FFFFFFFull / ctas;
+  for (uint64_t r = 0; r < a.rows; r += most) {
+    SampleArgs part = a;
+    part.rows = a.rows - r < most ? a.rows - r : most;
+    part.logits += r * a.ld;
+    for (const float **q : {&part.temperature, &part.top_k, &part.top_p, &part.min_p, &part.uniform})
+      if (*q) *q += r;
+    if (part.ids) part.ids += r;
+    if (part.logprob) part.logprob += r;
+    if (part.kept) part.kept += r;
+    cfg.gridDim = dim3((unsigned)(part.rows * ctas));
+    e = cudaLaunchKernelEx(&cfg, kern, part, chunk);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace mgb
