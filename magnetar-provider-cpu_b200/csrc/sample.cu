@@ -10,9 +10,10 @@
 // A row is read once: a cluster of CTAs holds it in shared memory (a few CTAs an
 // SM, so that one row's loads overlap another's arithmetic), and the CTAs agree
 // on one number after another through distributed shared memory.
-//  - Small top_k: every CTA finds its own candidates (the bins of a histogram of
-//    the distance to its largest logit that hold its first top_k tokens), the
-//    first CTA sorts them all and does the rest: one cluster barrier a row.
+//  - Small top_k: the top_k-th largest of a CTA's 256 threads' own largest logits
+//    is a bound that at least top_k of its tokens reach and few others do; the
+//    first CTA sorts the tokens that reach their CTA's and does the rest: one
+//    cluster barrier a row.
 //  - Otherwise tau is searched by histograms of counts (top-k) or of mass (top-p)
 //    over ever smaller key ranges: first by distance to the largest logit, where
 //    tokens spread evenly over the bins, then by key.
@@ -76,6 +77,9 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // The weight function of a row.
 struct Weigh {
   float top, chi, clo;  // the largest logit; log2(e) / T as the sum of two floats
+  const uint2 *pow2;    // g_pow2 in shared memory (lanes look different entries up,
+                        // which constant memory serves one after the other: 562
+                        // against PLACEHOLDER us for 256 rows of 128,256)
   __device__ __forceinline__ uint64_t operator()(float v) const {
     if (__isinff(top)) return v == top ? 1ull << ONE_BITS : 0;  // +inf
     // v - top = d + e exactly; times (chi + clo): p + r
@@ -95,9 +99,10 @@ struct Weigh {
     q = fmaf(s, q, 0.693147180559945f);
     q *= s;
     const int ni = (int)n, j = ni & 63, N = ni >> 6;
-    const float hi = (float)g_pow2.hi[j] * 1.1920929e-7f;  // exact
-    const int32_t tail = __float2int_rn(fmaf(hi, q, g_pow2.lo[j]) * 68719476736.f);  // 2^36
-    const uint64_t one = ((uint64_t)g_pow2.hi[j] << (ONE_BITS - 23)) +
+    const uint2 power = pow2[j];
+    const float hi = (float)power.x * 1.1920929e-7f;  // exact
+    const int32_t tail = __float2int_rn(fmaf(hi, q, __uint_as_float(power.y)) * 68719476736.f);  // 2^36
+    const uint64_t one = ((uint64_t)power.x << (ONE_BITS - 23)) +
                          (uint64_t)((int64_t)tail << (ONE_BITS - 36));
     if (N >= 0) return one << N;  // s may round p up to 0
     return (one + (1ull << (-N - 1))) >> -N;
@@ -120,19 +125,21 @@ __device__ __forceinline__ int distance_bin(float top, float v) {
 }
 
 struct Shared {
-  unsigned long long hist[BINS];        // counts or masses; the sort's buffer
-  unsigned long long list[LIST];        // first CTA: its cluster's candidates / histogram
+  unsigned long long list[LIST];        // the first CTA: its cluster's candidates; a histogram
+  alignas(8) uint32_t part[3][BINS];    // a histogram as it is filled (32-bit atomics are native:
+                                        // masses in three digits); the sort's buffer
   unsigned long long scan[WARPS];
   // what the CTAs tell each other, by rank
   unsigned long long top[MOST_CTAS];    // (key, ~index) of the largest logit
   unsigned long long mass[MOST_CTAS], cut_mass[MOST_CTAS];
   uint32_t live[MOST_CTAS], found[MOST_CTAS], ties[MOST_CTAS], count[MOST_CTAS];
   // the first CTA's answers
-  unsigned long long above;
+  unsigned long long found_above;
   uint32_t lo, hi;
   // of the CTA
   unsigned long long warp_mass[WARPS];
-  uint32_t warp_ties[WARPS], warp_count[WARPS], taken, bin;
+  unsigned long long above;
+  uint32_t warp_ties[WARPS], warp_count[WARPS], own[THREADS], taken, bin;
 };
 
 __device__ __forceinline__ unsigned long long block_max(unsigned long long v, Shared &s) {
@@ -197,6 +204,11 @@ struct Row {
   uint32_t top_key;
 };
 
+// A mass in three digits of a histogram: a CTA's part of at most 2^17 tokens (a
+// row of 2^20 in 8 CTAs) keeps the sums of 15-bit digits below 2^32; a mass is
+// below 2^45.
+constexpr int DIGIT = 15;
+
 // The largest key in [lo, hi] at which the count (MASS: the mass) of the keys from
 // hi down to it reaches `target` (>= 1, at most what [lo, hi] holds); above: the
 // count or mass of the keys over it.  The whole cluster.
@@ -210,29 +222,48 @@ __device__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t hi, unsigned 
   while (lo < hi) {
     int shift = 0;
     while (((hi - lo) >> shift) >= BINS) ++shift;
-    for (int i = threadIdx.x; i < BINS; i += THREADS) {
-      s.hist[i] = 0;
-      if (rank == 0 && ctas > 1) s.list[i] = 0;  // the cluster's histogram
-    }
-    cluster.sync();
+    for (int i = threadIdx.x; i < BINS; i += THREADS)
+#pragma unroll
+      for (int d = 0; d < (MASS ? 3 : 1); ++d) s.part[d][i] = 0;
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
       const float v = row.v[i];
       const uint32_t key = key_of(v);
       if (key < lo || key > hi) continue;
       const int b = linear ? distance_bin(row.top, v) : (int)((hi - key) >> shift);
-      atomicAdd(&s.hist[b], MASS ? (unsigned long long)weigh(v) : 1ull);
+      if (MASS) {
+        const uint64_t w = weigh(v);
+        const uint32_t d0 = (uint32_t)w & ((1u << DIGIT) - 1), d1 = (uint32_t)(w >> DIGIT) & ((1u << DIGIT) - 1),
+                       d2 = (uint32_t)(w >> (2 * DIGIT));
+        if (d0) atomicAdd(&s.part[0][b], d0);
+        if (d1) atomicAdd(&s.part[1][b], d1);
+        if (d2) atomicAdd(&s.part[2][b], d2);
+      } else {
+        atomicAdd(&s.part[0][b], 1u);
+      }
     }
     __syncthreads();
-    if (ctas > 1) {
-      unsigned long long *all = cluster.map_shared_rank(s.list, 0);
-      for (int i = threadIdx.x; i < BINS; i += THREADS)
-        if (s.hist[i]) atomicAdd(&all[i], s.hist[i]);
-      cluster.sync();
-    }
+    for (int i = threadIdx.x; i < BINS; i += THREADS)
+      s.list[i] = MASS ? s.part[0][i] + ((unsigned long long)s.part[1][i] << DIGIT) +
+                             ((unsigned long long)s.part[2][i] << (2 * DIGIT))
+                       : s.part[0][i];
+    cluster.sync();
     if (rank == 0) {
+      unsigned long long c[BINS / THREADS];
+#pragma unroll
+      for (int j = 0; j < BINS / THREADS; ++j) c[j] = 0;
+      for (int o = 0; o < ctas; ++o) {
+        const unsigned long long *h = cluster.map_shared_rank(s.list, o);
+#pragma unroll
+        for (int j = 0; j < BINS / THREADS; ++j) c[j] += h[j * THREADS + threadIdx.x];
+      }
+      unsigned long long *all = reinterpret_cast<unsigned long long *>(s.part[0]);  // [BINS]: two of three
+#pragma unroll
+      for (int j = 0; j < BINS / THREADS; ++j) all[j * THREADS + threadIdx.x] = c[j];
+      __syncthreads();
       int bin;
       unsigned long long before;
-      find_bin(ctas > 1 ? s.list : s.hist, target - above, s, bin, before);
+      find_bin(all, target - above, s, bin, before);
       if (threadIdx.x < (unsigned)ctas) {
         uint32_t nlo = lo, nhi = hi;
         if (linear) {
@@ -256,13 +287,13 @@ __device__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t hi, unsigned 
         Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
         o->lo = nlo;
         o->hi = nhi;
-        o->above = above + before;
+        o->found_above = above + before;
       }
     }
     cluster.sync();
     lo = s.lo;
     hi = s.hi;
-    above = s.above;
+    above = s.found_above;
     linear = false;
   }
   __syncthreads();
@@ -281,7 +312,9 @@ __device__ __forceinline__ void answer(const SampleArgs &p, uint64_t r, float id
 template <bool STAGED>
 __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs p, uint32_t chunk) {
   __shared__ Shared s;
+  __shared__ uint2 pow2[64];
   extern __shared__ __align__(16) float data[];
+  if (threadIdx.x < 64) pow2[threadIdx.x] = make_uint2(g_pow2.hi[threadIdx.x], __float_as_uint(g_pow2.lo[threadIdx.x]));
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -333,6 +366,7 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
     }
   }
   row.v = STAGED ? data : src;
+  const uint32_t own = (uint32_t)(best >> 32);  // this thread's largest key
   best = block_max(best, s);
   {
     unsigned long long total;
@@ -343,40 +377,38 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
   cluster.barrier_wait();
 
   // small top_k: this CTA's candidates, to the first CTA's list
+  static_assert(LIST <= BINS && BINS * 8 <= sizeof(s.part), "the sort's buffer");
   const uint32_t room = LIST / ctas;
   const bool few = !greedy && kf >= 1.f && kf < (float)MOST_TOP_K + 1.f && kf < (float)room + 1.f;
   uint32_t found = 0xFFFFFFFFu;  // none sent
   if (few) {
     const uint32_t k = (uint32_t)kf;
-    const float top = value_of((uint32_t)(best >> 32));
-    int last = BINS;
+    uint32_t bound = 1;  // every live token
     if (threadIdx.x == 0) s.taken = 0;
-    if (live > room && !__isinff(top)) {
-      for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
+    if (live > room) {
+      s.own[threadIdx.x] = own;
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
-        const float v = row.v[i];
-        // (the last bins do not matter: k <= room < live)
-        if (key_of(v)) atomicAdd(&s.hist[distance_bin(top, v)], 1ull);
-      }
+      // the k-th largest of the threads' largest keys (k <= THREADS): the one with
+      // fewer than k above it and k at least as large
+      uint32_t over = 0, level = 0;
+#pragma unroll 8
+      for (int j = 0; j < THREADS; ++j) over += s.own[j] > own, level += s.own[j] == own;
+      if (over < k && over + level >= k) s.bin = own;  // (equal keys agree)
       __syncthreads();
-      unsigned long long before;
-      find_bin(s.hist, k, s, last, before);
-      found = (uint32_t)(before + s.hist[last]);
+      bound = max(s.bin, 1u);
     } else {
-      found = live;
       __syncthreads();
     }
-    if (found <= room) {
-      unsigned long long *list = cluster.map_shared_rank(s.list, 0) + rank * room;
-      for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
-        const float v = row.v[i];
-        const uint32_t key = key_of(v);
-        if (key && (last == BINS || distance_bin(top, v) <= last))
-          list[atomicAdd(&s.taken, 1u)] =
-              ((unsigned long long)key << 32) | (0xFFFFFFFFu - (row.first + i));
+    unsigned long long *list = cluster.map_shared_rank(s.list, 0) + rank * room;
+    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
+      const uint32_t key = key_of(row.v[i]);
+      if (key >= bound) {
+        const uint32_t at = atomicAdd(&s.taken, 1u);
+        if (at < room) list[at] = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (row.first + i));
       }
     }
+    __syncthreads();
+    found = s.taken;  // (above room: too many tokens reach the bound)
   }
   if (threadIdx.x < (unsigned)ctas) {
     Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
@@ -403,6 +435,7 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
   row.top = value_of(row.top_key);
   Weigh weigh;
   weigh.top = row.top;
+  weigh.pow2 = pow2;
   {
     const double c = fmin(1.4426950408889634 / (double)temp, 1e30);  // 1 / T stays finite
     weigh.chi = (float)c;
@@ -422,27 +455,28 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
   if (listed) {
     // ---- the first CTA sorts the candidates, best first, and does the rest
     if (rank) return;
+    unsigned long long *sorted = reinterpret_cast<unsigned long long *>(s.part[0]);  // [LIST]: two of three
     uint32_t n = 0;
     for (int c = 0; c < ctas; ++c) {
-      for (uint32_t i = threadIdx.x; i < s.found[c]; i += THREADS) s.hist[n + i] = s.list[c * room + i];
+      for (uint32_t i = threadIdx.x; i < s.found[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
       n += s.found[c];
     }
     uint32_t size = 2;
     while (size < n) size <<= 1;
-    for (uint32_t i = n + threadIdx.x; i < size; i += THREADS) s.hist[i] = 0;
+    for (uint32_t i = n + threadIdx.x; i < size; i += THREADS) sorted[i] = 0;
     __syncthreads();
     for (uint32_t k = 2; k <= size; k <<= 1)
       for (uint32_t j = k >> 1; j; j >>= 1) {
         for (uint32_t i = threadIdx.x; i < size / 2; i += THREADS) {
           const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
-          const unsigned long long x = s.hist[a], y = s.hist[b];
-          if ((x < y) == ((a & k) == 0)) s.hist[a] = y, s.hist[b] = x;
+          const unsigned long long x = sorted[a], y = sorted[b];
+          if ((x < y) == ((a & k) == 0)) sorted[a] = y, sorted[b] = x;
         }
         __syncthreads();
       }
     const uint32_t i = threadIdx.x;
     n = min(n, (uint32_t)kf);  // <= THREADS
-    const unsigned long long mine = i < n ? s.hist[i] : 0;
+    const unsigned long long mine = i < n ? sorted[i] : 0;
     const uint32_t key = (uint32_t)(mine >> 32), token = 0xFFFFFFFFu - (uint32_t)mine;
     const unsigned long long w = i < n ? weigh(value_of(key)) : 0;
     unsigned long long total;
@@ -458,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
     if (i < n) {
       unsigned long long upto = 0;  // the kept mass of the tokens up to this one
       for (uint32_t j = 0; j < n; ++j)
-        if ((uint32_t)s.hist[j] >= (uint32_t)mine) upto += s.list[j];
+        if ((uint32_t)sorted[j] >= (uint32_t)mine) upto += s.list[j];
       if (upto > target && upto - w <= target)
         answer(p, r, (float)token, (float)(log((double)w) - log((double)total)), n);
     }
