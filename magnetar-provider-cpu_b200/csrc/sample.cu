@@ -77,125 +77,167 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // The weight function of a row.
 struct Weigh {
   float top, chi, clo;  // the largest logit; log2(e) / T as the sum of two floats
-  const uint2 *pow2;    // g_pow2 in shared memory (lanes look different entries up,
-                        // which constant memory serves one after the other: 562
-                        // against PLACEHOLDER us for 256 rows of 128,256)
+  const float2 *pow2;   // g_pow2 in shared memory (lanes look different entries up,
+                        // which constant memory serves one after the other: 256 rows
+                        // of 128,256 without cuts took 562 us, then 261)
   __device__ __forceinline__ uint64_t operator()(float v) const {
     if (__isinff(top)) return v == top ? 1ull << ONE_BITS : 0;  // +inf
     // v - top = d + e exactly; times (chi + clo): p + r
     const float d = v - top, b = d - v;
     const float e = (v - (d - b)) + (-top - b);
     const float p = d * chi;
-    if (!(p > -60.f)) return 0;  // below half a unit (also v = -inf, NaN)
+    if (!(p > -44.f)) return 0;  // below half a unit (also v = -inf, NaN)
     float r = fmaf(d, chi, -p);
     r = fmaf(d, clo, r);
     r = fmaf(e, chi, r);
-    // 2^(p + r) = 2^N 2^(j / 64) 2^s, |s| <= 1/128; the last factor by its
-    // Taylor polynomial (next term 2^-44)
-    const float n = rintf(p * 64.f);
+    // 2^(p + r) = 2^N 2^(j / 64) 2^s, |s| <= 1/128; the last factor by its Taylor
+    // polynomial (next term 2^-44).  (Rounding by adding 1.5 2^23 leaves the integer
+    // in the float's bits: the conversion units are far slower than the arithmetic.)
+    const float big = fmaf(p, 64.f, 12582912.f), n = big - 12582912.f;
     const float s = fmaf(n, -0.015625f, p) + r;
     float q = fmaf(s, 0.009618129107628f, 0.055504108664822f);
     q = fmaf(s, q, 0.240226506959101f);
     q = fmaf(s, q, 0.693147180559945f);
     q *= s;
-    const int ni = (int)n, j = ni & 63, N = ni >> 6;
-    const uint2 power = pow2[j];
-    const float hi = (float)power.x * 1.1920929e-7f;  // exact
-    const int32_t tail = __float2int_rn(fmaf(hi, q, __uint_as_float(power.y)) * 68719476736.f);  // 2^36
-    const uint64_t one = ((uint64_t)power.x << (ONE_BITS - 23)) +
-                         (uint64_t)((int64_t)tail << (ONE_BITS - 36));
-    if (N >= 0) return one << N;  // s may round p up to 0
-    return (one + (1ull << (-N - 1))) >> -N;
+    const int ni = __float_as_int(big) - 0x4B400000, j = ni & 63, N = ni >> 6;
+    const float2 power = pow2[j];
+    // the last two factors in units of 2^-31 (below 2)
+    const uint32_t lead = (__float_as_uint(power.x) << 8) | 0x80000000u;
+    const uint32_t one = lead + (uint32_t)__float2int_rn(fmaf(power.x, q, power.y) * 2147483648.f);
+    const int down = 31 - ONE_BITS - N;
+    if (down > 0) return ((one >> (down - 1)) + 1) >> 1;  // (down <= 32)
+    return (uint64_t)one << -down;
   }
 };
 
 constexpr int BINS = 1024;
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
 constexpr int MOST_CTAS = 8;      // of a cluster
-constexpr int LIST = 1024;        // candidates the first CTA sorts
-constexpr int MOST_TOP_K = THREADS;  // of the candidate path
+constexpr int LIST = 1024;        // tokens the first CTA sorts at most
 constexpr uint32_t LOWEST = 0x00800000u;  // the key of the lowest finite value
-constexpr float BIN_SCALE = 16.f;    // bins of the distance to the largest logit
+// A token's distance to the largest logit as a number of 20 bits, monotonic: 1,024
+// bins of 1/16, of 1,024 parts each.
+constexpr float CODE_SCALE = 16384.f;
+constexpr int CODE_MOST = (1 << 20) - 1;
 
-// The bin of a live logit by its distance to the largest one: monotonic.
-__device__ __forceinline__ int distance_bin(float top, float v) {
-  const int b = (int)((top - v) * BIN_SCALE);  // (saturates)
-  return b < BINS - 1 ? b : BINS - 1;
+typedef unsigned long long u64;  // what atomicAdd and shuffles take
+
+// A token in the order: larger is earlier.
+__device__ __forceinline__ u64 place_of(uint32_t key, uint32_t index) {
+  return ((u64)key << 32) | (0xFFFFFFFFu - index);
+}
+__device__ __forceinline__ uint32_t index_of(u64 place) { return 0xFFFFFFFFu - (uint32_t)place; }
+
+__device__ __forceinline__ int code_of(float top, float v) {
+  const int c = (int)((top - v) * CODE_SCALE);  // (saturates)
+  return c < CODE_MOST ? c : CODE_MOST;
 }
 
+template <int THREADS>
 struct Shared {
-  unsigned long long list[LIST];        // the first CTA: its cluster's candidates; a histogram
+  static constexpr int WARPS = THREADS / 32;
+  u64 list[LIST];                       // the first CTA: its cluster's tokens; a histogram
   alignas(8) uint32_t part[3][BINS];    // a histogram as it is filled (32-bit atomics are native:
                                         // masses in three digits); the sort's buffer
-  unsigned long long scan[WARPS];
+  u64 scan[WARPS];
   // what the CTAs tell each other, by rank
-  unsigned long long top[MOST_CTAS];    // (key, ~index) of the largest logit
-  unsigned long long mass[MOST_CTAS], cut_mass[MOST_CTAS];
-  uint32_t live[MOST_CTAS], found[MOST_CTAS], ties[MOST_CTAS], count[MOST_CTAS];
+  u64 top[MOST_CTAS];                   // the place of the largest logit
+  u64 mass[MOST_CTAS];
+  uint32_t live[MOST_CTAS], found[MOST_CTAS], count[MOST_CTAS], ties[MOST_CTAS], kept[MOST_CTAS];
   // the first CTA's answers
-  unsigned long long found_above;
+  u64 found_above, cut, target;
   uint32_t lo, hi;
+  int border;
   // of the CTA
-  unsigned long long warp_mass[WARPS];
-  unsigned long long above;
+  u64 above, warp_mass[WARPS];
   uint32_t warp_ties[WARPS], warp_count[WARPS], own[THREADS], taken, bin;
 };
 
-__device__ __forceinline__ unsigned long long block_max(unsigned long long v, Shared &s) {
+template <int THREADS>
+__device__ __forceinline__ u64 block_max(u64 v, Shared<THREADS> &s) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const unsigned long long u = __shfl_xor_sync(0xffffffffu, v, o);
+    const u64 u = __shfl_xor_sync(0xffffffffu, v, o);
     v = v > u ? v : u;
   }
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) v = v > s.scan[w] ? v : s.scan[w];
+  for (int w = 0; w < THREADS / 32; ++w) v = v > s.scan[w] ? v : s.scan[w];
   return v;
 }
 
 // Inclusive sum over the CTA's threads.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, Shared &s,
-                                                         unsigned long long &total) {
+template <int THREADS>
+__device__ __forceinline__ u64 block_scan(u64 v, Shared<THREADS> &s, u64 &total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+    const u64 u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
   __syncthreads();
   if (lane == 31) s.scan[warp] = v;
   __syncthreads();
   total = 0;
-  unsigned long long before = 0;
+  u64 before = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += s.scan[w];
     total += s.scan[w];
   }
   return before + v;
 }
 
-// The first bin at which the running sum of hist reaches target, and the sum
-// before it; all threads (sums of `hist`, which 4 bins a thread).
-__device__ __forceinline__ void find_bin(const unsigned long long *hist, unsigned long long target,
-                                         Shared &s, int &bin, unsigned long long &before) {
-  unsigned long long c[BINS / THREADS], v = 0, total;
+// The first of n entries (n a multiple of THREADS) at which the running sum
+// reaches target, and the sum before it; all threads.
+template <int PER, int THREADS>
+__device__ __forceinline__ void find_entry(const u64 *e, u64 target, Shared<THREADS> &s, int &at, u64 &before) {
+  u64 c[PER], v = 0, total;
 #pragma unroll
-  for (int i = 0; i < BINS / THREADS; ++i) c[i] = hist[threadIdx.x * (BINS / THREADS) + i], v += c[i];
-  unsigned long long run = block_scan(v, s, total) - v;
+  for (int i = 0; i < PER; ++i) c[i] = e[threadIdx.x * PER + i], v += c[i];
+  u64 run = block_scan(v, s, total) - v;
 #pragma unroll
-  for (int i = 0; i < BINS / THREADS; ++i) {
-    if (run < target && run + c[i] >= target)
-      s.bin = threadIdx.x * (BINS / THREADS) + i, s.above = run;
+  for (int i = 0; i < PER; ++i) {
+    if (run < target && run + c[i] >= target) s.bin = threadIdx.x * PER + i, s.above = run;
     run += c[i];
   }
   __syncthreads();
-  bin = (int)s.bin;
+  at = (int)s.bin;
   before = s.above;
+  __syncthreads();
 }
+
+// n places (n <= LIST) into descending order, in place.
+template <int THREADS>
+__device__ __forceinline__ void sort_places(u64 *e, uint32_t n) {
+  uint32_t size = 2;
+  while (size < n) size <<= 1;
+  for (uint32_t i = n + threadIdx.x; i < size; i += THREADS) e[i] = 0;
+  __syncthreads();
+  for (uint32_t k = 2; k <= size; k <<= 1)
+    for (uint32_t j = k >> 1; j; j >>= 1) {
+      for (uint32_t i = threadIdx.x; i < size / 2; i += THREADS) {
+        const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
+        const u64 x = e[a], y = e[b];
+        if ((x < y) == ((a & k) == 0)) e[a] = y, e[b] = x;
+      }
+      __syncthreads();
+    }
+}
+
+// Whether a token's place is above a given one, without building its key.
+struct Over {
+  float v;
+  uint32_t limit;
+  __device__ __forceinline__ explicit Over(u64 place) {
+    v = place >> 32 ? value_of((uint32_t)(place >> 32)) : __int_as_float(0xff800000);
+    limit = place >> 32 ? 0xFFFFFFFFu - (uint32_t)place : 0;
+  }
+  __device__ __forceinline__ bool operator()(float x, uint32_t index) const {
+    return x > v || (x == v && index < limit);
+  }
+};
 
 struct Row {
   const float *v;      // this CTA's part of the row
@@ -204,88 +246,122 @@ struct Row {
   uint32_t top_key;
 };
 
-// A mass in three digits of a histogram: a CTA's part of at most 2^17 tokens (a
-// row of 2^20 in 8 CTAs) keeps the sums of 15-bit digits below 2^32; a mass is
-// below 2^45.
-constexpr int DIGIT = 15;
+// Calls f(logit, position) for every token of the CTA's part, 16 bytes at a time
+// where it can.
+template <int THREADS, typename F>
+__device__ __forceinline__ void for_each(const float *v, uint32_t n, const F &f) {
+  if ((reinterpret_cast<uintptr_t>(v) & 15) == 0) {
+    const uint32_t n4 = n / 4;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < n4; i += THREADS) {
+      const float4 x = reinterpret_cast<const float4 *>(v)[i];
+      f(x.x, 4 * i);
+      f(x.y, 4 * i + 1);
+      f(x.z, 4 * i + 2);
+      f(x.w, 4 * i + 3);
+    }
+    for (uint32_t i = 4 * n4 + threadIdx.x; i < n; i += THREADS) f(v[i], i);
+  } else {
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) f(v[i], i);
+  }
+}
+
+// A mass (below 2^44) in three digits of a histogram: with n tokens of a CTA, log2 n
+// below L, digits of 32 - L bits keep their sums below 2^32.  The third has 44 - 2
+// (32 - L) bits left, too many where L is above 17: it then goes into 64 bits.
+struct Digits {
+  int bits;
+  bool wide;
+  __device__ __forceinline__ explicit Digits(uint32_t n) {
+    int L = 0;
+    while ((1u << L) < n) ++L;  // n <= 2^20
+    bits = L < 15 ? 17 : 32 - L;
+    wide = L > 17;
+  }
+};
+
+// The tokens' counts (MASS: masses) by bin, summed over the cluster in the first
+// CTA's part[0..1], as u64.  bin(v, position): a token's bin, or -1.
+template <bool MASS, int THREADS, typename B>
+__device__ __forceinline__ u64 *histogram(const Row &row, const B &bin, const Weigh &weigh, Shared<THREADS> &s,
+                                          cg::cluster_group &cluster) {
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const Digits digits(row.n);
+  const int D = digits.bits;
+  const uint32_t mask = (1u << D) - 1;
+  for (int i = threadIdx.x; i < BINS; i += THREADS)
+#pragma unroll
+    for (int d = 0; d < (MASS ? 3 : 1); ++d) s.part[d][i] = 0;
+  if (MASS)
+    for (int i = threadIdx.x; i < LIST; i += THREADS) s.list[i] = 0;
+  __syncthreads();
+  for_each<THREADS>(row.v, row.n, [&](float v, uint32_t i) {
+    const int b = bin(v, i);
+    if (b < 0) return;
+    if (MASS) {
+      const uint64_t w = weigh(v);
+      const uint32_t d0 = (uint32_t)w & mask, d1 = (uint32_t)(w >> D) & mask, d2 = (uint32_t)(w >> (2 * D));
+      if (d0) atomicAdd(&s.part[0][b], d0);
+      if (d1) atomicAdd(&s.part[1][b], d1);
+      if (d2) {
+        if (digits.wide) atomicAdd(&s.list[b], (u64)d2 << (2 * D));
+        else atomicAdd(&s.part[2][b], d2);
+      }
+    } else {
+      atomicAdd(&s.part[0][b], 1u);
+    }
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += THREADS)
+    s.list[i] = MASS ? s.list[i] + s.part[0][i] + ((u64)s.part[1][i] << D) + ((u64)s.part[2][i] << (2 * D))
+                     : s.part[0][i];
+  cluster.sync();
+  u64 *all = reinterpret_cast<u64 *>(s.part[0]);  // [BINS]: two of the three
+  if (rank == 0) {
+    u64 c[BINS / THREADS];
+#pragma unroll
+    for (int j = 0; j < BINS / THREADS; ++j) c[j] = 0;
+    for (int o = 0; o < ctas; ++o) {
+      const u64 *h = cluster.map_shared_rank(s.list, o);
+#pragma unroll
+      for (int j = 0; j < BINS / THREADS; ++j) c[j] += h[j * THREADS + threadIdx.x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < BINS / THREADS; ++j) all[j * THREADS + threadIdx.x] = c[j];
+    __syncthreads();
+  }
+  return all;
+}
 
 // The largest key in [lo, hi] at which the count (MASS: the mass) of the keys from
-// hi down to it reaches `target` (>= 1, at most what [lo, hi] holds); above: the
-// count or mass of the keys over it.  The whole cluster.
-template <bool MASS>
-__device__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t hi, unsigned long long target,
-                             const Weigh &weigh, Shared &s, cg::cluster_group &cluster,
-                             unsigned long long &above) {
+// hi down to it, of places above `over`, reaches `target` (>= 1, at most what
+// there is); above: the count or mass of the keys over it.  The whole cluster.
+template <bool MASS, int THREADS>
+__device__ __noinline__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t hi, u64 over, u64 target,
+                                          const Weigh &weigh, Shared<THREADS> &s, cg::cluster_group cluster,
+                                          u64 &above) {
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  bool linear = !__isinff(row.top);
   above = 0;
   while (lo < hi) {
     int shift = 0;
     while (((hi - lo) >> shift) >= BINS) ++shift;
-    for (int i = threadIdx.x; i < BINS; i += THREADS)
-#pragma unroll
-      for (int d = 0; d < (MASS ? 3 : 1); ++d) s.part[d][i] = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
-      const float v = row.v[i];
-      const uint32_t key = key_of(v);
-      if (key < lo || key > hi) continue;
-      const int b = linear ? distance_bin(row.top, v) : (int)((hi - key) >> shift);
-      if (MASS) {
-        const uint64_t w = weigh(v);
-        const uint32_t d0 = (uint32_t)w & ((1u << DIGIT) - 1), d1 = (uint32_t)(w >> DIGIT) & ((1u << DIGIT) - 1),
-                       d2 = (uint32_t)(w >> (2 * DIGIT));
-        if (d0) atomicAdd(&s.part[0][b], d0);
-        if (d1) atomicAdd(&s.part[1][b], d1);
-        if (d2) atomicAdd(&s.part[2][b], d2);
-      } else {
-        atomicAdd(&s.part[0][b], 1u);
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += THREADS)
-      s.list[i] = MASS ? s.part[0][i] + ((unsigned long long)s.part[1][i] << DIGIT) +
-                             ((unsigned long long)s.part[2][i] << (2 * DIGIT))
-                       : s.part[0][i];
-    cluster.sync();
+    const u64 *all = histogram<MASS, THREADS>(
+        row,
+        [&](float v, uint32_t i) {
+          const uint32_t key = key_of(v);
+          return key >= lo && key <= hi && place_of(key, row.first + i) > over ? (int)((hi - key) >> shift) : -1;
+        },
+        weigh, s, cluster);
     if (rank == 0) {
-      unsigned long long c[BINS / THREADS];
-#pragma unroll
-      for (int j = 0; j < BINS / THREADS; ++j) c[j] = 0;
-      for (int o = 0; o < ctas; ++o) {
-        const unsigned long long *h = cluster.map_shared_rank(s.list, o);
-#pragma unroll
-        for (int j = 0; j < BINS / THREADS; ++j) c[j] += h[j * THREADS + threadIdx.x];
-      }
-      unsigned long long *all = reinterpret_cast<unsigned long long *>(s.part[0]);  // [BINS]: two of three
-#pragma unroll
-      for (int j = 0; j < BINS / THREADS; ++j) all[j * THREADS + threadIdx.x] = c[j];
-      __syncthreads();
       int bin;
-      unsigned long long before;
-      find_bin(all, target - above, s, bin, before);
+      u64 before;
+      find_entry<BINS / THREADS>(all, target - above, s, bin, before);
       if (threadIdx.x < (unsigned)ctas) {
-        uint32_t nlo = lo, nhi = hi;
-        if (linear) {
-          // bins fall as keys grow: the keys of the bin, by bisection
-          auto edge = [&](int b) {  // the smallest key in [lo, hi] whose bin is at most b
-            uint32_t l = lo, h = hi;
-            while (l < h) {
-              const uint32_t m = l + (h - l) / 2;
-              if (distance_bin(row.top, value_of(m)) <= b) h = m;
-              else l = m + 1;
-            }
-            return l;
-          };
-          nlo = edge(bin);
-          nhi = bin ? edge(bin - 1) - 1 : hi;
-        } else {
-          nhi = hi - ((uint32_t)bin << shift);
-          const uint32_t width = (1u << shift) - 1;
-          nlo = nhi - lo > width ? nhi - width : lo;
-        }
-        Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
-        o->lo = nlo;
+        const uint32_t nhi = hi - ((uint32_t)bin << shift), width = (1u << shift) - 1;
+        Shared<THREADS> *o = cluster.map_shared_rank(&s, threadIdx.x);
+        o->lo = nhi - lo > width ? nhi - width : lo;
         o->hi = nhi;
         o->found_above = above + before;
       }
@@ -294,10 +370,167 @@ __device__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t hi, unsigned 
     lo = s.lo;
     hi = s.hi;
     above = s.found_above;
-    linear = false;
   }
   __syncthreads();
   return hi;
+}
+
+// What is kept: the places above `over`, and `ties` tokens of key tau besides (the
+// lowest indices).
+struct Cut {
+  u64 over;
+  uint32_t tau;
+  u64 ties;
+};
+
+// The tokens of the bin `border` that are over the cut, to the first CTA's list;
+// s.count of every CTA tells how many there are.  The caller's cluster barrier
+// follows.
+template <int THREADS>
+__device__ __forceinline__ void list_token(const Row &row, uint32_t i, float v, u64 *list, uint32_t room,
+                                           Shared<THREADS> &s) {
+  const uint32_t at = atomicAdd(&s.taken, 1u);
+  if (at < room) list[at] = place_of(key_of(v), row.first + i);
+}
+
+// The first CTA: its cluster's list, best first, in part[0..1]; returns their number.
+template <int THREADS>
+__device__ __forceinline__ uint32_t sort_list(int ctas, uint32_t room, Shared<THREADS> &s) {
+  u64 *sorted = reinterpret_cast<u64 *>(s.part[0]);
+  uint32_t n = 0;
+  for (int c = 0; c < ctas; ++c) {
+    for (uint32_t i = threadIdx.x; i < s.count[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
+    n += s.count[c];
+  }
+  sort_places<THREADS>(sorted, n);
+  return n;
+}
+
+// Where a border cannot be listed: the key at which the count (MASS: the mass) of
+// what is kept so far reaches target, and how many of its tokens stay.
+template <bool MASS, int THREADS>
+__device__ __noinline__ void cut_by_key(const Row &row, u64 target, const Weigh &weigh, Shared<THREADS> &s,
+                                        cg::cluster_group cluster, Cut &cut) {
+  u64 above;
+  const uint32_t lo = cut.ties ? cut.tau : LOWEST;
+  const uint32_t key = find_key<MASS, THREADS>(row, lo, row.top_key, cut.ties ? 0 : cut.over, target, weigh, s,
+                                               cluster, above);
+  const u64 w = MASS ? weigh(value_of(key)) : 1;
+  u64 need = w ? (target - above + w - 1) / w : 1;
+  if (cut.ties && key == cut.tau && cut.ties < need) need = cut.ties;
+  cut.tau = key;
+  cut.ties = need;
+  cut.over = place_of(key, 0);  // every place of a larger key
+}
+
+// Cuts behind the token at which the count (MASS: the mass) of what is kept so
+// far, in order, reaches its target: target_of(all of it), at least 1.  Histograms
+// of the distance to the largest logit find the border's bin, and part of the bin
+// where that holds too many tokens; the first CTA sorts those.  The whole cluster.
+template <bool MASS, int THREADS, typename F>
+__device__ void cut_at(const Row &row, const F &target_of, const Weigh &weigh, Shared<THREADS> &s,
+                       cg::cluster_group cluster, Cut &cut) {
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const uint32_t room = LIST / ctas;
+  const Over over(cut.over);
+  // the first CTA finds the entry of its histogram and tells all; the total counts
+  // where it is the first level's
+  auto tell = [&](const u64 *all, bool first_level) {
+    if (rank == 0) {
+      u64 c[BINS / THREADS], v = 0, total;
+#pragma unroll
+      for (int i = 0; i < BINS / THREADS; ++i) c[i] = all[threadIdx.x * (BINS / THREADS) + i], v += c[i];
+      block_scan(v, s, total);
+      if (cut.ties) total += cut.ties * (MASS ? weigh(value_of(cut.tau)) : 1);
+      const u64 target = first_level ? target_of(total) : s.target;
+      const u64 above = first_level ? 0 : s.found_above;
+      __syncthreads();
+      int bin;
+      u64 before;
+      find_entry<BINS / THREADS>(all, target - above, s, bin, before);
+      if (threadIdx.x < (unsigned)ctas) {
+        Shared<THREADS> *o = cluster.map_shared_rank(&s, threadIdx.x);
+        o->border = bin;
+        o->found_above = above + before;
+        o->target = target;
+      }
+    }
+    if (threadIdx.x == 0) s.taken = 0;
+    cluster.sync();
+  };
+  if (cut.ties == 0 && !__isinff(row.top)) {
+    tell(histogram<MASS, THREADS>(
+             row, [&](float v, uint32_t i) { return over(v, row.first + i) ? code_of(row.top, v) >> 10 : -1; },
+             weigh, s, cluster),
+         true);
+    int border = s.border, part = -1;
+    for (int level = 0; level < 2; ++level) {
+      auto inside = [&](float v, uint32_t i) {
+        if (!over(v, row.first + i)) return false;
+        const int c = code_of(row.top, v);
+        return part < 0 ? c >> 10 == border : c == part;
+      };
+      u64 *list = cluster.map_shared_rank(s.list, 0) + rank * room;
+      for_each<THREADS>(row.v, row.n, [&](float v, uint32_t i) {
+        if (!inside(v, i)) return;
+        const uint32_t at = atomicAdd(&s.taken, 1u);
+        if (at < room) list[at] = place_of(key_of(v), row.first + i);
+      });
+      __syncthreads();
+      if (threadIdx.x < (unsigned)ctas) cluster.map_shared_rank(&s, threadIdx.x)->count[rank] = s.taken;
+      cluster.sync();
+      bool listed = true;
+      for (int c = 0; c < ctas; ++c) listed = listed && s.count[c] <= room;
+      if (listed) {
+        if (rank == 0) {
+          u64 *sorted = reinterpret_cast<u64 *>(s.part[0]);
+          uint32_t n = 0;
+          for (int c = 0; c < ctas; ++c) {
+            for (uint32_t i = threadIdx.x; i < s.count[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
+            n += s.count[c];
+          }
+          sort_places<THREADS>(sorted, n);
+          for (uint32_t i = threadIdx.x; i < LIST; i += THREADS)
+            s.list[i] = i >= n ? 0 : MASS ? weigh(value_of((uint32_t)(sorted[i] >> 32))) : 1;
+          __syncthreads();
+          int at;
+          u64 unused;
+          find_entry<LIST / THREADS>(s.list, s.target - s.found_above, s, at, unused);
+          if (threadIdx.x < (unsigned)ctas) cluster.map_shared_rank(&s, threadIdx.x)->cut = sorted[at] - 1;
+        }
+        cluster.sync();
+        cut.over = s.cut;
+        __syncthreads();
+        return;
+      }
+      if (level) break;
+      tell(histogram<MASS, THREADS>(
+               row,
+               [&](float v, uint32_t i) {
+                 if (!over(v, row.first + i)) return -1;
+                 const int c = code_of(row.top, v);
+                 return c >> 10 == border ? c & 1023 : -1;
+               },
+               weigh, s, cluster),
+           false);
+      part = (border << 10) | s.border;
+    }
+  } else {
+    tell(histogram<MASS, THREADS>(
+             row, [&](float v, uint32_t i) { return over(v, row.first + i) ? 0 : -1; }, weigh, s, cluster),
+         true);
+  }
+  // too many tokens in one place: by keys
+  const u64 target = s.target;
+  u64 above;
+  const uint32_t key = find_key<MASS, THREADS>(row, cut.ties ? cut.tau : LOWEST, row.top_key,
+                                               cut.ties ? 0 : cut.over, target, weigh, s, cluster, above);
+  const u64 w = MASS ? weigh(value_of(key)) : 1;
+  u64 need = w ? (target - above + w - 1) / w : 1;
+  if (cut.ties && key == cut.tau && cut.ties < need) need = cut.ties;
+  cut.tau = key;
+  cut.ties = need;
+  cut.over = place_of(key, 0);  // every place of a larger key
 }
 
 __device__ __forceinline__ void answer(const SampleArgs &p, uint64_t r, float id, float logprob,
@@ -308,13 +541,15 @@ __device__ __forceinline__ void answer(const SampleArgs &p, uint64_t r, float id
 }
 
 // One row a cluster.  STAGED: each CTA's part of the row is in its shared memory;
-// otherwise (vocabularies that do not fit) it is read from global memory again.
-template <bool STAGED>
-__global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs p, uint32_t chunk) {
-  __shared__ Shared s;
-  __shared__ uint2 pow2[64];
+// otherwise it is read again (from L2, mostly).
+template <int THREADS, bool STAGED>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
+    mgb_sample_kernel(const SampleArgs p, uint32_t chunk) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ Shared<THREADS> s;
+  __shared__ float2 pow2[64];
   extern __shared__ __align__(16) float data[];
-  if (threadIdx.x < 64) pow2[threadIdx.x] = make_uint2(g_pow2.hi[threadIdx.x], __float_as_uint(g_pow2.lo[threadIdx.x]));
+  if (threadIdx.x < 64) pow2[threadIdx.x] = make_float2((float)g_pow2.hi[threadIdx.x] * 1.1920929e-7f, g_pow2.lo[threadIdx.x]);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -332,14 +567,12 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
   const bool greedy = !(temp > 0.f) || !p.uniform;
   const float kf = p.top_k ? p.top_k[r] : 0.f;
 
-  // the CTA's largest (key, ~index) and live tokens; the row comes in once
-  unsigned long long best = 0;
-  uint32_t live = 0;
+  // the thread's largest key and its position, and the live tokens
+  uint32_t own = 0, own_at = 0, live = 0;
   auto see = [&](float v, uint32_t i) {
     const uint32_t key = key_of(v);
     live += key != 0;
-    const unsigned long long c = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (row.first + i));
-    if (key && c > best) best = c;
+    if (key > own) own = key, own_at = i;  // (positions rise: the first of equals stays)
   };
   if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
     const uint32_t n4 = row.n / 4;
@@ -366,20 +599,18 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
     }
   }
   row.v = STAGED ? data : src;
-  const uint32_t own = (uint32_t)(best >> 32);  // this thread's largest key
-  best = block_max(best, s);
+  u64 best = block_max(own ? place_of(own, row.first + own_at) : 0ull, s);
   {
-    unsigned long long total;
+    u64 total;
     block_scan(live, s, total);
     live = (uint32_t)total;
   }
-
   cluster.barrier_wait();
 
   // small top_k: this CTA's candidates, to the first CTA's list
   static_assert(LIST <= BINS && BINS * 8 <= sizeof(s.part), "the sort's buffer");
   const uint32_t room = LIST / ctas;
-  const bool few = !greedy && kf >= 1.f && kf < (float)MOST_TOP_K + 1.f && kf < (float)room + 1.f;
+  const bool few = !greedy && kf >= 1.f && kf < 257.f && kf < (float)room + 1.f;
   uint32_t found = 0xFFFFFFFFu;  // none sent
   if (few) {
     const uint32_t k = (uint32_t)kf;
@@ -399,19 +630,19 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
     } else {
       __syncthreads();
     }
-    unsigned long long *list = cluster.map_shared_rank(s.list, 0) + rank * room;
-    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
-      const uint32_t key = key_of(row.v[i]);
+    u64 *list = cluster.map_shared_rank(s.list, 0) + rank * room;
+    for_each<THREADS>(row.v, row.n, [&](float v, uint32_t i) {
+      const uint32_t key = key_of(v);
       if (key >= bound) {
         const uint32_t at = atomicAdd(&s.taken, 1u);
-        if (at < room) list[at] = ((unsigned long long)key << 32) | (0xFFFFFFFFu - (row.first + i));
+        if (at < room) list[at] = place_of(key, row.first + i);
       }
-    }
+    });
     __syncthreads();
     found = s.taken;  // (above room: too many tokens reach the bound)
   }
   if (threadIdx.x < (unsigned)ctas) {
-    Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
+    Shared<THREADS> *o = cluster.map_shared_rank(&s, threadIdx.x);
     o->top[rank] = best;
     o->live[rank] = live;
     o->found[rank] = found;
@@ -428,7 +659,7 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
   if (!row.top_key || greedy) {
     if (rank == 0 && threadIdx.x == 0) {
       if (!row.top_key) answer(p, r, -1.f, __int_as_float(0xff800000), 0);
-      else answer(p, r, (float)(0xFFFFFFFFu - (uint32_t)best), 0.f, 1);
+      else answer(p, r, (float)index_of(best), 0.f, 1);
     }
     return;
   }
@@ -444,111 +675,97 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
   const float pf = p.top_p ? p.top_p[r] : 1.f, mf = p.min_p ? p.min_p[r] : 0.f;
   const float uf = p.uniform[r];
   const double u = uf > 0.f ? (double)fminf(uf, 0.99999994f) : 0.0;
-  const unsigned long long least =
-      mf > 0.f ? (unsigned long long)ceil((double)fminf(mf, 1.f) * (double)(1ull << ONE_BITS)) : 0;
-  auto mass_target = [&](unsigned long long total) {  // of top-p, in [1, total]
+  const u64 least = mf > 0.f ? (u64)ceil((double)fminf(mf, 1.f) * (double)(1ull << ONE_BITS)) : 0;
+  auto mass_target = [&](u64 total) {  // of top-p, in [1, total]
     const double want = ceil((double)fmaxf(pf, 0.f) * (double)total);
-    const unsigned long long t = want < 1.0 ? 1ull : (unsigned long long)want;
+    const u64 t = want < 1.0 ? 1ull : (u64)want;
     return t < total ? t : total;
   };
 
   if (listed) {
     // ---- the first CTA sorts the candidates, best first, and does the rest
     if (rank) return;
-    unsigned long long *sorted = reinterpret_cast<unsigned long long *>(s.part[0]);  // [LIST]: two of three
+    u64 *sorted = reinterpret_cast<u64 *>(s.part[0]);  // [LIST]: two of three
     uint32_t n = 0;
     for (int c = 0; c < ctas; ++c) {
       for (uint32_t i = threadIdx.x; i < s.found[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
       n += s.found[c];
     }
-    uint32_t size = 2;
-    while (size < n) size <<= 1;
-    for (uint32_t i = n + threadIdx.x; i < size; i += THREADS) sorted[i] = 0;
-    __syncthreads();
-    for (uint32_t k = 2; k <= size; k <<= 1)
-      for (uint32_t j = k >> 1; j; j >>= 1) {
-        for (uint32_t i = threadIdx.x; i < size / 2; i += THREADS) {
-          const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
-          const unsigned long long x = sorted[a], y = sorted[b];
-          if ((x < y) == ((a & k) == 0)) sorted[a] = y, sorted[b] = x;
-        }
-        __syncthreads();
-      }
+    sort_places<THREADS>(sorted, n);
     const uint32_t i = threadIdx.x;
     n = min(n, (uint32_t)kf);  // <= THREADS
-    const unsigned long long mine = i < n ? sorted[i] : 0;
-    const uint32_t key = (uint32_t)(mine >> 32), token = 0xFFFFFFFFu - (uint32_t)mine;
-    const unsigned long long w = i < n ? weigh(value_of(key)) : 0;
-    unsigned long long total;
-    const unsigned long long sum = block_scan(w, s, total);
+    const u64 mine = i < n ? sorted[i] : 0;
+    const uint32_t key = (uint32_t)(mine >> 32);
+    const u64 w = i < n ? weigh(value_of(key)) : 0;
+    u64 total;
+    const u64 sum = block_scan(w, s, total);
     if (pf < 1.f) n = __syncthreads_count(i < n && sum - w < mass_target(total));
     n = __syncthreads_count(i < n && (w >= least || key == row.top_key));
     s.list[i] = w;
     if (i + 1 == n) s.above = sum;  // the kept total
     __syncthreads();
     total = s.above;
-    unsigned long long target = (unsigned long long)(u * (double)total);
+    u64 target = (u64)(u * (double)total);
     if (target >= total) target = total - 1;
     if (i < n) {
-      unsigned long long upto = 0;  // the kept mass of the tokens up to this one
+      u64 upto = 0;  // the kept mass of the tokens up to this one
       for (uint32_t j = 0; j < n; ++j)
         if ((uint32_t)sorted[j] >= (uint32_t)mine) upto += s.list[j];
       if (upto > target && upto - w <= target)
-        answer(p, r, (float)token, (float)(log((double)w) - log((double)total)), n);
+        answer(p, r, (float)index_of(mine), (float)(log((double)w) - log((double)total)), n);
     }
     return;
   }
 
-  // ---- the cuts: everything above tau, and `ties` tokens of key tau
-  uint32_t tau = 0;
-  unsigned long long ties = 0, above;
-  if (kf >= 1.f && floorf(kf) < (float)live) {
-    const unsigned long long k = (unsigned long long)kf;
-    tau = find_key<false>(row, LOWEST, row.top_key, k, weigh, s, cluster, above);
-    ties = k - above;
-  }
-  if (pf < 1.f) {
-    unsigned long long gt = 0, total;
-    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
-      const float v = row.v[i];
-      if (key_of(v) > tau) gt += weigh(v);
+  // ---- the cuts
+  Cut cut{0, 0, 0};  // every live token (their places are above 0)
+  if (kf >= 1.f && floorf(kf) < (float)live) cut_at<false, THREADS>(row, [&](u64) { return (u64)kf; }, weigh, s, cluster, cut);
+  if (pf < 1.f) cut_at<true, THREADS>(row, mass_target, weigh, s, cluster, cut);
+  if (least) {  // weights fall with the key: the smallest that is heavy enough
+    uint32_t l = LOWEST, h = row.top_key;
+    while (l < h) {
+      const uint32_t m = l + (h - l) / 2;
+      if (weigh(value_of(m)) >= least) h = m;
+      else l = m + 1;
     }
-    block_scan(gt, s, total);
-    if (threadIdx.x < (unsigned)ctas) cluster.map_shared_rank(&s, threadIdx.x)->cut_mass[rank] = total;
-    cluster.sync();
-    total = ties * (tau ? weigh(value_of(tau)) : 0);
-    for (int c = 0; c < ctas; ++c) total += s.cut_mass[c];
-    const unsigned long long target = mass_target(total);
-    const uint32_t key = find_key<true>(row, tau ? tau : LOWEST, row.top_key, target, weigh, s, cluster, above);
-    const unsigned long long w = weigh(value_of(key));
-    const unsigned long long need = w ? (target - above + w - 1) / w : 1;
-    ties = key == tau && ties < need ? ties : need;
-    tau = key;
+    const u64 light = ((u64)l << 32) - 1;
+    cut.over = cut.over > light ? cut.over : light;
+    if (cut.tau < l) cut.ties = 0;
   }
-  const unsigned long long wt = tau ? weigh(value_of(tau)) : 0;
-  if (tau && tau != row.top_key && wt < least) ties = 0;
+  const u64 wt = cut.ties ? weigh(value_of(cut.tau)) : 0;
+  const Over over(cut.over);
 
   // ---- kept mass and ties of every warp's stretch of the CTA's part
-  const uint32_t stretch = (row.n + WARPS - 1) / WARPS;
+  const uint32_t stretch = ((row.n + WARPS - 1) / WARPS + 3) & ~3u;
   const uint32_t s0 = min(row.n, warp * stretch), s1 = min(row.n, s0 + stretch);
-  auto kept = [&](float v, uint32_t key) {  // the weight of a token above tau, if it stays
-    const unsigned long long w = weigh(v);
-    return w >= least || key == row.top_key ? w : 0;
-  };
+  const uint32_t tie_key = cut.ties ? cut.tau : 0;
   {
-    unsigned long long mass = 0;
+    u64 mass = 0;
     uint32_t tied = 0, count = 0;
-    for (uint32_t i = s0 + lane; i < s1; i += 32) {
-      const float v = row.v[i];
-      const uint32_t key = key_of(v);
-      if (key > tau) {
-        const unsigned long long w = weigh(v);
-        const bool in = w >= least || key == row.top_key;
-        mass += in ? w : 0;
-        count += in;
-      } else if (key && key == tau) {
+    auto add = [&](float v, uint32_t i) {
+      if (over(v, row.first + i)) {
+        mass += weigh(v);
+        ++count;
+      } else if (tie_key && key_of(v) == tie_key) {
         ++tied;
       }
+    };
+    if ((reinterpret_cast<uintptr_t>(row.v) & 15) == 0) {
+#pragma unroll 2
+      for (uint32_t i = s0 + 4 * lane; i < s1; i += 128) {
+        if (i + 4 <= s1) {
+          const float4 x = *reinterpret_cast<const float4 *>(row.v + i);
+          add(x.x, i);
+          add(x.y, i + 1);
+          add(x.z, i + 2);
+          add(x.w, i + 3);
+        } else {
+          for (uint32_t j = i; j < s1; ++j) add(row.v[j], j);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (uint32_t i = s0 + lane; i < s1; i += 32) add(row.v[i], i);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -560,86 +777,93 @@ __global__ void __launch_bounds__(THREADS, 3) mgb_sample_kernel(const SampleArgs
     if (lane == 0) s.warp_mass[warp] = mass, s.warp_ties[warp] = tied, s.warp_count[warp] = count;
     __syncthreads();
     if (threadIdx.x < (unsigned)ctas) {
-      Shared *o = cluster.map_shared_rank(&s, threadIdx.x);
-      unsigned long long m = 0;
+      Shared<THREADS> *o = cluster.map_shared_rank(&s, threadIdx.x);
+      u64 m = 0;
       uint32_t t = 0, c = 0;
       for (int w = 0; w < WARPS; ++w) m += s.warp_mass[w], t += s.warp_ties[w], c += s.warp_count[w];
       o->mass[rank] = m;
       o->ties[rank] = t;
-      o->count[rank] = c;
+      o->kept[rank] = c;
     }
   }
   cluster.sync();  // (the last one: nothing remote is touched after it)
-  unsigned long long total = 0, before = 0, left = ties;
-  uint32_t count = 0, mine_ties = 0;
+  // the order's running sums: over the CTAs, then over the warps' stretches of the
+  // CTA that holds the token
+  u64 total = 0, left = cut.ties;
+  uint32_t count = 0;
   for (int c = 0; c < ctas; ++c) {
-    if (c == rank) {  // this warp's place in the order
-      unsigned long long l = left;
-      before = total;
-      for (int w = 0; w < WARPS; ++w) {
-        const unsigned long long take = l < s.warp_ties[w] ? l : s.warp_ties[w];
-        if (w == warp) {
-          mine_ties = (uint32_t)take;
-          break;
-        }
-        before += s.warp_mass[w] + take * wt;
-        l -= take;
-      }
-    }
-    const unsigned long long take = left < s.ties[c] ? left : s.ties[c];
+    const u64 take = left < s.ties[c] ? left : s.ties[c];
     total += s.mass[c] + take * wt;
-    count += s.count[c] + (uint32_t)take;
+    count += s.kept[c] + (uint32_t)take;
     left -= take;
   }
-  unsigned long long target = (unsigned long long)(u * (double)total);  // the first sum above it
+  u64 target = (u64)(u * (double)total);  // the first sum above it
   if (target >= total) target = total - 1;
-  if (before > target || target >= before + s.warp_mass[warp] + mine_ties * wt) return;
-  unsigned long long run = before;
-  uint32_t tie_run = 0;
-  for (uint32_t i0 = s0; i0 < s1; i0 += 32) {
-    const uint32_t i = i0 + lane;
-    const float v = i < s1 ? row.v[i] : 0.f;
-    const uint32_t key = i < s1 ? key_of(v) : 0;
-    const bool tie = key && key == tau;
-    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    unsigned long long w = 0;
-    if (tie) w = tie_run + __popc(tie_mask & ((1u << lane) - 1)) < mine_ties ? wt : 0;
-    else if (key > tau) w = kept(v, key);
-    tie_run += __popc(tie_mask);
-    unsigned long long sum = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, w && run + sum > target);
-    if (hit) {
-      if (lane == __ffs(hit) - 1)
-        answer(p, r, (float)(row.first + i), (float)(log((double)w) - log((double)total)), count);
+  u64 run = 0;
+  left = cut.ties;
+  int owner = 0;
+  for (;; ++owner) {
+    const u64 take = left < s.ties[owner] ? left : s.ties[owner], m = s.mass[owner] + take * wt;
+    if (target < run + m) break;
+    run += m;
+    left -= take;
+  }
+  if (rank != owner) return;
+  int w = 0;
+  u64 quota = 0;  // ties that stay in the stretch
+  for (;; ++w) {
+    quota = left < s.warp_ties[w] ? left : s.warp_ties[w];
+    const u64 m = s.warp_mass[w] + quota * wt;
+    if (target < run + m) break;
+    run += m;
+    left -= quota;
+  }
+  // a few neighbouring tokens of the stretch a thread
+  const uint32_t b0 = min(row.n, w * stretch), b1 = min(row.n, b0 + stretch);
+  const uint32_t each = (b1 - b0 + THREADS - 1) / THREADS;
+  const uint32_t t0 = min(b1, b0 + threadIdx.x * each), t1 = min(b1, t0 + each);
+  u64 mass = 0, tied = 0, unused;
+#pragma unroll 4
+  for (uint32_t i = t0; i < t1; ++i) {
+    const float v = row.v[i];
+    if (over(v, row.first + i)) mass += weigh(v);
+    else if (tie_key && key_of(v) == tie_key) ++tied;
+  }
+  u64 ties_before = tie_key ? block_scan(tied, s, unused) - tied : 0;
+  const u64 mine = ties_before >= quota ? 0 : tied < quota - ties_before ? tied : quota - ties_before;
+  mass += mine * wt;
+  u64 sum = run + block_scan(mass, s, unused) - mass;
+  if (target < sum || target >= sum + mass) return;
+  for (uint32_t i = t0; i < t1; ++i) {
+    const float v = row.v[i];
+    u64 weight = 0;
+    if (over(v, row.first + i)) weight = weigh(v);
+    else if (tie_key && key_of(v) == tie_key && ties_before++ < quota) weight = wt;
+    sum += weight;
+    if (sum > target) {
+      answer(p, r, (float)(row.first + i), (float)(log((double)weight) - log((double)total)), count);
       return;
     }
-    run += __shfl_sync(0xffffffffu, sum, 31);
   }
 }
 
 uint64_t sample_scratch_bytes(uint64_t, uint64_t) { return 0; }
 
-cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const int sms = device_sms(dev);
-  // CTAs of a row: parts of up to 16,384 tokens (64 KB: three CTAs an SM), and,
-  // with few rows, as many as leave each 2,048
-  uint32_t ctas = 1;
-  while (ctas < MOST_CTAS && (ceil_div(a.vocab, ctas) > 16384 ||
-                              (a.rows * ctas * 2 <= (uint64_t)sms && ceil_div(a.vocab, 2 * ctas) >= 2048)))
-    ctas *= 2;
-  const uint32_t chunk = (uint32_t)(ceil_div(ceil_div(a.vocab, ctas), 4) * 4);
-  const bool staged = chunk <= 48 * 1024;
+template <int THREADS, bool STAGED>
+static cudaError_t launch_sample_kernel(const SampleArgs &a, uint32_t ctas, uint32_t chunk, int dev,
+                                        cudaStream_t stream) {
+  auto *kern = mgb_sample_kernel<THREADS, STAGED>;
+  if (STAGED) {  // the opt-in is an attribute of the function on a device: once each
+    static std::atomic<uint64_t> opted{0};
+    if (!(opted.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024);
+      if (e != cudaSuccess) return e;
+      opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = staged ? chunk * 4 : 0;
+  cfg.dynamicSmemBytes = STAGED ? chunk * 4 : 0;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -649,15 +873,6 @@ cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  auto *kern = staged ? mgb_sample_kernel<true> : mgb_sample_kernel<false>;
-  if (staged) {  // the opt-in is an attribute of the function on a device: once each
-    static std::atomic<uint64_t> opted{0};
-    if (!(opted.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 196608);
-      if (e != cudaSuccess) return e;
-      opted.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
-    }
-  }
   // a grid holds 2^31 - 1 CTAs
   const uint64_t most = 0x7FFFFFFFull / ctas;
   for (uint64_t r = 0; r < a.rows; r += most) {
@@ -670,10 +885,29 @@ cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
     if (part.logprob) part.logprob += r;
     if (part.kept) part.kept += r;
     cfg.gridDim = dim3((unsigned)(part.rows * ctas));
-    e = cudaLaunchKernelEx(&cfg, kern, part, chunk);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, part, chunk);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
+}
+
+cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t sms = (uint64_t)device_sms(dev);
+  // Rows that fill the SMs by themselves: a CTA of 512 threads each, two an SM.
+  if (a.rows > sms / 2 && a.vocab >= 4096)
+    return launch_sample_kernel<512, false>(a, 1, (uint32_t)a.vocab, dev, stream);
+  // Fewer: a cluster each, parts of up to 16,384 tokens (64 KB), and as many CTAs
+  // as leave each 2,048.
+  uint32_t ctas = 1;
+  while (ctas < MOST_CTAS && (ceil_div(a.vocab, ctas) > 16384 ||
+                              (a.rows * ctas * 2 <= sms && ceil_div(a.vocab, 2 * ctas) >= 2048)))
+    ctas *= 2;
+  const uint32_t chunk = (uint32_t)(ceil_div(ceil_div(a.vocab, ctas), 4) * 4);
+  if (chunk <= 48 * 1024) return launch_sample_kernel<256, true>(a, ctas, chunk, dev, stream);
+  return launch_sample_kernel<256, false>(a, ctas, chunk, dev, stream);
 }
 
 }  // namespace mgb
