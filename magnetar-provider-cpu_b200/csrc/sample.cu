@@ -25,6 +25,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <cfloat>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -35,35 +36,16 @@ namespace cg = cooperative_groups;
 
 constexpr int ONE_BITS = 43;  // weight 1
 
-// 2^(j / 64): the nearest multiple of 2^-23 (in those units) and the rest.
-struct Pow2Table {
-  uint32_t hi[64];
-  float lo[64];
-};
-__constant__ Pow2Table g_pow2 = {
-    {
-     8388608u, 8479954u, 8572295u, 8665641u, 8760003u, 8855394u, 8951823u, 9049301u,
-     9147842u, 9247455u, 9348154u, 9449948u, 9552851u, 9656875u, 9762032u, 9868333u,
-     9975792u, 10084422u, 10194234u, 10305242u, 10417458u, 10530897u, 10645571u, 10761494u,
-     10878679u, 10997140u, 11116891u, 11237946u, 11360319u, 11484025u, 11609078u, 11735492u,
-     11863283u, 11992466u, 12123055u, 12255067u, 12388516u, 12523418u, 12659789u, 12797645u,
-     12937002u, 13077877u, 13220286u, 13364245u, 13509772u, 13656884u, 13805598u, 13955931u,
-     14107901u, 14261526u, 14416824u, 14573813u, 14732511u, 14892937u, 15055111u, 15219050u,
-     15384775u, 15552304u, 15721658u, 15892855u, 16065917u, 16240863u, 16417715u, 16596492u},
-    {
-     0.00000000e+00f, -5.71160541e-09f, -4.81155986e-08f, -2.80908932e-08f, 4.83347016e-08f,
-     -4.90716943e-08f, -5.93375198e-08f, 5.46159455e-08f, -1.30775399e-08f, 4.26050200e-08f,
-     -5.43554002e-08f, 3.12364143e-08f, 5.38622231e-08f, 2.19222827e-08f, -4.05144149e-08f,
-     2.56697508e-08f, 3.79763527e-08f, -5.06975653e-08f, -3.26739489e-08f, -4.13620036e-08f,
-     4.49683810e-08f, 7.32223748e-09f, 1.41933332e-09f, -3.81662169e-08f, -4.01899953e-08f,
-     -3.49657157e-08f, -3.49637332e-08f, -3.46167397e-08f, -1.01233493e-08f, -3.84588184e-08f,
-     -5.87557736e-08f, 8.68943406e-09f, 2.42032350e-08f, -1.34299292e-08f, 3.32419994e-08f,
-     -3.62865755e-08f, -4.50089885e-08f, -3.42362014e-08f, -2.49593732e-08f, -1.76285688e-08f,
-     8.07090483e-09f, -2.57646651e-08f, -5.66102543e-08f, -4.90313679e-10f, 9.83621717e-09f,
-     -1.72600831e-08f, -5.12497209e-08f, -3.92029875e-08f, -2.47553267e-08f, -2.86514723e-08f,
-     -4.84961760e-08f, -5.85022342e-08f, -9.23577037e-09f, 5.34319788e-08f, -1.14150449e-08f,
-     3.73625824e-08f, -1.12392780e-08f, 1.43656118e-08f, -4.66300563e-08f, 2.81033845e-08f,
-     9.84532811e-09f, 5.35707230e-08f, -1.70218044e-08f, 6.03272632e-09f}};
+// 2^(j / 64) in units of 2^-31.
+__constant__ uint32_t g_pow2[64] = {
+    2147483648u, 2170868212u, 2194507417u, 2218404036u, 2242560872u, 2266980759u, 2291666561u, 2316621173u,
+    2341847524u, 2367348571u, 2393127307u, 2419186755u, 2445529972u, 2472160047u, 2499080105u, 2526293303u,
+    2553802834u, 2581611923u, 2609723834u, 2638141863u, 2666869345u, 2695909648u, 2725266179u, 2754942382u,
+    2784941738u, 2815267765u, 2845924021u, 2876914102u, 2908241642u, 2939910317u, 2971923842u, 3004285971u,
+    3037000500u, 3070071267u, 3103502151u, 3137297074u, 3171459999u, 3205994934u, 3240905930u, 3276197082u,
+    3311872529u, 3347936457u, 3384393094u, 3421246719u, 3458501653u, 3496162267u, 3534232978u, 3572718252u,
+    3611622603u, 3650950594u, 3690706840u, 3730896002u, 3771522796u, 3812591987u, 3854108391u, 3896076880u,
+    3938502376u, 3981389855u, 4024744348u, 4068570940u, 4112874773u, 4157661043u, 4202935003u, 4248701965u};
 
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);  // -0 -> +0
@@ -77,9 +59,11 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // The weight function of a row.
 struct Weigh {
   float top, chi, clo;  // the largest logit; log2(e) / T as the sum of two floats
-  const float2 *pow2;   // g_pow2 in shared memory (lanes look different entries up,
-                        // which constant memory serves one after the other: 256 rows
-                        // of 128,256 without cuts took 562 us, then 261)
+  const uint32_t *pow2;  // g_pow2 in shared memory: lanes look different entries up,
+                         // which constant memory serves one after the other, and two
+                         // words in each bank keep few of them waiting for one another
+  // the distance to the largest logit in octaves: monotonic
+  __device__ __forceinline__ float octaves(float v) const { return (top - v) * chi; }
   __device__ __forceinline__ uint64_t operator()(float v) const {
     if (__isinff(top)) return v == top ? 1ull << ONE_BITS : 0;  // +inf
     // v - top = d + e exactly; times (chi + clo): p + r
@@ -99,11 +83,10 @@ struct Weigh {
     q = fmaf(s, q, 0.240226506959101f);
     q = fmaf(s, q, 0.693147180559945f);
     q *= s;
-    const int ni = __float_as_int(big) - 0x4B400000, j = ni & 63, N = ni >> 6;
-    const float2 power = pow2[j];
-    // the last two factors in units of 2^-31 (below 2)
-    const uint32_t lead = (__float_as_uint(power.x) << 8) | 0x80000000u;
-    const uint32_t one = lead + (uint32_t)__float2int_rn(fmaf(power.x, q, power.y) * 2147483648.f);
+    const int ni = __float_as_int(big) - 0x4B400000, N = ni >> 6;
+    const uint32_t lead = pow2[ni & 63];
+    // the last two factors in units of 2^-31 (below 2): lead (1 + q), q in 2^-38
+    const uint32_t one = lead + ((__mulhi((int)(lead >> 1), __float2int_rn(q * 0x1p38f)) + 16) >> 5);
     const int down = 31 - ONE_BITS - N;
     if (down > 0) return ((one >> (down - 1)) + 1) >> 1;  // (down <= 32)
     return (uint64_t)one << -down;
@@ -114,10 +97,11 @@ constexpr int BINS = 1024;
 constexpr int MOST_CTAS = 8;      // of a cluster
 constexpr int LIST = 1024;        // tokens the first CTA sorts at most
 constexpr uint32_t LOWEST = 0x00800000u;  // the key of the lowest finite value
-// A token's distance to the largest logit as a number of 20 bits, monotonic: 1,024
-// bins of 1/16, of 1,024 parts each.
+// A token's distance to the largest logit (in octaves of the weight where masses
+// are summed) as a number of 20 bits, monotonic: 1,024 bins of 1/16, of 1,024 parts.
 constexpr float CODE_SCALE = 16384.f;
 constexpr int CODE_MOST = (1 << 20) - 1;
+constexpr uint32_t MOST_TOKENS = 1 << 17;  // of a CTA
 
 typedef unsigned long long u64;  // what atomicAdd and shuffles take
 
@@ -127,8 +111,9 @@ __device__ __forceinline__ u64 place_of(uint32_t key, uint32_t index) {
 }
 __device__ __forceinline__ uint32_t index_of(u64 place) { return 0xFFFFFFFFu - (uint32_t)place; }
 
-__device__ __forceinline__ int code_of(float top, float v) {
-  const int c = (int)((top - v) * CODE_SCALE);  // (saturates)
+template <bool MASS>
+__device__ __forceinline__ int code_of(const Weigh &weigh, float v) {
+  const int c = (int)((MASS ? weigh.octaves(v) : weigh.top - v) * CODE_SCALE);  // (saturates)
   return c < CODE_MOST ? c : CODE_MOST;
 }
 
@@ -142,14 +127,15 @@ struct Shared {
   // what the CTAs tell each other, by rank
   u64 top[MOST_CTAS];                   // the place of the largest logit
   u64 mass[MOST_CTAS];
+  float bound[MOST_CTAS];
   uint32_t live[MOST_CTAS], found[MOST_CTAS], count[MOST_CTAS], ties[MOST_CTAS], kept[MOST_CTAS];
   // the first CTA's answers
   u64 found_above, cut, target;
   uint32_t lo, hi;
-  int border;
+  int border, many;
   // of the CTA
   u64 above, warp_mass[WARPS];
-  uint32_t warp_ties[WARPS], warp_count[WARPS], own[THREADS], taken, bin;
+  uint32_t warp_ties[WARPS], warp_count[WARPS], taken, bin;
 };
 
 template <int THREADS>
@@ -208,9 +194,20 @@ __device__ __forceinline__ void find_entry(const u64 *e, u64 target, Shared<THRE
   __syncthreads();
 }
 
-// n places (n <= LIST) into descending order, in place.
+// n different places (n <= LIST) into descending order, in place.
 template <int THREADS>
 __device__ __forceinline__ void sort_places(u64 *e, uint32_t n) {
+  if (n <= 256 && n <= THREADS) {  // each counts those before it (a barrier a step costs more)
+    const u64 mine = threadIdx.x < n ? e[threadIdx.x] : 0;
+    uint32_t at = 0;
+    if (threadIdx.x < n)
+#pragma unroll 4
+      for (uint32_t i = 0; i < n; ++i) at += e[i] > mine;
+    __syncthreads();
+    if (threadIdx.x < n) e[at] = mine;
+    __syncthreads();
+    return;
+  }
   uint32_t size = 2;
   while (size < n) size <<= 1;
   for (uint32_t i = n + threadIdx.x; i < size; i += THREADS) e[i] = 0;
@@ -246,67 +243,96 @@ struct Row {
   uint32_t top_key;
 };
 
-// Calls f(logit, position) for every token of the CTA's part, 16 bytes at a time
-// where it can.
-template <int THREADS, typename F>
-__device__ __forceinline__ void for_each(const float *v, uint32_t n, const F &f) {
+// Calls f(logit, position) for the tokens [from, to) of the CTA's part (from a
+// multiple of 4), spread over THREADS threads, 16 bytes at a time where it can, and copies them; a thread's
+// positions rise.  (AHEAD loads are issued before the first f, whose atomics and
+// stores no load is moved over: the candidates of 256 rows of 128,256 took 34 us of
+// a row's time without that.)
+template <int THREADS, int AHEAD = 4, bool COPY = false, typename F>
+__device__ __forceinline__ void for_each(const float *v, uint32_t from, uint32_t to, const F &f,
+                                         float *copy = nullptr, uint32_t thread = threadIdx.x) {
+  uint32_t i = from;
   if ((reinterpret_cast<uintptr_t>(v) & 15) == 0) {
-    const uint32_t n4 = n / 4;
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < n4; i += THREADS) {
-      const float4 x = reinterpret_cast<const float4 *>(v)[i];
-      f(x.x, 4 * i);
-      f(x.y, 4 * i + 1);
-      f(x.z, 4 * i + 2);
-      f(x.w, 4 * i + 3);
+    const float4 *v4 = reinterpret_cast<const float4 *>(v);
+    const uint32_t n4 = to / 4;
+    auto four = [&](const float4 &x, uint32_t at) {
+      if (COPY) reinterpret_cast<float4 *>(copy)[at] = x;
+      f(x.x, 4 * at);
+      f(x.y, 4 * at + 1);
+      f(x.z, 4 * at + 2);
+      f(x.w, 4 * at + 3);
+    };
+    uint32_t j = from / 4 + thread;
+    for (; j + (AHEAD - 1) * THREADS < n4; j += AHEAD * THREADS) {
+      float4 x[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) x[a] = v4[j + a * THREADS];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) four(x[a], j + a * THREADS);
     }
-    for (uint32_t i = 4 * n4 + threadIdx.x; i < n; i += THREADS) f(v[i], i);
-  } else {
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) f(v[i], i);
+    for (; j < n4; j += THREADS) four(v4[j], j);
+    i = max(from, 4 * n4);
   }
+  i += thread;
+  auto one = [&](float x, uint32_t at) {
+    if (COPY) copy[at] = x;
+    f(x, at);
+  };
+  for (; i + 3 * THREADS < to; i += 4 * THREADS) {
+    float x[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) x[a] = v[i + a * THREADS];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) one(x[a], i + a * THREADS);
+  }
+  for (; i < to; i += THREADS) one(v[i], i);
 }
 
-// A mass (below 2^44) in three digits of a histogram: with n tokens of a CTA, log2 n
-// below L, digits of 32 - L bits keep their sums below 2^32.  The third has 44 - 2
-// (32 - L) bits left, too many where L is above 17: it then goes into 64 bits.
-struct Digits {
-  int bits;
-  bool wide;
-  __device__ __forceinline__ explicit Digits(uint32_t n) {
-    int L = 0;
-    while ((1u << L) < n) ++L;  // n <= 2^20
-    bits = L < 15 ? 17 : 32 - L;
-    wide = L > 17;
+// A value that at least k of the threads' keys reach and few more (the lowest
+// finite value where fewer than k are live).
+template <int THREADS>
+__device__ __forceinline__ float kth_largest(uint32_t own, uint32_t k) {
+  uint32_t lo = LOWEST, hi = 0xFF800000u;  // (+inf)
+  while (lo < hi) {
+    const uint32_t m = lo + (hi - lo + 1) / 2;
+    const uint32_t n = __syncthreads_count(own >= m);
+    if (n >= k) lo = m;
+    else hi = m - 1;
+    if (n >= k && n <= k + k / 8) break;
   }
-};
+  return value_of(lo);
+}
 
 // The tokens' counts (MASS: masses) by bin, summed over the cluster in the first
-// CTA's part[0..1], as u64.  bin(v, position): a token's bin, or -1.
-template <bool MASS, int THREADS, typename B>
-__device__ __forceinline__ u64 *histogram(const Row &row, const B &bin, const Weigh &weigh, Shared<THREADS> &s,
-                                          cg::cluster_group &cluster) {
+// CTA's part[0..1], as u64.  bin(v, position): a token's bin, or -1.  A mass is
+// added in digits, whose sums over a CTA's tokens stay below 2^32: 15 bits, three of
+// them, for MOST_TOKENS; with NARROW and about half of those, two of 16 bits.
+// NARROW: bin b's weights are multiples of 2^low(b) and at most 2^32 of that (a
+// thousandth more where they round up).
+template <bool MASS, bool NARROW, int THREADS, typename B, typename L>
+__device__ __forceinline__ u64 *histogram(const Row &row, const B &bin, const L &low, const Weigh &weigh,
+                                          Shared<THREADS> &s, cg::cluster_group &cluster) {
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const Digits digits(row.n);
-  const int D = digits.bits;
+  const bool two = NARROW && row.n <= 65000;
+  const int D = two ? 16 : 15;
   const uint32_t mask = (1u << D) - 1;
   for (int i = threadIdx.x; i < BINS; i += THREADS)
 #pragma unroll
     for (int d = 0; d < (MASS ? 3 : 1); ++d) s.part[d][i] = 0;
-  if (MASS)
-    for (int i = threadIdx.x; i < LIST; i += THREADS) s.list[i] = 0;
   __syncthreads();
-  for_each<THREADS>(row.v, row.n, [&](float v, uint32_t i) {
+  for_each<THREADS>(row.v, 0, row.n, [&](float v, uint32_t i) {
     const int b = bin(v, i);
     if (b < 0) return;
     if (MASS) {
-      const uint64_t w = weigh(v);
-      const uint32_t d0 = (uint32_t)w & mask, d1 = (uint32_t)(w >> D) & mask, d2 = (uint32_t)(w >> (2 * D));
-      if (d0) atomicAdd(&s.part[0][b], d0);
-      if (d1) atomicAdd(&s.part[1][b], d1);
-      if (d2) {
-        if (digits.wide) atomicAdd(&s.list[b], (u64)d2 << (2 * D));
-        else atomicAdd(&s.part[2][b], d2);
+      const uint64_t w = weigh(v) >> low(b);
+      if (!w) return;
+      atomicAdd(&s.part[0][b], (uint32_t)w & mask);
+      if (two) {
+        atomicAdd(&s.part[1][b], (uint32_t)(w >> 16));
+      } else {
+        const uint32_t d1 = (uint32_t)(w >> 15) & mask, d2 = (uint32_t)(w >> 30);
+        atomicAdd(&s.part[1][b], d1);
+        if (d2) atomicAdd(&s.part[2][b], d2);
       }
     } else {
       atomicAdd(&s.part[0][b], 1u);
@@ -314,7 +340,7 @@ __device__ __forceinline__ u64 *histogram(const Row &row, const B &bin, const We
   });
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS)
-    s.list[i] = MASS ? s.list[i] + s.part[0][i] + ((u64)s.part[1][i] << D) + ((u64)s.part[2][i] << (2 * D))
+    s.list[i] = MASS ? (s.part[0][i] + ((u64)s.part[1][i] << D) + ((u64)s.part[2][i] << 30)) << low(i)
                      : s.part[0][i];
   cluster.sync();
   u64 *all = reinterpret_cast<u64 *>(s.part[0]);  // [BINS]: two of the three
@@ -347,13 +373,13 @@ __device__ __noinline__ uint32_t find_key(const Row &row, uint32_t lo, uint32_t 
   while (lo < hi) {
     int shift = 0;
     while (((hi - lo) >> shift) >= BINS) ++shift;
-    const u64 *all = histogram<MASS, THREADS>(
+    const u64 *all = histogram<MASS, false, THREADS>(
         row,
         [&](float v, uint32_t i) {
           const uint32_t key = key_of(v);
           return key >= lo && key <= hi && place_of(key, row.first + i) > over ? (int)((hi - key) >> shift) : -1;
         },
-        weigh, s, cluster);
+        [](int) { return 0; }, weigh, s, cluster);
     if (rank == 0) {
       int bin;
       u64 before;
@@ -383,25 +409,22 @@ struct Cut {
   u64 ties;
 };
 
-// The tokens of the bin `border` that are over the cut, to the first CTA's list;
-// s.count of every CTA tells how many there are.  The caller's cluster barrier
-// follows.
+// The first CTA: what its cluster's list holds from `bound` on, best first, in
+// part[0..1]; returns its number.
 template <int THREADS>
-__device__ __forceinline__ void list_token(const Row &row, uint32_t i, float v, u64 *list, uint32_t room,
-                                           Shared<THREADS> &s) {
-  const uint32_t at = atomicAdd(&s.taken, 1u);
-  if (at < room) list[at] = place_of(key_of(v), row.first + i);
-}
-
-// The first CTA: its cluster's list, best first, in part[0..1]; returns their number.
-template <int THREADS>
-__device__ __forceinline__ uint32_t sort_list(int ctas, uint32_t room, Shared<THREADS> &s) {
+__device__ __forceinline__ uint32_t sort_list(int ctas, uint32_t room, const uint32_t *count, float bound,
+                                              Shared<THREADS> &s) {
   u64 *sorted = reinterpret_cast<u64 *>(s.part[0]);
-  uint32_t n = 0;
-  for (int c = 0; c < ctas; ++c) {
-    for (uint32_t i = threadIdx.x; i < s.count[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
-    n += s.count[c];
-  }
+  __syncthreads();
+  if (threadIdx.x == 0) s.taken = 0;
+  __syncthreads();
+  for (int c = 0; c < ctas; ++c)
+    for (uint32_t i = threadIdx.x; i < count[c]; i += THREADS) {
+      const u64 place = s.list[c * room + i];
+      if (value_of((uint32_t)(place >> 32)) >= bound) sorted[atomicAdd(&s.taken, 1u)] = place;
+    }
+  __syncthreads();
+  const uint32_t n = s.taken;
   sort_places<THREADS>(sorted, n);
   return n;
 }
@@ -451,6 +474,8 @@ __device__ void cut_at(const Row &row, const F &target_of, const Weigh &weigh, S
       if (threadIdx.x < (unsigned)ctas) {
         Shared<THREADS> *o = cluster.map_shared_rank(&s, threadIdx.x);
         o->border = bin;
+        // more tokens than can be listed (of masses: even if each had its bin's most)
+        o->many = (MASS ? exp2f(bin * 0.0625f - (float)ONE_BITS) : 1.f) * (float)all[bin] > (float)LIST;
         o->found_above = above + before;
         o->target = target;
       }
@@ -459,19 +484,34 @@ __device__ void cut_at(const Row &row, const F &target_of, const Weigh &weigh, S
     cluster.sync();
   };
   if (cut.ties == 0 && !__isinff(row.top)) {
-    tell(histogram<MASS, THREADS>(
-             row, [&](float v, uint32_t i) { return over(v, row.first + i) ? code_of(row.top, v) >> 10 : -1; },
-             weigh, s, cluster),
+    // a bin's weights lie within 1/16 octave, and have 32 bits
+    tell(histogram<MASS, true, THREADS>(
+             row,
+             [&](float v, uint32_t i) { return over(v, row.first + i) ? code_of<MASS>(weigh, v) >> 10 : -1; },
+             [](int b) { return b < 11 * 16 ? 11 - (b >> 4) : 0; }, weigh, s, cluster),
          true);
-    int border = s.border, part = -1;
-    for (int level = 0; level < 2; ++level) {
+    const int border = s.border;
+    int part = -1;
+    for (int level = s.many; level < 2; ++level) {
+      if (level == 1) {
+        tell(histogram<MASS, true, THREADS>(
+                 row,
+                 [&](float v, uint32_t i) {
+                   if (!over(v, row.first + i)) return -1;
+                   const int c = code_of<MASS>(weigh, v);
+                   return c >> 10 == border ? c & 1023 : -1;
+                 },
+                 [=](int) { return border < 11 * 16 ? 11 - (border >> 4) : 0; }, weigh, s, cluster),
+             false);
+        part = (border << 10) | s.border;
+      }
       auto inside = [&](float v, uint32_t i) {
         if (!over(v, row.first + i)) return false;
-        const int c = code_of(row.top, v);
+        const int c = code_of<MASS>(weigh, v);
         return part < 0 ? c >> 10 == border : c == part;
       };
       u64 *list = cluster.map_shared_rank(s.list, 0) + rank * room;
-      for_each<THREADS>(row.v, row.n, [&](float v, uint32_t i) {
+      for_each<THREADS>(row.v, 0, row.n, [&](float v, uint32_t i) {
         if (!inside(v, i)) return;
         const uint32_t at = atomicAdd(&s.taken, 1u);
         if (at < room) list[at] = place_of(key_of(v), row.first + i);
@@ -483,13 +523,8 @@ __device__ void cut_at(const Row &row, const F &target_of, const Weigh &weigh, S
       for (int c = 0; c < ctas; ++c) listed = listed && s.count[c] <= room;
       if (listed) {
         if (rank == 0) {
-          u64 *sorted = reinterpret_cast<u64 *>(s.part[0]);
-          uint32_t n = 0;
-          for (int c = 0; c < ctas; ++c) {
-            for (uint32_t i = threadIdx.x; i < s.count[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
-            n += s.count[c];
-          }
-          sort_places<THREADS>(sorted, n);
+          const u64 *sorted = reinterpret_cast<const u64 *>(s.part[0]);
+          const uint32_t n = sort_list<THREADS>(ctas, room, s.count, -FLT_MAX, s);
           for (uint32_t i = threadIdx.x; i < LIST; i += THREADS)
             s.list[i] = i >= n ? 0 : MASS ? weigh(value_of((uint32_t)(sorted[i] >> 32))) : 1;
           __syncthreads();
@@ -503,34 +538,14 @@ __device__ void cut_at(const Row &row, const F &target_of, const Weigh &weigh, S
         __syncthreads();
         return;
       }
-      if (level) break;
-      tell(histogram<MASS, THREADS>(
-               row,
-               [&](float v, uint32_t i) {
-                 if (!over(v, row.first + i)) return -1;
-                 const int c = code_of(row.top, v);
-                 return c >> 10 == border ? c & 1023 : -1;
-               },
-               weigh, s, cluster),
-           false);
-      part = (border << 10) | s.border;
     }
   } else {
-    tell(histogram<MASS, THREADS>(
-             row, [&](float v, uint32_t i) { return over(v, row.first + i) ? 0 : -1; }, weigh, s, cluster),
+    tell(histogram<MASS, false, THREADS>(
+             row, [&](float v, uint32_t i) { return over(v, row.first + i) ? 0 : -1; }, [](int) { return 0; },
+             weigh, s, cluster),
          true);
   }
-  // too many tokens in one place: by keys
-  const u64 target = s.target;
-  u64 above;
-  const uint32_t key = find_key<MASS, THREADS>(row, cut.ties ? cut.tau : LOWEST, row.top_key,
-                                               cut.ties ? 0 : cut.over, target, weigh, s, cluster, above);
-  const u64 w = MASS ? weigh(value_of(key)) : 1;
-  u64 need = w ? (target - above + w - 1) / w : 1;
-  if (cut.ties && key == cut.tau && cut.ties < need) need = cut.ties;
-  cut.tau = key;
-  cut.ties = need;
-  cut.over = place_of(key, 0);  // every place of a larger key
+  cut_by_key<MASS, THREADS>(row, s.target, weigh, s, cluster, cut);  // too many tokens in one place
 }
 
 __device__ __forceinline__ void answer(const SampleArgs &p, uint64_t r, float id, float logprob,
@@ -547,9 +562,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
     mgb_sample_kernel(const SampleArgs p, uint32_t chunk) {
   constexpr int WARPS = THREADS / 32;
   __shared__ Shared<THREADS> s;
-  __shared__ float2 pow2[64];
+  __shared__ uint32_t pow2[64];
   extern __shared__ __align__(16) float data[];
-  if (threadIdx.x < 64) pow2[threadIdx.x] = make_float2((float)g_pow2.hi[threadIdx.x] * 1.1920929e-7f, g_pow2.lo[threadIdx.x]);
+  if (threadIdx.x < 64) pow2[threadIdx.x] = g_pow2[threadIdx.x];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -574,29 +589,32 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
     live += key != 0;
     if (key > own) own = key, own_at = i;  // (positions rise: the first of equals stays)
   };
-  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-    const uint32_t n4 = row.n / 4;
-#pragma unroll 8
-    for (uint32_t i = threadIdx.x; i < n4; i += THREADS) {
-      const float4 v = reinterpret_cast<const float4 *>(src)[i];
-      if (STAGED) reinterpret_cast<float4 *>(data)[i] = v;
-      see(v.x, 4 * i);
-      see(v.y, 4 * i + 1);
-      see(v.z, 4 * i + 2);
-      see(v.w, 4 * i + 3);
-    }
-    for (uint32_t i = 4 * n4 + threadIdx.x; i < row.n; i += THREADS) {
-      const float v = src[i];
-      if (STAGED) data[i] = v;
-      see(v, i);
-    }
-  } else {
-#pragma unroll 8
-    for (uint32_t i = threadIdx.x; i < row.n; i += THREADS) {
-      const float v = src[i];
-      if (STAGED) data[i] = v;
-      see(v, i);
-    }
+  // small top_k: this CTA's candidates, to the first CTA's list
+  static_assert(LIST <= BINS && BINS * 8 <= sizeof(s.part), "the sort's buffer");
+  const uint32_t room = LIST / ctas;
+  const bool few = !greedy && kf >= 1.f && kf < 257.f && kf < (float)room + 1.f;
+  u64 *list = cluster.map_shared_rank(s.list, 0) + rank * room;
+  float bound;
+  auto take = [&](float v, uint32_t i) {
+    if (!(v >= bound)) return;
+    const uint32_t at = atomicAdd(&s.taken, 1u);
+    if (at < room) list[at] = place_of(key_of(v), row.first + i);
+  };
+  // From the threads' largest of a first part comes a bound for the rest, whose
+  // candidates are so listed as they are read.
+  const uint32_t head = few && row.n >= 32 * THREADS ? row.n / 4 & ~3u : row.n;
+  if (threadIdx.x == 0) s.taken = 0;
+  for_each<THREADS, 8, STAGED>(src, 0, head, see, data);
+  cluster.barrier_wait();
+  if (head < row.n) {
+    bound = kth_largest<THREADS>(own, (uint32_t)kf);
+    for_each<THREADS, 8, STAGED>(
+        src, head, row.n,
+        [&](float v, uint32_t i) {
+          see(v, i);
+          take(v, i);
+        },
+        data);
   }
   row.v = STAGED ? data : src;
   u64 best = block_max(own ? place_of(own, row.first + own_at) : 0ull, s);
@@ -605,39 +623,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
     block_scan(live, s, total);
     live = (uint32_t)total;
   }
-  cluster.barrier_wait();
-
-  // small top_k: this CTA's candidates, to the first CTA's list
-  static_assert(LIST <= BINS && BINS * 8 <= sizeof(s.part), "the sort's buffer");
-  const uint32_t room = LIST / ctas;
-  const bool few = !greedy && kf >= 1.f && kf < 257.f && kf < (float)room + 1.f;
   uint32_t found = 0xFFFFFFFFu;  // none sent
   if (few) {
-    const uint32_t k = (uint32_t)kf;
-    uint32_t bound = 1;  // every live token
-    if (threadIdx.x == 0) s.taken = 0;
-    if (live > room) {
-      s.own[threadIdx.x] = own;
-      __syncthreads();
-      // the k-th largest of the threads' largest keys (k <= THREADS): the one with
-      // fewer than k above it and k at least as large
-      uint32_t over = 0, level = 0;
-#pragma unroll 8
-      for (int j = 0; j < THREADS; ++j) over += s.own[j] > own, level += s.own[j] == own;
-      if (over < k && over + level >= k) s.bin = own;  // (equal keys agree)
-      __syncthreads();
-      bound = max(s.bin, 1u);
-    } else {
-      __syncthreads();
-    }
-    u64 *list = cluster.map_shared_rank(s.list, 0) + rank * room;
-    for_each<THREADS>(row.v, row.n, [&](float v, uint32_t i) {
-      const uint32_t key = key_of(v);
-      if (key >= bound) {
-        const uint32_t at = atomicAdd(&s.taken, 1u);
-        if (at < room) list[at] = place_of(key, row.first + i);
-      }
-    });
+    // what is listed is a superset: the first CTA leaves out what is below all bounds
+    bound = live > room ? kth_largest<THREADS>(own, (uint32_t)kf) : -FLT_MAX;
+    const bool kept = s.taken <= room;
+    __syncthreads();
+    if (!kept && threadIdx.x == 0) s.taken = 0;
+    __syncthreads();
+    for_each<THREADS>(row.v, 0, kept ? head : row.n, take);
     __syncthreads();
     found = s.taken;  // (above room: too many tokens reach the bound)
   }
@@ -646,6 +640,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
     o->top[rank] = best;
     o->live[rank] = live;
     o->found[rank] = found;
+    o->bound[rank] = bound;
   }
   cluster.sync();
   bool listed = few;
@@ -685,13 +680,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
   if (listed) {
     // ---- the first CTA sorts the candidates, best first, and does the rest
     if (rank) return;
-    u64 *sorted = reinterpret_cast<u64 *>(s.part[0]);  // [LIST]: two of three
-    uint32_t n = 0;
-    for (int c = 0; c < ctas; ++c) {
-      for (uint32_t i = threadIdx.x; i < s.found[c]; i += THREADS) sorted[n + i] = s.list[c * room + i];
-      n += s.found[c];
-    }
-    sort_places<THREADS>(sorted, n);
+    const u64 *sorted = reinterpret_cast<const u64 *>(s.part[0]);
+    float least_bound = s.bound[0];
+    for (int c = 1; c < ctas; ++c) least_bound = fmaxf(least_bound, s.bound[c]);
+    uint32_t n = sort_list<THREADS>(ctas, room, s.found, least_bound, s);
     const uint32_t i = threadIdx.x;
     n = min(n, (uint32_t)kf);  // <= THREADS
     const u64 mine = i < n ? sorted[i] : 0;
@@ -719,7 +711,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
 
   // ---- the cuts
   Cut cut{0, 0, 0};  // every live token (their places are above 0)
-  if (kf >= 1.f && floorf(kf) < (float)live) cut_at<false, THREADS>(row, [&](u64) { return (u64)kf; }, weigh, s, cluster, cut);
+  if (kf >= 1.f && floorf(kf) < (float)live)
+    cut_at<false, THREADS>(row, [&](u64) { return (u64)kf; }, weigh, s, cluster, cut);
   if (pf < 1.f) cut_at<true, THREADS>(row, mass_target, weigh, s, cluster, cut);
   if (least) {  // weights fall with the key: the smallest that is heavy enough
     uint32_t l = LOWEST, h = row.top_key;
@@ -750,23 +743,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
         ++tied;
       }
     };
-    if ((reinterpret_cast<uintptr_t>(row.v) & 15) == 0) {
-#pragma unroll 2
-      for (uint32_t i = s0 + 4 * lane; i < s1; i += 128) {
-        if (i + 4 <= s1) {
-          const float4 x = *reinterpret_cast<const float4 *>(row.v + i);
-          add(x.x, i);
-          add(x.y, i + 1);
-          add(x.z, i + 2);
-          add(x.w, i + 3);
-        } else {
-          for (uint32_t j = i; j < s1; ++j) add(row.v[j], j);
-        }
-      }
-    } else {
-#pragma unroll 4
-      for (uint32_t i = s0 + lane; i < s1; i += 32) add(row.v[i], i);
-    }
+    for_each<32>(row.v, s0, s1, add, nullptr, lane);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       mass += __shfl_xor_sync(0xffffffffu, mass, o);
@@ -896,9 +873,14 @@ cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const uint64_t sms = (uint64_t)device_sms(dev);
-  // Rows that fill the SMs by themselves: a CTA of 512 threads each, two an SM.
-  if (a.rows > sms / 2 && a.vocab >= 4096)
-    return launch_sample_kernel<512, false>(a, 1, (uint32_t)a.vocab, dev, stream);
+  // Rows that fill the SMs by themselves: CTAs of 512 threads, two an SM.  Two of
+  // them a row, so that rows with little to do leave their SMs to the others.
+  if (a.rows > sms / 2 && a.vocab >= 4096) {
+    uint32_t ctas = 2;
+    while (ceil_div(a.vocab, ctas) > MOST_TOKENS) ctas *= 2;
+    const uint32_t chunk = (uint32_t)(ceil_div(ceil_div(a.vocab, ctas), 4) * 4);
+    return launch_sample_kernel<512, false>(a, ctas, chunk, dev, stream);
+  }
   // Fewer: a cluster each, parts of up to 16,384 tokens (64 KB), and as many CTAs
   // as leave each 2,048.
   uint32_t ctas = 1;
