@@ -256,10 +256,7 @@ static int current_sms() {
 }
 
 // Tokens of one expert in a pass over its rows: m is the most it can have.
-static int pass_tokens(int fmt, uint64_t m) {
-  const int t = m <= 8 ? 8 : m <= 16 ? 16 : 32;
-  return t < moe::max_tokens(fmt) ? t : moe::max_tokens(fmt);
-}
+static int pass_tokens(uint64_t m) { return m <= 8 ? 8 : moe::MOST_TOKENS; }
 
 static cudaError_t moe_product(int fmt, const moe::Args *a, int tokens, int sms, int *ctas_per_sm,
                                cudaStream_t stream) {
@@ -308,7 +305,7 @@ struct MoeScratch {
     for (int i = 0; i < 2; ++i) place[i] = take(slots * 4), share[i] = take(8);
     // the second product's results take the first one's place
     auto rows = [&](int fmt, uint64_t tiles) {
-      const int tokens = pass_tokens(fmt, m);
+      const int tokens = pass_tokens(m);
       int per_sm = 0;
       moe_product(fmt, nullptr, tokens, sms, &per_sm, nullptr);
       return part_rows(slots, tokens, tiles, (uint64_t)sms * per_sm);
@@ -394,7 +391,7 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   a.cols = hidden;
   a.slots = slots;
   a.act_div = (int)top_k;
-  e = moe_product(ex.gate_up_format, &a, pass_tokens(ex.gate_up_format, m), sms, nullptr, stream);
+  e = moe_product(ex.gate_up_format, &a, pass_tokens(m), sms, nullptr, stream);
   if (e != cudaSuccess) return e;
   const Parts gu{a.out, a.place, a.share, 2 * (int)ceil_div(ffn, moe::TILE), (int)ceil_div(hidden, moe::stage_cols(ex.gate_up_format)), 2 * ffn};
   const uint32_t h_smem = (uint32_t)h_runs(ffn) * RUN * 4;
@@ -414,7 +411,7 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   a.rows = hidden;
   a.cols = ffn;
   a.act_div = 1;
-  e = moe_product(ex.down_format, &a, pass_tokens(ex.down_format, m), sms, nullptr, stream);
+  e = moe_product(ex.down_format, &a, pass_tokens(m), sms, nullptr, stream);
   if (e != cudaSuccess) return e;
   const Parts dn{a.out, a.place, a.share, (int)ceil_div(hidden, moe::TILE), 
                  (int)ceil_div(ffn, moe::stage_cols(ex.down_format)), hidden};

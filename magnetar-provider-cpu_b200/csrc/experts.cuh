@@ -185,6 +185,12 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// K-major without a swizzle: cores of 8 rows and 16 bytes, two along K side by side,
+// 8-row groups 256 bytes apart.
+__device__ __forceinline__ uint64_t desc_cores(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(256 >> 4) << 32) |
+         ((uint64_t)1 << 46);
+}
 // D f32, A and B f16, M = 128
 __device__ __forceinline__ uint32_t idesc_f16(int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
@@ -213,7 +219,10 @@ template <int FMT>
 struct Stage {
   static constexpr int RUNS = FMT == Q4_K || FMT == Q4_0 || FMT == IQ4_NL ? 8 : 4;
   static constexpr int QS = (FMT == Q8_0 ? 32 : FMT == Q6_K ? 24 : 16) * RUNS;
-  static constexpr int STRIDE = QS + 16;  // 8 rows of one run fall into different banks
+  // 8 rows of one run fall into different banks: by a gap, or 128-byte rows by an
+  // exclusive or of the chunk with the row
+  static constexpr bool SWIZZLED = QS == 128;
+  static constexpr int STRIDE = SWIZZLED ? 128 : QS + 16;
   // the super-block's header (Q5_K: and these runs' fifth bits), or an f16 a run
   static constexpr int HEAD = FMT == Q4_K ? 16 : FMT == Q5_K || FMT == Q6_K ? 32 : 2 * RUNS;
   static constexpr uint32_t WARP_BYTES = 32 * (STRIDE + HEAD);
@@ -225,9 +234,9 @@ __host__ __device__ constexpr int stage_cols(int f) {
 }
 
 // Run j of a row's stage, run jb of its super-block, as A operand registers: 16
-// (Q6_K: o and then the low part in o2).
+// (Q6_K: o and then the low part in o2).  sw: what the row's chunks are permuted with.
 template <int FMT>
-__device__ __forceinline__ void unpack(const uint8_t *row, const uint8_t *head, const uint4 &h, int j,
+__device__ __forceinline__ void unpack(const uint8_t *row, int sw, const uint8_t *head, const uint4 &h, int j,
                                        int jb, const uint32_t (&lut)[4], uint32_t (&o)[16],
                                        uint32_t (&o2)[16]) {
   if (FMT == Q4_K || FMT == Q5_K) {
@@ -235,7 +244,7 @@ __device__ __forceinline__ void unpack(const uint8_t *row, const uint8_t *head, 
     q4k_scale_min(jb, h.y, h.z, h.w, sc, mn);
     const uint32_t s = sub2(sc * 0x10001u + both(0x6400u), both(0x6400u));  // (1024 + sc) - 1024
     const uint32_t f = mul2(s, both(H_2P10)), f16th = FMT == Q4_K ? mul2(s, both(H_2P6)) : f;
-    const uint4 q = *reinterpret_cast<const uint4 *>(row + j * 16);
+    const uint4 q = *reinterpret_cast<const uint4 *>(row + ((j ^ sw) << 4));
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
     const uint32_t hb = FMT == Q5_K ? *reinterpret_cast<const uint32_t *>(head + 16 + 4 * j) : 0;
 #pragma unroll
@@ -279,7 +288,7 @@ __device__ __forceinline__ void unpack(const uint8_t *row, const uint8_t *head, 
       }
     }
   } else if (FMT == Q4_0) {
-    const uint4 q = *reinterpret_cast<const uint4 *>(row + j * 16);
+    const uint4 q = *reinterpret_cast<const uint4 *>(row + ((j ^ sw) << 4));
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -292,13 +301,13 @@ __device__ __forceinline__ void unpack(const uint8_t *row, const uint8_t *head, 
   } else {
     uint32_t c[8];  // value + 128, bytes in value order
     if (FMT == Q8_0) {
-      const uint4 a = *reinterpret_cast<const uint4 *>(row + j * 32);
-      const uint4 b = *reinterpret_cast<const uint4 *>(row + j * 32 + 16);
+      const uint4 a = *reinterpret_cast<const uint4 *>(row + (((2 * j) ^ sw) << 4));
+      const uint4 b = *reinterpret_cast<const uint4 *>(row + (((2 * j + 1) ^ sw) << 4));
       const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) c[i] = w[i] ^ 0x80808080u;
     } else {
-      const uint4 q = *reinterpret_cast<const uint4 *>(row + j * 16);
+      const uint4 q = *reinterpret_cast<const uint4 *>(row + ((j ^ sw) << 4));
       const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -344,16 +353,15 @@ __host__ __device__ __forceinline__ int parts_of(int u, int nb, int share) {
   return (int)((uint32_t)((u + 1) * nb - 1) / (uint32_t)share) - first_cta(u, nb, share) + 1;
 }
 
-// Tokens a pass takes at most, by format: 32 tokens need 64 columns of results,
-// which the formats with a result per run (several of them a step) do not have.
-__host__ __device__ constexpr int max_tokens(int fmt) { return k_format(fmt) ? 32 : 16; }
+// Tokens a pass takes at most.  32 would take 256 TMEM columns, two CTAs an SM: 64
+// tokens of eight experts (Q4_K, Q5_K) took 567 us with them and 472 us without, and
+// of a smaller layer 256 tokens, 64 an expert, 345 us and 324 us.
+constexpr int MOST_TOKENS = 16;
 
 // The shape of a kernel for up to T tokens a pass.  TMEM: the A operand of a
 // step (16 columns a run, Q6_K 32), the mins as an operand (8), the results (N a
-// step, or N a run), the min products.  Up to 16 tokens fit 128 columns, so that
-// four CTAs share an SM (three where shared memory does not hold four): their
-// waits for the tensor core, TMEM and memory cover one another.  32 tokens take
-// 256 columns and have room for a second A buffer instead.
+// step, or N a run), the min products.  They fit 128 columns, so that four CTAs
+// share an SM: their waits for the tensor core, TMEM and memory cover one another.
 template <int FMT, int T>
 struct Shape {
   using S = Stage<FMT>;
@@ -361,28 +369,27 @@ struct Shape {
   static constexpr int STEP = FMT == Q6_K || (!k_format(FMT) && T > 8) ? 2 : 4;  // runs
   static constexpr int STEPS = S::RUNS / STEP;
   static constexpr int A_COLS = STEP * (FMT == Q6_K ? 32 : 16);
-  static constexpr int A_BUFS = T > 16 ? 2 : 1;
-  static constexpr int SUM_ROWS = T < 16 ? 16 : T;  // N of the min product
-  static constexpr int MIN_A = A_BUFS * A_COLS;
+  static constexpr int SUM_ROWS = 16;  // N of the min product
+  static constexpr int MIN_A = A_COLS;
   static constexpr int D = MIN_A + (has_min(FMT) ? 8 : 0);
   static constexpr int MIN_D = D + (k_format(FMT) ? N : STEP * N);
   static constexpr int USED = MIN_D + (has_min(FMT) ? SUM_ROWS : 0);
-  static constexpr int TMEM = USED <= 128 ? 128 : 256;
-  static_assert(USED <= 256, "TMEM columns");
+  static constexpr int TMEM = 128;
+  static_assert(USED <= TMEM && T <= SUM_ROWS, "TMEM columns");
   // shared memory: the activation ring (a step: T rows of high and T of low
   // terms, 64 bytes a run), the sums of two stages, the warps' weight rings,
   // barriers; the plan follows
   static constexpr int B_DEPTH = T > 8 || has_min(FMT) ? 2 : 3;
   static constexpr uint32_t B_ATOM = N * 128;  // two runs of every row
   static constexpr uint32_t B_STEP = B_ATOM * (STEP / 2);
-  static constexpr uint32_t SUMS = has_min(FMT) ? SUM_ROWS * 128 : 0;
+  static constexpr uint32_t SUMS = has_min(FMT) ? SUM_ROWS * 32 : 0;
   static constexpr uint32_t BEFORE = 1024 + B_DEPTH * B_STEP + 2 * SUMS + 64;
-  static constexpr uint32_t ROOM = (T > 16 ? 112 : 55) * 1024;  // of a CTA
+  static constexpr uint32_t ROOM = 55 * 1024;  // of a CTA
   static constexpr int W_FIT = (int)((ROOM - BEFORE) / (4 * S::WARP_BYTES));
   static constexpr int W_DEPTH = W_FIT < 2 ? 2 : W_FIT > 4 ? 4 : W_FIT;
   static constexpr uint32_t W_RING = 4 * W_DEPTH * S::WARP_BYTES;
   static constexpr uint32_t FIXED = BEFORE + W_RING;
-  static constexpr int CTAS = TMEM == 256 ? 2 : FIXED <= 56 * 1024 ? 4 : 3;
+  static constexpr int CTAS = FIXED <= 56 * 1024 ? 4 : 3;
 };
 __host__ __device__ inline uint32_t plan_bytes(int experts, int slots) {
   return (uint32_t)(2 * (experts + 1) * 4 + slots * 2 + 15) / 16 * 16;
@@ -553,7 +560,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
           const int blocks = runs / 8, block = f.b * S::RUNS / 8;
           for (int q = lane; q < 2 * f.n; q += 32) {
             const int t = q >> 1, c = q & 1;
-            cp_async16_at(sd + t * 128 + ((c ^ (t & 7)) << 4),
+            cp_async16_at(sd + (t >> 3) * 256 + c * 128 + (t & 7) * 16,
                           p.act.sums + ((uint64_t)list[f.begin + t] * blocks + block) * 16 + c * 8);
           }
           fsum ^= 1;
@@ -565,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
     };
 #pragma unroll
     for (int i = 0; i < X::B_DEPTH - 1; ++i) fetch();
-    const uint64_t b0 = desc_sw128(smem_u32(b_ring)), s0 = desc_sw128(smem_u32(sum_ring));
+    const uint64_t b0 = desc_sw128(smem_u32(b_ring)), s0 = desc_cores(smem_u32(sum_ring));
     Cursor c = start();
     int slot = 0, sum_slot = 0;
     uint32_t q = 0;
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
         if (lane == 0) {
           fence_after();
           const uint64_t bd = b0 + (((uint64_t)slot * X::B_STEP) >> 4);
-          const uint32_t a = tmem + (X::A_BUFS > 1 ? (q & 1) * X::A_COLS : 0);
+          const uint32_t a = tmem;
           const int r = min(STEP, runs - b * S::RUNS - s * STEP);
 #pragma unroll
           for (int j = 0; j < STEP; ++j) {
@@ -644,12 +651,15 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
         const uint32_t at = (uint32_t)f.b * S::QS;
         if (EVEN) {
           const bool mine = lane % PER_ROW < chunks;
-          uint8_t *d = st + (lane / PER_ROW) * S::STRIDE + (lane % PER_ROW) * 16;
-          const int rows = p.rows - frow0 - lane / PER_ROW;  // this lane's rows are below it
+          const int r = lane / PER_ROW, ch = lane % PER_ROW;
+          // (SWIZZLED: rows r + 4 c, of which every second has the same low bits)
+          const uint32_t d = smem_u32(st + r * S::STRIDE) + ((S::SWIZZLED ? ch ^ r : ch) << 4);
+          const int rows = p.rows - frow0 - r;  // this lane's rows are below it
 #pragma unroll
           for (int c = 0; c < 32 / AT_ONCE; ++c)
             if (mine && c * AT_ONCE < rows)
-              cp_async16(d + c * AT_ONCE * S::STRIDE, fq + at + (uint64_t)(c * AT_ONCE) * L.qs_row);
+              cp_async16_at((S::SWIZZLED && (c & 1) ? d ^ 64u : d) + c * AT_ONCE * S::STRIDE,
+                            fq + at + (uint64_t)(c * AT_ONCE) * L.qs_row);
         } else {
 #pragma unroll
           for (int c0 = 0; c0 < PER_ROW * 32; c0 += 32) {
@@ -687,6 +697,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
         for (int c = 0; c < 4; ++c) lut[i] |= (uint32_t)((iq4nl_value(4 * i + c) + 128) & 0xFF) << (8 * c);
 
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const int sw = S::SWIZZLED ? lane & 7 : 0;
     float acc[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) acc[t] = 0.f;
@@ -777,27 +788,20 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
       for (int s = 0; s < STEPS; ++s) {
         if (!KF && s >= steps) break;
         const int r = KF ? STEP : min(STEP, left - s * STEP);
-        // one A buffer: its last reader, the step before, is waited for first; two:
-        // this one's, two steps back, was waited for at the step before
-        if (X::A_BUFS == 1 && q > 0) {
+        if (q > 0) {  // the step before has read the A operand
           collect();
           if (!ok) break;
         }
-        const uint32_t a = lanes + (X::A_BUFS > 1 ? (q & 1) * X::A_COLS : 0);
 #pragma unroll
         for (int j = 0; j < STEP; ++j) {
           if (!KF && j >= r) break;
           uint32_t o[16], o2[16];
-          unpack<FMT>(row, head, h, s * STEP + j, jb0 + s * STEP + j, lut, o, o2);
-          tmem_st16(a + j * 16, o);
-          if (FMT == Q6_K) tmem_st16(a + X::A_COLS / 2 + j * 16, o2);
-        }
-        if (X::A_BUFS > 1 && q > 0) {
-          collect();
-          if (!ok) break;
+          unpack<FMT>(row, sw, head, h, s * STEP + j, jb0 + s * STEP + j, lut, o, o2);
+          tmem_st16(lanes + j * 16, o);
+          if (FMT == Q6_K) tmem_st16(lanes + X::A_COLS / 2 + j * 16, o2);
         }
         if (has_min(FMT) && s == 0) {
-          // (one buffer: after the step before is done)  The stage's mins as f16 integers (zero for the runs of the super-block's
+          // the stage's mins as f16 integers (zero for the runs of the super-block's
           // other stage), twice: for the high and the low terms of the sums
           uint32_t m[8];
 #pragma unroll

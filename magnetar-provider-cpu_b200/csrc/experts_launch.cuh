@@ -46,8 +46,6 @@ template <int FMT>
 cudaError_t launch_moe_product(const moe::Args *a, int tokens, int sms, int *ctas_per_sm,
                                cudaStream_t stream) {
   if (tokens == 8) return launch_moe_one<FMT, 8>(a, sms, ctas_per_sm, stream);
-  if constexpr (moe::max_tokens(FMT) > 16)
-    if (tokens == 32) return launch_moe_one<FMT, 32>(a, sms, ctas_per_sm, stream);
   return launch_moe_one<FMT, 16>(a, sms, ctas_per_sm, stream);
 }
 
