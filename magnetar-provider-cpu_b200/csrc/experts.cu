@@ -7,6 +7,8 @@
 // slots.  The two products are in experts.cuh.
 #include <cooperative_groups.h>
 
+#include <climits>
+
 #include "experts.cuh"
 
 namespace mgb {
@@ -27,7 +29,7 @@ __device__ __forceinline__ void pack_row(int fmt, const float *x, uint64_t row, 
   const int lane = threadIdx.x & 31;
   const float *xr = x + row * cols;
   float mx = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int j = threadIdx.x; j < cols; j += CTA_THREADS) mx = fmaxf(mx, fabsf(xr[j]));
 #pragma unroll
   for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
@@ -48,9 +50,18 @@ __global__ void __launch_bounds__(256)
   pack_row<256>(fmt, x, blockIdx.y, cols, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8, o);
 }
 
+// Doubles as integers in the same order, -0 as +0, NaN (0) below all, and back.
+__device__ __forceinline__ uint64_t order_key(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+  return v != v ? 0 : b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double order_value(uint64_t k) {
+  return __longlong_as_double((long long)(k >> 63 ? k ^ 1ull << 63 : ~k));
+}
+
 // One cluster per token: its warps take the experts' logits and, with `pack`,
 // the token's runs; the first CTA's first warp then picks.  A logit is a sum of
-// f32 products in chains of hidden / 128 a lane, joined in f64.
+// f32 products in chains of at most hidden / 128 a lane, joined in f64.
 __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREADS)
     mgb_moe_route_kernel(const float *__restrict__ router, int experts, int hidden,
                          const float *x, int top_k, int normalize, float scale, float *ids,
@@ -68,12 +79,17 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
   double *zs = cluster.map_shared_rank(z, 0);
   const float *xr = x + (size_t)token * hidden;
   const bool wide = hidden % 4 == 0 && ((uintptr_t)router & 15) == 0 && ((uintptr_t)x & 15) == 0;
-  for (int e = warp; e < experts; e += WARPS) {
-    const float *r = router + (size_t)e * hidden;
+  // few experts: several warps each, a stretch of the columns a warp
+  int stretches = 1;
+  while (experts * stretches * 2 <= WARPS && hidden >= 1024 * stretches) stretches *= 2;
+  const int columns = (hidden / stretches + 127) & ~127;
+  for (int i = warp; i < experts * stretches; i += WARPS) {
+    const int from = min(hidden, i % stretches * columns), to = min(hidden, from + columns);
+    const float *r = router + (size_t)(i / stretches) * hidden;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (wide) {
-#pragma unroll 4
-      for (int j = lane * 4; j < hidden; j += 128) {
+#pragma unroll 8
+      for (int j = from + lane * 4; j < to; j += 128) {
         const float4 a = *reinterpret_cast<const float4 *>(xr + j);
         const float4 b = __ldg(reinterpret_cast<const float4 *>(r + j));
         s[0] = fmaf(a.x, b.x, s[0]);
@@ -82,56 +98,65 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
         s[3] = fmaf(a.w, b.w, s[3]);
       }
     } else {
-      for (int j = lane; j < hidden; j += 128)
+      for (int j = from + lane; j < to; j += 128)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          if (j + 32 * c < hidden) s[c] = fmaf(xr[j + 32 * c], r[j + 32 * c], s[c]);
+          if (j + 32 * c < to) s[c] = fmaf(xr[j + 32 * c], r[j + 32 * c], s[c]);
     }
     double d = ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) zs[e] = d;
+    if (lane == 0) zs[i] = d;
   }
   if (pack) pack_row<ROUTE_THREADS>(fmt, x, token, hidden, warp, WARPS, packed);
   cluster.sync();
   if (rank || threadIdx.x >= 32) return;
-
-  // best-first: the largest logit left, the lowest id among equals, NaN last
-  auto before = [](double a, int i, double b, int j) {  // (a, i) sorts before (b, j)
-    if (i < 0 || j < 0) return i >= 0;
-    const bool na = a != a, nb = b != b;
-    if (na || nb) return na == nb ? i < j : nb;
-    return a > b || (a == b && i < j);
-  };
-  uint32_t taken = 0;  // bit c: expert 32 c + lane
-  double top = 0.0, total = 0.0, sum = 0.0, mine = 0.0;  // lane k keeps choice k's share
-  for (int k = 0; k < top_k; ++k) {
-    double v = 0.0;
-    int best = -1;
-    for (int c = 0; c * 32 + lane < experts; ++c)
-      if (!(taken >> c & 1) && before(z[c * 32 + lane], c * 32 + lane, v, best))
-        v = z[c * 32 + lane], best = c * 32 + lane;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const double ov = __shfl_xor_sync(0xffffffffu, v, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, best, o);
-      if (before(ov, oi, v, best)) v = ov, best = oi;
-    }
-    if ((best & 31) == lane) taken |= 1u << (best >> 5);
-    if (k == 0) {
-      top = v;
-      if (!normalize) {
-        for (int e = lane; e < experts; e += 32) total += exp(z[e] - top);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      }
-    }
-    const double share = exp(v - top);
-    sum += share;
-    if (lane == k) mine = share, ids[(size_t)token * top_k + k] = (float)best;
+  if (stretches > 1) {  // (at most 32 experts)
+    double d = 0.0;
+    if (lane < experts)
+      for (int i = 0; i < stretches; ++i) d += z[lane * stretches + i];
+    __syncwarp();
+    if (lane < experts) z[lane] = d;
+    __syncwarp();
   }
-  if (lane < top_k)
-    weights[(size_t)token * top_k + lane] = (float)(mine / (normalize ? sum : total) * (double)scale);
+
+  // Best first: the largest logit left, the lowest id among equals, NaN last.  A lane
+  // keeps the best of its experts lane, lane + 32, ..., and looks again when that is
+  // taken; the warp's best by three reductions of words.
+  uint32_t taken = 0;  // bit c: expert 32 c + lane
+  uint64_t key = 0;
+  int best = INT_MAX;
+  auto look = [&]() {
+    key = 0, best = INT_MAX;
+    for (int c = 0; c * 32 + lane < experts; ++c) {
+      if (taken >> c & 1) continue;
+      const uint64_t k = order_key(z[c * 32 + lane]);
+      if (best == INT_MAX || k > key) key = k, best = c * 32 + lane;
+    }
+  };
+  look();
+  uint64_t mine = 0;  // of the lane-th choice
+  for (int k = 0; k < top_k; ++k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+    const bool a = (uint32_t)(key >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, a ? (uint32_t)key : 0u);
+    const int e = __reduce_min_sync(0xffffffffu, a && (uint32_t)key == lo ? best : INT_MAX);
+    if (lane == k) mine = (uint64_t)hi << 32 | lo, ids[(size_t)token * top_k + k] = (float)e;
+    if (e == best) {
+      taken |= 1u << (e >> 5);
+      look();
+    }
+  }
+  const double v = order_value(mine), top = __shfl_sync(0xffffffffu, v, 0);
+  const double share = lane < top_k ? exp(v - top) : 0.0;
+  double total = share;
+  if (!normalize) {
+    total = 0.0;
+    for (int e = lane; e < experts; e += 32) total += exp(z[e] - top);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane < top_k) weights[(size_t)token * top_k + lane] = (float)(share / total * (double)scale);
 }
 
 // How the parts of a product are found: what its kernel left and the shapes.
@@ -145,18 +170,7 @@ struct Parts {
 __device__ __forceinline__ int tile_parts(const Parts &p, int place, int share, int tile) {
   return moe::parts_of((place >> 16) * p.tiles + tile, p.nb, share);
 }
-// The sum of n parts of value c of a slot; the first two (all there are in most
-// tiles) are loaded together.
-__device__ __forceinline__ float part_sum(const Parts &p, int place, int used, int n, int c) {
-  const float *at = p.out + (uint64_t)(place & 0xFFFF) * p.width + c;
-  const uint64_t step = (uint64_t)used * p.width;
-  float s = at[0];
-  if (n > 1) s += at[step];
-  for (int i = 2; i < n; ++i) s += at[i * step];
-  return s;
-}
-
-// Four values (c and the rows' widths are multiples of 32).
+// The sum of n parts of a slot's result, in order: four values (c and the rows' widths are multiples of 32).
 __device__ __forceinline__ float4 part_sum4(const Parts &p, int place, int used, int n, int c) {
   const float *at = p.out + (uint64_t)(place & 0xFFFF) * p.width + c;
   const uint64_t step = (uint64_t)used * p.width;
@@ -235,13 +249,33 @@ __global__ void __launch_bounds__(256)
   const int token = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
   if (c >= hidden) return;
   const int share = p.share[0], used = p.share[1];
+  const uint64_t step = (uint64_t)used * p.width;
   float a = 0.f;
-#pragma unroll 4
-  for (int j = 0; j < top_k; ++j) {
-    const int place = p.place[token * top_k + j];
-    if (place < 0) continue;
-    const int n = tile_parts(p, place, share, c / moe::TILE);
-    a = fmaf(weights[token * top_k + j], part_sum(p, place, used, n, c), a);
+  for (int j0 = 0; j0 < top_k; j0 += 4) {  // four slots' loads at a time
+    int n[4];
+    float w[4], v[4], v1[4];
+    const float *at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = token * top_k + min(j0 + i, top_k - 1);
+      const int place = j0 + i < top_k ? p.place[j] : -1;
+      w[i] = weights[j];
+      n[i] = place < 0 ? 0 : tile_parts(p, place, share, c / moe::TILE);
+      at[i] = p.out + (uint64_t)(place & 0xFFFF) * p.width + c;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = n[i] > 0 ? at[i][0] : 0.f;
+      v1[i] = n[i] > 1 ? at[i][step] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!n[i]) continue;  // (not even a NaN weight of it counts)
+      float s = v[i];
+      if (n[i] > 1) s += v1[i];
+      for (int q = 2; q < n[i]; ++q) s += at[i][q * step];
+      a = fmaf(w[i], s, a);
+    }
   }
   const size_t at = (size_t)token * hidden + c;
   y[at] = addend ? addend[at] + a : a;

@@ -10,14 +10,16 @@
 // rounding: a code masked out of its quant word is an f16 subnormal (q 2^-24, or
 // 16 times that for the next nibble), one f16 multiply by the run's integer
 // scale (Q4_K, Q5_K: sc q <= 1953 < 2048) or one multiply-add with the code's
-// offset gives an exact normal number.  Two codes a register, written to TMEM
+// offset gives an exact number.  Two codes a register, written to TMEM
 // (tcgen05.st) as the A operand: nothing goes back through shared memory.  What
 // is left of a weight's scale is one f32 factor per row and 256 values (K
 // formats) or per row and 32 values (the others), which multiplies the MMA's
 // result as it is read from TMEM into the row's f32 sums.  Q6_K's products
-// sc (q - 32) need 13 bits: they enter as two operands, sc ((q >> 1) - 16) and
-// sc (q & 1) / 2.  Q4_K's and Q5_K's mins multiply the runs' activation sums,
-// by one more MMA a block (8 runs, two terms each).
+// sc (q - 32) need 13 bits: they enter as two operands, sc n of the low nibble
+// and 16 sc (h - 2) of the two high bits, which so need no joining (one token of
+// two wide experts: 132 us with joined codes split by their lowest bit, 112 us so).
+// Q4_K's and Q5_K's mins multiply the runs' activation sums, by one more MMA a
+// block (8 runs, two terms each).
 //
 // Activations.  A row is held as 2^-k (hi + lo), two f16 terms with k such that
 // the row's largest value lies in [2^13, 2^14): 22 bits of every value down to
@@ -227,7 +229,7 @@ struct Stage {
   static constexpr int HEAD = FMT == Q4_K ? 16 : FMT == Q5_K || FMT == Q6_K ? 32 : 2 * RUNS;
   static constexpr uint32_t WARP_BYTES = 32 * (STRIDE + HEAD);
   // f32 factor that undoes the codes' scaling
-  static constexpr float UNIT = FMT == Q4_K || FMT == Q5_K ? 16384.f : FMT == Q6_K ? 2048.f : 1024.f;
+  static constexpr float UNIT = FMT == Q4_K || FMT == Q5_K ? 16384.f : FMT == Q6_K ? 1048576.f : 1024.f;
 };
 __host__ __device__ constexpr int stage_cols(int f) {
   return f == Q4_K || f == Q4_0 || f == IQ4_NL ? 256 : 128;
@@ -271,20 +273,26 @@ __device__ __forceinline__ void unpack(const uint8_t *row, int sw, const uint8_t
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
     const uint32_t sp = *reinterpret_cast<const uint16_t *>(head + 2 * jb) ^ 0x8080u;  // + 128 each
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t sc = (i < 2 ? sp : sp >> 8) & 0xFFu;
-      const uint32_t s = sub2(sc * 0x10001u + both(0x6400u), both(0x6480u));  // -1152
-      const uint32_t half = mul2(s, both(0x1000u));  // s 2^-11
-      uint32_t ev, od;
-      q6k_codes(w[i], i < 2 ? hw.x : hw.y, i, ev, od);
-      const uint32_t c[4] = {ev & 0x00FF00FFu, od & 0x00FF00FFu, (ev >> 8) & 0x00FF00FFu,
-                             (od >> 8) & 0x00FF00FFu};
+    for (int a = 0; a < 2; ++a) {  // 16 values of one scale
+      const uint32_t sc = (a ? sp >> 8 : sp) & 0xFFu;
+      const uint32_t s = sub2(sc * 0x10001u + both(0x6400u), both(0x6480u));  // - 1152
+      const uint32_t s2 = mul2(s, both(0x4400u)), s4 = mul2(s, both(0x4C00u));  // s 2^2, s 2^4
+      const uint32_t s6 = mul2(s, both(H_2P6)), s8 = mul2(s, both(0x5C00u));
+      const uint32_t off = mul2(s, both(0x8200u));  // -s 2^-15
+      const uint32_t hs = a ? hw.y : hw.x, ht = hs >> 8;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        // ((c >> 1) - 16) 2^-10 times sc; (c & 1) times sc 2^-11
-        const uint32_t top = fma2((c[r] >> 1) & 0x001F001Fu, both(H_2P14), both(0xA400u));
-        o[4 * i + r] = mul2(top, s);
-        o2[4 * i + r] = mul2((c[r] & 0x00010001u) * 0x3C00u, half);
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t n = w[2 * a + b], u = n >> 8;
+        const int at = 8 * a + 4 * b;
+        o[at] = mul2(n & 0x000F000Fu, s4);
+        o[at + 1] = mul2(n & 0x00F000F0u, s);
+        o[at + 2] = mul2(u & 0x000F000Fu, s4);
+        o[at + 3] = mul2(u & 0x00F000F0u, s);
+        const uint32_t even = b ? 0x00300030u : 0x00030003u, odd = even << 2;
+        o2[at] = fma2(hs & even, b ? s4 : s8, off);
+        o2[at + 1] = fma2(hs & odd, b ? s2 : s6, off);
+        o2[at + 2] = fma2(ht & even, b ? s4 : s8, off);
+        o2[at + 3] = fma2(ht & odd, b ? s2 : s6, off);
       }
     }
   } else if (FMT == Q4_0) {
@@ -630,7 +638,6 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
     uint8_t *ring = w_ring + warp * X::W_DEPTH * S::WARP_BYTES;
     const bool aligned = KF || L.sc_row % 16 == 0;
     constexpr int PER_ROW = S::QS / 16, AT_ONCE = 32 / PER_ROW;  // chunks of a row; rows a copy round
-    constexpr bool EVEN = 32 % PER_ROW == 0;                     // (Q6_K: 6 chunks a row)
     Cursor f = start();
     int fslot = 0, frow0 = 0;
     const uint8_t *fq = nullptr, *fh = nullptr;  // this lane's quants and header of stage 0
@@ -639,7 +646,7 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
       const uint8_t *w = second ? p.w1 : p.w0;
       frow0 = (second ? f.tile - tiles1 : f.tile) * TILE + warp * 32;
       const uint64_t row = (uint64_t)f.expert * p.rows + frow0;
-      fq = EVEN ? w + (row + lane / PER_ROW) * L.qs_row + (lane % PER_ROW) * 16 : w + row * L.qs_row;
+      fq = w + (row + lane / PER_ROW) * L.qs_row + (lane % PER_ROW) * 16;
       fh = w + L.qs_bytes + (row + lane) * L.sc_row;
     };
     if (f.left > 0) point();
@@ -649,25 +656,16 @@ __global__ void __launch_bounds__(THREADS, Shape<FMT, T>::CTAS) mgb_moe_product_
         const int left = runs - f.b * S::RUNS;
         const int chunks = left >= S::RUNS ? PER_ROW : FMT == Q8_0 ? 2 * left : FMT == Q6_K ? left * 3 / 2 : left;
         const uint32_t at = (uint32_t)f.b * S::QS;
-        if (EVEN) {
-          const bool mine = lane % PER_ROW < chunks;
-          const int r = lane / PER_ROW, ch = lane % PER_ROW;
-          // (SWIZZLED: rows r + 4 c, of which every second has the same low bits)
-          const uint32_t d = smem_u32(st + r * S::STRIDE) + ((S::SWIZZLED ? ch ^ r : ch) << 4);
-          const int rows = p.rows - frow0 - r;  // this lane's rows are below it
+        const int r = lane / PER_ROW, ch = lane % PER_ROW;
+        const bool mine = r < AT_ONCE && ch < chunks;
+        // (SWIZZLED: rows r + 4 c, of which every second has the same low bits)
+        const uint32_t d = smem_u32(st + r * S::STRIDE) + ((S::SWIZZLED ? ch ^ r : ch) << 4);
+        const int rows = min(32, p.rows - frow0) - r;  // this lane's rows are below it
 #pragma unroll
-          for (int c = 0; c < 32 / AT_ONCE; ++c)
-            if (mine && c * AT_ONCE < rows)
-              cp_async16_at((S::SWIZZLED && (c & 1) ? d ^ 64u : d) + c * AT_ONCE * S::STRIDE,
-                            fq + at + (uint64_t)(c * AT_ONCE) * L.qs_row);
-        } else {
-#pragma unroll
-          for (int c0 = 0; c0 < PER_ROW * 32; c0 += 32) {
-            const int r = (c0 + lane) / PER_ROW, c = (c0 + lane) % PER_ROW;
-            if (frow0 + r < p.rows && c < chunks)
-              cp_async16(st + r * S::STRIDE + c * 16, fq + at + (uint64_t)r * L.qs_row + c * 16);
-          }
-        }
+        for (int c = 0; c < (31 + AT_ONCE) / AT_ONCE; ++c)
+          if (mine && c * AT_ONCE < rows)
+            cp_async16_at((S::SWIZZLED && (c & 1) ? d ^ 64u : d) + c * AT_ONCE * S::STRIDE,
+                          fq + at + (uint64_t)(c * AT_ONCE) * L.qs_row);
         if (frow0 + lane < p.rows && aligned) {
           uint8_t *d = st + 32 * S::STRIDE + lane * S::HEAD;
           if (FMT == Q5_K) {
