@@ -229,7 +229,7 @@ struct Stage {
   static constexpr int HEAD = FMT == Q4_K ? 16 : FMT == Q5_K || FMT == Q6_K ? 32 : 2 * RUNS;
   static constexpr uint32_t WARP_BYTES = 32 * (STRIDE + HEAD);
   // f32 factor that undoes the codes' scaling
-  static constexpr float UNIT = FMT == Q4_K || FMT == Q5_K ? 16384.f : FMT == Q6_K ? 1048576.f : 1024.f;
+  static constexpr float UNIT = FMT == Q4_K || FMT == Q5_K ? 16384.f : FMT == Q6_K ? 1048576.f : FMT == Q4_0 ? 1024.f : 1.f;
 };
 __host__ __device__ constexpr int stage_cols(int f) {
   return f == Q4_K || f == Q4_0 || f == IQ4_NL ? 256 : 128;
@@ -325,9 +325,9 @@ __device__ __forceinline__ void unpack(const uint8_t *row, int sw, const uint8_t
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // (c - 128) 2^-10
-      o[2 * i] = fma2(c[i] & 0x00FF00FFu, both(H_2P14), both(0xB000u));
-      o[2 * i + 1] = fma2((c[i] >> 8) & 0x00FF00FFu, both(H_2P14), both(0xB000u));
+    for (int i = 0; i < 8; ++i) {  // the bytes under 0x64: (1024 + c) - 1152
+      o[2 * i] = sub2(__byte_perm(c[i], 0x64646464u, 0x4240u), both(0x6480u));
+      o[2 * i + 1] = sub2(__byte_perm(c[i], 0x64646464u, 0x4341u), both(0x6480u));
     }
   }
 }
