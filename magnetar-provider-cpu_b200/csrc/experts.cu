@@ -289,8 +289,13 @@ static int current_sms() {
   return device_sms(dev);
 }
 
-// Tokens of one expert in a pass over its rows: m is the most it can have.
-static int pass_tokens(uint64_t m) { return m <= 8 ? 8 : moe::MOST_TOKENS; }
+// Tokens of one expert in a pass over its rows: 8 where no expert has more (m) or
+// few will.  At 2, 4, 6 and 8 tokens an expert (64 or 16 experts, Q8_0) 8 a pass
+// take 199, 263, 88 and 102 us and 16 take 245, 279, 98 and 103 us; in Q4_K 161, 194,
+// 77 and 87 us, and 166, 196, 73 and 76 us.
+static int pass_tokens(uint64_t m, uint64_t slots, uint64_t experts) {
+  return m <= 8 || slots <= 4 * experts ? 8 : moe::MOST_TOKENS;
+}
 
 static cudaError_t moe_product(int fmt, const moe::Args *a, int tokens, int sms, int *ctas_per_sm,
                                cudaStream_t stream) {
@@ -339,7 +344,7 @@ struct MoeScratch {
     for (int i = 0; i < 2; ++i) place[i] = take(slots * 4), share[i] = take(8);
     // the second product's results take the first one's place
     auto rows = [&](int fmt, uint64_t tiles) {
-      const int tokens = pass_tokens(m);
+      const int tokens = pass_tokens(m, slots, ex.experts);
       int per_sm = 0;
       moe_product(fmt, nullptr, tokens, sms, &per_sm, nullptr);
       return part_rows(slots, tokens, tiles, (uint64_t)sms * per_sm);
@@ -404,6 +409,7 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   const MoeScratch s(ex, m, top_k, sms);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   const int hidden = (int)ex.hidden, ffn = (int)ex.ffn, slots = (int)(m * top_k);
+  const int tokens = pass_tokens(m, slots, ex.experts);
   if (!packed) {
     e = launch_chained(mgb_moe_pack_kernel, dim3((unsigned)ceil_div(hidden / RUN, 32), (unsigned)m),
                        dim3(256), 0, stream, ex.gate_up_format, x, hidden, s.x(ws));
@@ -425,9 +431,10 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   a.cols = hidden;
   a.slots = slots;
   a.act_div = (int)top_k;
-  e = moe_product(ex.gate_up_format, &a, pass_tokens(m), sms, nullptr, stream);
+  e = moe_product(ex.gate_up_format, &a, tokens, sms, nullptr, stream);
   if (e != cudaSuccess) return e;
-  const Parts gu{a.out, a.place, a.share, 2 * (int)ceil_div(ffn, moe::TILE), (int)ceil_div(hidden, moe::stage_cols(ex.gate_up_format)), 2 * ffn};
+  const Parts gu{a.out, a.place, a.share, 2 * (int)ceil_div(ffn, moe::TILE),
+                 (int)ceil_div(hidden, moe::stage_cols(ex.gate_up_format)), 2 * ffn};
   const uint32_t h_smem = (uint32_t)h_runs(ffn) * RUN * 4;
   if (h_smem > 48 * 1024) {
     e = cudaFuncSetAttribute(mgb_moe_h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h_smem);
@@ -445,9 +452,9 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   a.rows = hidden;
   a.cols = ffn;
   a.act_div = 1;
-  e = moe_product(ex.down_format, &a, pass_tokens(m), sms, nullptr, stream);
+  e = moe_product(ex.down_format, &a, tokens, sms, nullptr, stream);
   if (e != cudaSuccess) return e;
-  const Parts dn{a.out, a.place, a.share, (int)ceil_div(hidden, moe::TILE), 
+  const Parts dn{a.out, a.place, a.share, (int)ceil_div(hidden, moe::TILE),
                  (int)ceil_div(ffn, moe::stage_cols(ex.down_format)), hidden};
   return launch_chained(mgb_moe_combine_kernel, dim3((unsigned)ceil_div(hidden, 256), (unsigned)m),
                         dim3(256), 0, stream, dn, weights, hidden, (int)top_k, addend, y);
