@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "common.cuh"
@@ -62,6 +63,7 @@ struct Params {
   int tile_rows;     // rows of a tile: 16, 32 or 64
   int splits;        // slices of k (the CTAs of a cluster, or of the grid)
   bool wide_a, wide_b, wide_x, wide_y;  // 16-byte loads are aligned
+  bool early;        // B's ring and the parts of h do not share their place
 };
 
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -73,45 +75,65 @@ __device__ __forceinline__ void grid_dependents() {
 
 // Shared memory of a CTA that plans for itself.
 struct SmallPlan {
-  int id[INLINE_ROWS];
-  int16_t order[INLINE_ROWS], head[INLINE_ROWS];
+  alignas(16) int id[INLINE_ROWS];
+  int16_t order[INLINE_ROWS];
   Tile tiles[INLINE_ROWS];
-  int ntiles;
+  uint32_t heads[INLINE_ROWS / 32];  // the positions at which tiles start
 };
 
-// Rows sorted by (id, row), tiles of up to tile_rows rows of one id.
-__device__ void plan_small(const Params &p, SmallPlan &s, bool report) {
-  const int i = threadIdx.x;
-  if (i == 0) s.ntiles = 0;
-  int id = -1;
-  if (i < p.m) {
-    id = adapter_of(p.ids[i], p.count);
-    if (id == -2) {
-      if (report && p.bad) atomicMin(p.bad, (uint32_t)i);
-      id = -1;
+// Rows sorted by (id, row), tiles of up to tile_rows rows of one id; returns their
+// number.
+__device__ __forceinline__ int plan_small(const Params &p, SmallPlan &s, bool report) {
+  if (threadIdx.x < INLINE_ROWS) {
+    const int i = threadIdx.x;
+    int id = INT_MAX;
+    if (i < p.m) {
+      id = adapter_of(p.ids[i], p.count);
+      if (id == -2) {
+        if (report && p.bad) atomicMin(p.bad, (uint32_t)i);
+        id = -1;
+      }
     }
     s.id[i] = id;
+    if (i < INLINE_ROWS / 32) s.heads[i] = 0;
   }
   __syncthreads();
+  // two threads a row, four where that is all of them
+  const int several = p.m <= 64 ? 4 : 2, i = threadIdx.x / several, sub = threadIdx.x % several;
+  static_assert(32 * WARPS == 2 * INLINE_ROWS, "two threads a row");
+  const int id = s.id[i];
   int pos = 0, nth = 0, same = 0;
-  if (i < p.m) {
-    for (int j = 0; j < p.m; ++j) {
-      const int o = s.id[j];
-      pos += o < id || (o == id && j < i);
-      nth += o == id && j < i;
-      same += o == id;
+  if (i < p.m)
+    for (int j0 = 4 * sub; j0 < p.m; j0 += 4 * several) {
+      const int4 four = *reinterpret_cast<const int4 *>(s.id + j0);
+      const int o[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool before = o[c] == id && j0 + c < i;
+        pos += o[c] < id || before;
+        nth += before;
+        same += o[c] == id;
+      }
     }
-    s.order[pos] = (int16_t)i;
-    s.head[pos] = nth % p.tile_rows == 0;
+  for (int d = 1; d < several; d <<= 1) {
+    pos += __shfl_xor_sync(0xffffffffu, pos, d);
+    nth += __shfl_xor_sync(0xffffffffu, nth, d);
+    same += __shfl_xor_sync(0xffffffffu, same, d);
   }
+  const bool row = i < p.m && sub == 0, head = row && nth % p.tile_rows == 0;
+  if (row) s.order[pos] = (int16_t)i;
+  if (head) atomicOr(&s.heads[pos >> 5], 1u << (pos & 31));
   __syncthreads();
-  if (i < p.m && nth % p.tile_rows == 0) {
-    int t = 0;
-    for (int j = 0; j < pos; ++j) t += s.head[j];
-    s.tiles[t] = Tile{pos, min(p.tile_rows, same - nth), id};
-    if (pos + min(p.tile_rows, same - nth) == p.m) s.ntiles = t + 1;
+  int before = 0, all = 0;  // tiles that start earlier; tiles
+#pragma unroll
+  for (int w = 0; w < INLINE_ROWS / 32; ++w) {
+    const uint32_t h = s.heads[w];
+    all += __popc(h);
+    before += __popc(w < pos >> 5 ? h : w == pos >> 5 ? h & ((1u << (pos & 31)) - 1) : 0u);
   }
+  if (head) s.tiles[before] = Tile{pos, min(p.tile_rows, same - nth), id};
   __syncthreads();
+  return all;
 }
 
 __device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {  // exclusive
@@ -235,8 +257,7 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
 __device__ __forceinline__ bool find_tile(const Params &p, int t, SmallPlan &plan, int (&rows)[MOST_ROWS],
                                           bool report, Tile &tile) {
   const bool small = p.m <= INLINE_ROWS;
-  if (small) plan_small(p, plan, report);
-  if (t >= (small ? plan.ntiles : *p.ntiles)) return false;
+  if (t >= (small ? plan_small(p, plan, report) : *p.ntiles)) return false;
   tile = small ? plan.tiles[t] : p.tiles[t];
   if (threadIdx.x < MOST_ROWS) {
     const int i = tile.start + (threadIdx.x < tile.len ? threadIdx.x : 0);
@@ -349,8 +370,8 @@ struct Pairs {
 
 // ---- the kernel --------------------------------------------------------------------------------
 
-__device__ __forceinline__ void cp_async16(void *dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -367,7 +388,8 @@ template <typename T, int RC>
 struct Shared {
   static constexpr uint32_t ROW = RC * sizeof(T) + 16;  // neighbouring rows in different banks
   static constexpr uint32_t STAGE = COLS * ROW;
-  static constexpr int DEPTH = 2;
+  // as many stages as two CTAs an SM leave room for (f32 factors: one)
+  static constexpr int DEPTH = sizeof(T) == 4 || RC == 64 ? 2 : 96 / RC;
   static constexpr uint32_t RING = WARPS * DEPTH * STAGE;
 };
 __host__ __device__ inline int h_width(int rank, int rc) { return (rank + rc - 1) / rc * rc; }
@@ -434,6 +456,96 @@ __device__ __forceinline__ void shrink(const Params &p, const Tile &tile, const 
   }
 }
 
+// Few rows (of an adapter of up to 64 ranks): plain f32 arithmetic, of which a tensor
+// core's tile would leave most unused.
+constexpr int FEW = 4;
+__device__ __forceinline__ bool few_rows(const Params &p, const Tile &tile) {
+  return tile.len <= FEW && p.tile_rows == MOST_ROWS;
+}
+
+// shrink for few rows, two of them at a time.  A thread takes 4 neighbouring k of 16
+// ranks; a warp's lanes hand one another halves of their sums until each has one.
+template <typename T>
+__device__ __forceinline__ void shrink_few(const Params &p, const Tile &tile, const int (&rows)[MOST_ROWS],
+                                           int g0, int g1, int width, float *part) {
+  constexpr int RB = 16, PAIR = 2;
+  static_assert(FEW * (1 + WARPS) <= MOST_ROWS, "a part a warp");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = width + 4;
+  const T *a = static_cast<const T *>(p.a) + (uint64_t)tile.id * p.rank * p.k;
+  float *mine = part + (FEW + warp * FEW) * stride;
+  const int end = min(p.k, g1 * 32);
+  const bool wide = p.wide_a && p.wide_x;  // (k is a multiple of 4 then)
+  for (int i0 = 0; i0 < tile.len; i0 += PAIR) {
+    const float *x0 = p.x + (uint64_t)rows[i0] * p.k, *x1 = p.x + (uint64_t)rows[min(i0 + 1, tile.len - 1)] * p.k;
+    for (int r0 = 0; r0 < width; r0 += RB) {
+      float acc[PAIR][RB];
+#pragma unroll
+      for (int i = 0; i < PAIR; ++i)
+#pragma unroll
+        for (int r = 0; r < RB; ++r) acc[i][r] = 0.f;
+      for (int k = g0 * 32 + threadIdx.x * 4; k < end; k += WARPS * 128) {
+        Pairs<T, 4> w[RB];
+        Pairs<float, 4> v[PAIR];
+        if (wide) {  // (all loads before the first use)
+#pragma unroll
+          for (int r = 0; r < RB; ++r) w[r].load(a + (uint64_t)min(r0 + r, p.rank - 1) * p.k + k, 4, true);
+          v[0].load(x0 + k, 4, true);
+          v[1].load(x1 + k, 4, true);
+        } else {
+#pragma unroll
+          for (int r = 0; r < RB; ++r)
+            w[r].load(a + (uint64_t)min(r0 + r, p.rank - 1) * p.k + k, end - k, false);
+          v[0].load(x0 + k, end - k, false);
+          v[1].load(x1 + k, end - k, false);
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const float2 f = w[r].pair(s);
+#pragma unroll
+            for (int i = 0; i < PAIR; ++i) {
+              const float2 u = v[i].pair(s);
+              acc[i][r] = fmaf(f.y, u.y, fmaf(f.x, u.x, acc[i][r]));
+            }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < PAIR; ++i) {
+#pragma unroll
+        for (int o = 16, half = RB / 2; half; o >>= 1, half >>= 1)
+#pragma unroll
+          for (int r = 0; r < half; ++r) {
+            const float keep = lane & o ? acc[i][r + half] : acc[i][r];
+            const float give = lane & o ? acc[i][r] : acc[i][r + half];
+            acc[i][r] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        const float s = acc[i][0] + __shfl_xor_sync(0xffffffffu, acc[i][0], 1);
+        const int r = r0 + (lane >> 1);
+        if ((lane & 1) == 0 && i0 + i < tile.len) mine[(i0 + i) * stride + r] = r < p.rank ? s : 0.f;
+      }
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < tile.len * width; e += 32 * WARPS) {
+    const int at = e / width * stride + e % width;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += part[(FEW + w * FEW) * stride + at];
+    part[at] = s;
+  }
+  __syncthreads();
+}
+
+// h of few rows, [rows][width].
+template <typename F>
+__device__ __forceinline__ void h_values(float *h, int len, int width, const F &sum) {
+  for (int e = threadIdx.x; e < len * width / 2; e += 32 * WARPS) {
+    const int row = e / (width / 2), r = e % (width / 2) * 2;
+    *reinterpret_cast<float2 *>(h + row * width + r) = sum(row, r);
+  }
+}
+
 // h as operands: lane (g, t) of step q RC / 8 + s multiplies ranks q RC + t RC / 4 +
 // 2 s and the next.  sum(row, r): h of the tile's row at ranks r and r + 1.
 template <int RC, typename F>
@@ -453,45 +565,166 @@ __device__ __forceinline__ void h_operands(uint4 *hs, int mts, int width, const 
   }
 }
 
-// y = base + B h for the blocks of 32 outputs first, first + step, ... of this
-// warp.  Its four MMA column blocks are interleaved so that a lane ends up with 8
+// A warp's copies of B where 16-byte copies are aligned (WIDE): its blocks of 32
+// outputs first, first + step, ..., a pass of RC ranks of a block a stage, DEPTH
+// ahead.
+template <typename T, int RC, bool WIDE>
+struct Copies {
+  using SM = Shared<T, RC>;
+  static constexpr int CHUNKS = RC * sizeof(T) / 16;
+  static constexpr int ROWS = 32 / CHUNKS;  // of B at a time: a lane copies chunk lane % CHUNKS of one
+  const T *b;
+  uint8_t *ring;
+  int n, last, next, passes;
+  int fc, fp = 0, fslot = 0;
+  const uint8_t *src;                         // this lane's first chunk of the stage to be fetched
+  uint32_t dst, rows_step, block_step, have;  // bytes; have: of a row from the lane's chunk on
+  __device__ __forceinline__ Copies(const Params &p, const Tile &tile, int width, uint8_t *rings, int first,
+                                    int end, int step)
+      : b(static_cast<const T *>(p.b) + (uint64_t)max(tile.id, 0) * p.n * p.rank),
+        ring(rings + (threadIdx.x >> 5) * SM::DEPTH * SM::STAGE), n(p.n), last(min(p.n, end * COLS)),
+        next(step * COLS), passes(tile.id >= 0 ? width / RC : 0), fc(first * COLS) {
+    const int lane = threadIdx.x & 31, row = lane / CHUNKS, c = lane % CHUNKS;
+    const uint32_t row_bytes = (uint32_t)p.rank * sizeof(T);
+    src = reinterpret_cast<const uint8_t *>(b) + (uint64_t)(fc + row) * row_bytes + c * 16;
+    dst = smem_u32(ring) + row * SM::ROW + c * 16;
+    rows_step = ROWS * row_bytes;
+    block_step = (uint32_t)next * row_bytes;
+    have = max((int)row_bytes - c * 16, 0);
+  }
+  __device__ __forceinline__ void fetch() {
+    if (fc < last && passes) {
+      const int left = n - fc - (threadIdx.x & 31) / CHUNKS;
+      const bool in = fp * RC * (int)sizeof(T) < (int)have;  // (zeros behind the last rank)
+      const uint8_t *from = in ? src : reinterpret_cast<const uint8_t *>(b);
+      const uint32_t step = in ? rows_step : 0;
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i)
+        if (i * ROWS < left)
+          cp_async16(dst + fslot * SM::STAGE + i * ROWS * SM::ROW, from + (uint64_t)(uint32_t)i * step, in ? 16 : 0);
+      fslot = fslot + 1 == SM::DEPTH ? 0 : fslot + 1;
+      src += RC * sizeof(T);
+      if (++fp == passes) {
+        src += (uint64_t)block_step - (uint32_t)(passes * RC * (int)sizeof(T));
+        fp = 0;
+        fc += next;
+      }
+    }
+    cp_async_commit();
+  }
+  __device__ __forceinline__ void start() {
+    if (WIDE)
+#pragma unroll
+      for (int i = 0; i < SM::DEPTH; ++i) fetch();
+  }
+};
+
+// y = base + B h for few rows of up to RC ranks: a lane an output, two blocks of 32 of
+// the warp together, whose part of base is loaded two blocks ahead.  h: [rows][width].
+template <typename T, int RC, bool WIDE>
+__device__ __forceinline__ void expand_few(const Params &p, const Tile &tile, const int (&rows)[MOST_ROWS],
+                                           const float *h, int width, int first, Copies<T, RC, WIDE> &copies) {
+  using SM = Shared<T, RC>;
+  constexpr int TWO = 2, RB = 16;
+  const int lane = threadIdx.x & 31, last = copies.last;
+  const bool adapted = copies.passes != 0;
+  uint64_t at[FEW];  // this lane's first output of a row
+#pragma unroll
+  for (int i = 0; i < FEW; ++i) at[i] = (uint64_t)rows[i] * p.n + lane;
+  struct Old {
+    float v[TWO][FEW];
+  };
+  auto load_old = [&](Old &o, int c0) {
+    const bool in[TWO] = {p.base && c0 < last && c0 + lane < p.n,
+                          p.base && c0 + copies.next < last && c0 + copies.next + lane < p.n};
+#pragma unroll
+    for (int i = 0; i < FEW; ++i) {
+      if (i >= tile.len) break;
+#pragma unroll
+      for (int u = 0; u < TWO; ++u) o.v[u][i] = in[u] ? p.base[at[i] + c0 + u * copies.next] : 0.f;
+    }
+  };
+  Old next;
+  load_old(next, first);
+  int slot = 0;
+  for (int c0 = first; c0 < last; c0 += TWO * copies.next) {
+    const Old old = next;
+    load_old(next, c0 + TWO * copies.next);
+    float acc[TWO][FEW];
+#pragma unroll
+    for (int u = 0; u < TWO; ++u)
+#pragma unroll
+      for (int i = 0; i < FEW; ++i) acc[u][i] = 0.f;
+    if (adapted) {
+      if (WIDE) {
+        cp_async_wait<SM::DEPTH - TWO>();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int r0 = 0; r0 < RC; r0 += RB) {
+        if (r0 >= p.rank) break;
+        Pairs<T, RB> w[TWO];
+#pragma unroll
+        for (int u = 0; u < TWO; ++u) {
+          if (WIDE) {
+            const int at = slot + u >= SM::DEPTH ? slot + u - SM::DEPTH : slot + u;
+            w[u].load(reinterpret_cast<const T *>(copies.ring + at * SM::STAGE + lane * SM::ROW) + r0, RB, true);
+          } else {
+            w[u].load(copies.b + (uint64_t)min(c0 + u * copies.next + lane, p.n - 1) * p.rank + r0, p.rank - r0,
+                      false);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < FEW; ++i) {
+          if (i >= tile.len) break;
+#pragma unroll
+          for (int s = 0; s < RB / 2; ++s) {
+            const float2 v = *reinterpret_cast<const float2 *>(h + i * width + r0 + 2 * s);
+#pragma unroll
+            for (int u = 0; u < TWO; ++u) {
+              const float2 f = w[u].pair(s);
+              acc[u][i] = fmaf(f.y, v.y, fmaf(f.x, v.x, acc[u][i]));
+            }
+          }
+        }
+      }
+      if (WIDE) {
+        __syncwarp();
+        slot = slot + TWO >= SM::DEPTH ? slot + TWO - SM::DEPTH : slot + TWO;
+        copies.fetch();
+        copies.fetch();
+      }
+    }
+    const bool in[TWO] = {c0 + lane < p.n, c0 + copies.next < last && c0 + copies.next + lane < p.n};
+#pragma unroll
+    for (int i = 0; i < FEW; ++i) {
+      if (i >= tile.len) break;
+#pragma unroll
+      for (int u = 0; u < TWO; ++u)
+        if (in[u])
+          p.y[at[i] + c0 + u * copies.next] =
+              !adapted ? old.v[u][i] : p.base ? old.v[u][i] + acc[u][i] : acc[u][i];
+    }
+  }
+  if (WIDE) cp_async_wait<0>();
+}
+
+// y = base + B h for the copies' blocks of 32 outputs, which have been started.  An
+// MMA's four column blocks are interleaved so that a lane ends up with 8
 // neighbouring outputs of a row: column g of block n is output 8 (g / 2) + 2 n +
 // g % 2.
 template <typename T, int RC, bool WIDE>
 __device__ __forceinline__ void expand(const Params &p, const Tile &tile, const int (&rows)[MOST_ROWS],
-                                       const uint4 *hs, int width, uint8_t *ring, int first, int end,
-                                       int step) {
+                                       const uint4 *hs, int width, int first, Copies<T, RC, WIDE> &copies) {
   using SM = Shared<T, RC>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int mts = (tile.len + M - 1) / M;
-  constexpr int PER = RC / 4, STEPS = RC / 8, CHUNKS = RC * sizeof(T) / 16;
-  const int NEXT = step * COLS, last = min(p.n, end * COLS);
-  const T *b = static_cast<const T *>(p.b) + (uint64_t)max(tile.id, 0) * p.n * p.rank;
-  const int passes = tile.id >= 0 ? width / RC : 0, steps = width / 8;
-  ring += (threadIdx.x >> 5) * SM::DEPTH * SM::STAGE;
-  // WIDE: a warp's copies of B (a pass of a block a stage) run DEPTH ahead
-  int fc = first * COLS, fp = 0, fslot = 0, slot = 0;
-  auto fetch = [&]() {
-    if (fc < last && passes) {
-      uint8_t *st = ring + fslot * SM::STAGE;
-      const int have = (p.rank - fp * RC) * (int)sizeof(T);  // bytes of a row in this pass
-#pragma unroll
-      for (int i = 0; i < CHUNKS; ++i) {
-        const int q = i * 32 + lane, row = q / CHUNKS, c = q % CHUNKS;
-        const bool in = c * 16 < have;  // (zeros behind the last rank)
-        if (fc + row < p.n)
-          cp_async16(st + row * SM::ROW + c * 16,
-                     reinterpret_cast<const uint8_t *>(b + (uint64_t)(fc + row) * p.rank + fp * RC) +
-                         (in ? c * 16 : 0), in ? 16 : 0);
-      }
-      fslot = fslot + 1 == SM::DEPTH ? 0 : fslot + 1;
-      if (++fp == passes) fp = 0, fc += NEXT;
-    }
-    cp_async_commit();
-  };
-  if (WIDE)
-#pragma unroll
-    for (int i = 0; i < SM::DEPTH; ++i) fetch();
+  constexpr int PER = RC / 4, STEPS = RC / 8;
+  const int NEXT = copies.next, last = copies.last;
+  const T *b = copies.b;
+  const uint8_t *ring = copies.ring;
+  const int passes = copies.passes, steps = width / 8;
+  int slot = 0;
   // base (after the first pass: y) of lane (g, t)'s outputs c .. c + 7, c = c0 + 8 t,
   // of rows g and g + 8 of a block of rows; loaded one block ahead
   struct Old {
@@ -521,7 +754,7 @@ __device__ __forceinline__ void expand(const Params &p, const Tile &tile, const 
     }
   };
   Old next;
-  int c0 = first * COLS;
+  int c0 = first;
   if (c0 < last) load_old(next, c0, 0, 0);
   for (; c0 < last; c0 += NEXT) {
     const int c = c0 + 8 * t;
@@ -545,7 +778,7 @@ __device__ __forceinline__ void expand(const Params &p, const Tile &tile, const 
         if (WIDE) {
           __syncwarp();
           slot = slot + 1 == SM::DEPTH ? 0 : slot + 1;
-          fetch();
+          copies.fetch();
         }
       }
       const bool add = q || p.base;  // (more than one pass: the sums so far are in y)
@@ -615,26 +848,38 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   Tile tile;
   // (the whole cluster has one tile)
   if (!find_tile(p, blockIdx.x / ctas, plan, rows, blockIdx.x == 0, tile)) return;
+  const bool few = few_rows(p, tile);
+  // B's first copies are under way while h is taken, where shared memory holds both
+  const int first = cta * WARPS + warp;
+  Copies<T, RC, WIDE> copies(p, tile, width,
+                             smem + h_bytes(p.tile_rows, width) + (p.early ? part_bytes(p.tile_rows, width) : 0),
+                             first, (p.n + COLS - 1) / COLS, ctas * WARPS);
+  if (p.early) copies.start();
   if (tile.id >= 0) {
     const int groups = (p.k + 31) / 32, per = (groups + ctas - 1) / ctas;
     const int g0 = min(groups, cta * per), g1 = min(groups, g0 + per);
-    shrink<T, RC>(p, tile, rows, g0, g1, width, part);
+    if (few) shrink_few<T>(p, tile, rows, g0, g1, width, part);
+    else shrink<T, RC>(p, tile, rows, g0, g1, width, part);
     cluster.sync();
     const float scale = p.scales ? p.scales[tile.id] : 1.f;
-    h_operands<RC>(hs, (tile.len + M - 1) / M, width, [&](int row, int r) {
+    auto sum = [&](int row, int r) {
       float2 s = make_float2(0.f, 0.f);
       if (row >= tile.len) return s;
+#pragma unroll 4
       for (int c = 0; c < ctas; ++c) {  // in order
         const float2 u = *reinterpret_cast<const float2 *>(
             cluster.map_shared_rank(part + row * (width + 4) + r, c));
         s.x += u.x, s.y += u.y;
       }
       return make_float2(s.x * scale, s.y * scale);
-    });
+    };
+    if (few) h_values(reinterpret_cast<float *>(hs), tile.len, width, sum);
+    else h_operands<RC>(hs, (tile.len + M - 1) / M, width, sum);
     cluster.sync();  // h is complete, and no CTA reads another's part any more
   }
-  expand<T, RC, WIDE>(p, tile, rows, hs, width, smem + h_bytes(p.tile_rows, width), cta * WARPS + warp,
-                      (p.n + COLS - 1) / COLS, ctas * WARPS);
+  if (!p.early) copies.start();
+  if (few) expand_few<T, RC, WIDE>(p, tile, rows, reinterpret_cast<float *>(hs), width, first * COLS, copies);
+  else expand<T, RC, WIDE>(p, tile, rows, hs, width, first * COLS, copies);
 }
 
 // The two products apart, for grouped rows: CTA (slice of k, tile), and CTA
@@ -653,7 +898,8 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   if (!find_tile(p, blockIdx.x / p.splits, plan, rows, false, tile) || tile.id < 0) return;
   const int groups = (p.k + 31) / 32, per = (groups + p.splits - 1) / p.splits;
   const int g0 = min(groups, split * per), g1 = min(groups, g0 + per);
-  shrink<T, RC>(p, tile, rows, g0, g1, width, part);
+  if (few_rows(p, tile)) shrink_few<T>(p, tile, rows, g0, g1, width, part);
+  else shrink<T, RC>(p, tile, rows, g0, g1, width, part);
   const float scale = p.scales ? p.scales[tile.id] : 1.f;
   float *h = p.h + ((uint64_t)split * p.m + tile.start) * width;
   for (int i = threadIdx.x; i < tile.len * width; i += 32 * WARPS)
@@ -673,8 +919,9 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
   Tile tile;
   const int slice = blockIdx.x % slices;
   if (!find_tile(p, blockIdx.x / slices, plan, rows, false, tile)) return;
+  const bool few = few_rows(p, tile);
   if (tile.id >= 0) {
-    h_operands<RC>(hs, (tile.len + M - 1) / M, width, [&](int row, int r) {
+    auto sum = [&](int row, int r) {
       float2 s = make_float2(0.f, 0.f);
       if (row >= tile.len) return s;
       const float *at = p.h + (uint64_t)(tile.start + row) * width + r;
@@ -683,12 +930,18 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
         s.x += u.x, s.y += u.y;
       }
       return s;
-    });
+    };
+    if (few) h_values(reinterpret_cast<float *>(hs), tile.len, width, sum);
+    else h_operands<RC>(hs, (tile.len + M - 1) / M, width, sum);
     __syncthreads();
   }
   const int blocks = (p.n + COLS - 1) / COLS, per = (blocks + slices - 1) / slices;
-  expand<T, RC, WIDE>(p, tile, rows, hs, width, smem + h_bytes(p.tile_rows, width), slice * per + warp,
-                      min(blocks, (slice + 1) * per), WARPS);
+  const int first = slice * per + warp;
+  Copies<T, RC, WIDE> copies(p, tile, width, smem + h_bytes(p.tile_rows, width), first,
+                             min(blocks, (slice + 1) * per), WARPS);
+  copies.start();
+  if (few) expand_few<T, RC, WIDE>(p, tile, rows, reinterpret_cast<float *>(hs), width, first * COLS, copies);
+  else expand<T, RC, WIDE>(p, tile, rows, hs, width, first * COLS, copies);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -788,8 +1041,11 @@ cudaError_t launch_rc(const Params &p, unsigned tiles, int sms, cudaStream_t str
   cudaError_t e;
   if (p.m <= INLINE_ROWS) {
     if ((e = opt_in(mgb_adapter_kernel<T, RC, WIDE>, opted[0])) != cudaSuccess) return e;
+    Params q = p;
+    const uint32_t most = (sizeof(T) == 4 ? 216 : 108) * 1024;  // of one CTA an SM, of two
+    q.early = h + part + ring <= most;
     return launch_chained(mgb_adapter_kernel<T, RC, WIDE>, tiles * p.splits, 32 * WARPS,
-                          h + (part > ring ? part : ring), p.splits, stream, p);
+                          h + (q.early ? part + ring : part > ring ? part : ring), p.splits, stream, q);
   }
   if ((e = opt_in(mgb_adapter_h_kernel<T, RC>, opted[1])) != cudaSuccess) return e;
   if ((e = opt_in(mgb_adapter_y_kernel<T, RC, WIDE>, opted[2])) != cudaSuccess) return e;
