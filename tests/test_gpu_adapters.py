@@ -276,3 +276,58 @@ def test_other_stream_and_graph(torch_cuda):
         torch.cuda.synchronize()
         assert torch.equal(graphs[1][2], want)
         assert torch.equal(graphs[0][2], _call(torch, a, b, scales, "f16", ids, x * 2, base))
+
+
+@pytest.mark.parametrize("count,m", [(5000, 40), (5000, 600), (3, 5000), (4095, 4500), (9000, 4500)])
+def test_more_adapters_and_rows_than_the_sort_holds(torch_cuda, count, m):
+    """Adapters whose ids share a bucket of the sort, and more rows than it keeps."""
+    torch = torch_cuda
+    k, n, rank = 40, 36, 4
+    a, b, scales, x, base = _inputs(torch, m, k, n, rank, count, "f16")
+    g = torch.Generator().manual_seed(4)
+    ids = torch.randint(-1, count, (m,), generator=g)
+    ids[::7] = 1  # one bucket for 1, 4096 and 8191 where there are that many
+    ids[1::7] = min(4096, count - 1)
+    ids[2::7] = min(8191, count - 1)
+    want, mag = _expected(a, b, scales, ids.float(), x, base)
+    dev = [t.cuda() for t in (a, b, scales, ids.float(), x, base)]
+    y = _call(torch, *dev[:3], "f16", *dev[3:])
+    _check(y, want, mag, base, k, rank)
+    assert torch.equal(_call(torch, *dev[:3], "f16", *dev[3:]), y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m", [1, 4, 5, 40, 200])
+@pytest.mark.parametrize("rank", [64, 65, 130, 256])
+def test_large_ranks_in_place(torch_cuda, dtype, m, rank):
+    """Ranks of one pass and of several, which add up in y, where base is y."""
+    torch = torch_cuda
+    k, n, count = 136, 72, 2
+    a, b, scales, x, base = _inputs(torch, m, k, n, rank, count, dtype)
+    ids = (torch.arange(m) % 3 - 1).float() if m > 1 else torch.ones(1)
+    want, mag = _expected(a, b, scales, ids, x, base)
+    dev = [t.cuda() for t in (a, b, scales, ids, x, base)]
+    y = _call(torch, *dev[:3], dtype, *dev[3:5], dev[5], y=dev[5])
+    _check(y, want, mag, base, k, rank)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [1, 3, 8, 16, 24, 40, 64])
+@pytest.mark.parametrize("k,n", [(1, 1), (3, 31), (4, 33), (1032, 100), (2200, 72)])
+def test_tiles_on_both_sides_of_a_few_rows(torch_cuda, dtype, rank, k, n):
+    """One to six rows of an adapter in one call; lengths of one and odd ones."""
+    torch = torch_cuda
+    count = 6
+    ids = torch.tensor([a for a in range(count) for _ in range(a + 1)] + [-1]).float()
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(rank))]
+    m = len(ids)
+    a, b, scales, x, base = _inputs(torch, m, k, n, rank, count, dtype)
+    want, mag = _expected(a, b, scales, ids, x, base)
+    dev = [t.cuda() for t in (a, b, scales, ids, x, base)]
+    _check(_call(torch, *dev[:3], dtype, *dev[3:]), want, mag, base, k, rank)
+    # infinities of a row's own adapter reach that row alone
+    x[2, 0] = float("inf")
+    got = _call(torch, *dev[:3], dtype, dev[3], x.cuda(), dev[5]).cpu()
+    rest = torch.arange(m) != 2
+    _check(got[rest].cuda(), want[rest], mag[rest], base[rest], k, rank)
+    assert ids[2] < 0 or not bool(got[2].isfinite().any())

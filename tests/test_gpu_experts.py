@@ -322,3 +322,56 @@ def test_rows_behind_the_last_and_streams(torch_cuda, oracle):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(gy, layer.run(x * 0.5, ids.flip(0).contiguous(), weights))
+
+
+def test_the_largest_plan(torch_cuda, oracle):
+    """256 tokens, 32 slots each, 1,024 experts."""
+    torch = torch_cuda
+    layer = Layer(torch, oracle, mgb.Q8_0, mgb.Q4_0, 1024, 64, 32)
+    m, top_k = 256, 32
+    ids, weights = _choices(torch, m, 1024, top_k)
+    x = _x(torch, m, 64)
+    y = layer.run(x, ids.cuda(), weights.cuda())
+    some = torch.arange(0, m, 37)
+    layer.check(y[some.cuda()], *layer.expected(x[some.cuda()], ids[some], weights[some]))
+    # all of them on one expert
+    ids = torch.full((m, top_k), 1023.0)
+    y = layer.run(x, ids.cuda(), weights.cuda())
+    layer.check(y[some.cuda()], *layer.expected(x[some.cuda()], ids[some], weights[some]))
+    assert mgb.take_device_error(0) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,experts,top_k", [(9, 8, 2), (20, 5, 1), (33, 16, 2), (40, 2, 2), (24, 24, 4)])
+def test_passes_of_8_and_of_16(torch_cuda, oracle, fmt, m, experts, top_k):
+    """Few and many tokens an expert, on both sides of the passes' sizes."""
+    torch = torch_cuda
+    layer = Layer(torch, oracle, fmt, fmt, experts, 256, 512)
+    ids, weights = _choices(torch, m, experts, top_k)
+    ids[: m // 2, 0] = 1  # one expert has more than most
+    x = _x(torch, m, 256)
+    layer.check(layer.run(x, ids.cuda(), weights.cuda()), *layer.expected(x, ids, weights))
+    assert mgb.take_device_error(0) == 0
+
+
+@pytest.mark.parametrize("experts", [1, 2, 7, 8, 9, 31, 32, 33, 64])
+@pytest.mark.parametrize("hidden", [1024, 1056, 4096])
+def test_routing_by_several_warps(torch_cuda, experts, hidden):
+    """Few experts, whose logits several warps share."""
+    torch = torch_cuda
+    m, top_k = 3, min(2, experts)
+    g = torch.Generator().manual_seed(experts)
+    router = torch.randn(experts, hidden, generator=g)
+    x = torch.randn(m, hidden, generator=g)
+    z = x.double() @ router.double().T
+    ids, weights = torch.empty(m, top_k, device="cuda"), torch.empty(m, top_k, device="cuda")
+    r, xd = router.cuda(), x.cuda()  # (kept until the call is done)
+    mgb.moe_route(r.data_ptr(), experts, hidden, xd.data_ptr(), m, top_k, False,
+                  ids.data_ptr(), weights.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    best = torch.topk(z, top_k)
+    assert torch.equal(ids.cpu().long(), best.indices)
+    # a logit's f32 chains: at most 2^-20 of the root of the sum of its squares
+    off = 2.0 ** -20 * (x.norm(dim=1) * router.norm(dim=1).max()).max().double()
+    want = torch.softmax(z, 1).gather(1, best.indices)
+    assert bool(((weights.cpu().double() - want).abs() <= 2 * off * want + 1e-7).all())

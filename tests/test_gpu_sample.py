@@ -311,3 +311,39 @@ def test_streams_and_graph(torch_cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert (ids.cpu().numpy() == _call(torch, z, top_p=torch.full((6,), 0.9), uniform=1 - u)[0]).all()
+
+
+@pytest.mark.parametrize("vocab", [4096, 4099, 70001, 131001])
+def test_batches_that_fill_the_device(torch_cuda, vocab):
+    """More rows than half the SMs: masks, ties, infinities and settings of all kinds
+    in one call, on rows that are not 16-byte aligned too."""
+    torch = torch_cuda
+    rows = 160
+    ld = vocab + 1 if vocab % 2 else vocab + 4
+    z, u = _rows(torch, rows, ld, seed=8)
+    at = torch.arange(rows)
+    z[at % 5 == 1] = (z[at % 5 == 1] * 2).round() / 2
+    z[at % 10 == 2, vocab // 3:] = -INF
+    z[at % 10 == 7] = torch.finfo(torch.float32).min
+    z[7, 3] = 1.0
+    z[12] = -INF
+    z[17, ::3] = INF
+    z[22] = 0.25
+    z[27, 1::2] = float("nan")
+    z[32, 5:] = -INF
+    pick = lambda *v: torch.tensor(v, dtype=torch.float32)[at % len(v)]  # noqa: E731
+    _check(torch, z, temperature=pick(1.0, 0.7, 0.0, 2.5, 1.0, 1.0, 0.05),
+           top_k=pick(0, 50, 0, 1, 700, 0, 200, 256, 257, 0, 1500), top_p=pick(1.0, 0.95, 0.5),
+           min_p=pick(0.0, 0.0, 0.0, 0.1), uniform=u, vocab=vocab)
+
+
+def test_broad_rows(torch_cuda):
+    """High temperatures: every token within a few histogram bins; and the nucleus of
+    nearly equal logits."""
+    torch = torch_cuda
+    for rows, vocab in ((3, 20000), (80, 20000)):
+        z, u = _rows(torch, rows, vocab, seed=6)
+        for t, p in ((50.0, 0.4), (3e4, 0.9), (1e9, 0.7)):
+            _check(torch, z, temperature=torch.full((rows,), t), top_p=torch.full((rows,), p), uniform=u)
+        _check(torch, 1.0 + z * 2.0 ** -20, top_p=torch.full((rows,), 0.3), uniform=u)
+        _check(torch, z * 1e30, top_p=torch.full((rows,), 0.3), top_k=torch.full((rows,), 900.0), uniform=u)
