@@ -7,16 +7,26 @@
 // is kept is described by a key tau and how many tokens of key tau (the lowest
 // indices) stay: no sort of the vocabulary is needed, only the search for tau.
 //
-// A row is read once: a cluster of CTAs holds it in shared memory (a few CTAs an
-// SM, so that one row's loads overlap another's arithmetic), and the CTAs agree
-// on one number after another through distributed shared memory.
-//  - Small top_k: the top_k-th largest of a CTA's 256 threads' own largest logits
-//    is a bound that at least top_k of its tokens reach and few others do; the
-//    first CTA sorts the tokens that reach their CTA's and does the rest: one
-//    cluster barrier a row.
-//  - Otherwise tau is searched by histograms of counts (top-k) or of mass (top-p)
-//    over ever smaller key ranges: first by distance to the largest logit, where
-//    tokens spread evenly over the bins, then by key.
+// A row is held by a cluster, whose CTAs agree on one number after another through
+// distributed shared memory.  Few rows: up to eight CTAs of 256 threads a row, each
+// its part in shared memory.  Rows that fill the SMs by themselves: two CTAs of 512
+// threads a row, which read it again from L2; what a batch costs then is the
+// instructions a token takes, and one CTA a row would leave the SMs of greedy rows
+// idle beside those of broad ones (256 rows of 128,256, every row its own settings:
+// 320 us with one, 204 us with two; all rows top-k 50: 52 us and 74 us).
+//  - Small top_k: the top_k-th largest of the threads' own largest logits is a bound
+//    that at least top_k of a CTA's tokens reach and few others do.  One from the
+//    first quarter of the CTA's part bounds the rest as it is read; the first CTA
+//    sorts the tokens that reach all bounds and does what is left.
+//  - Otherwise the border is searched by histograms of counts (top-k) or of mass
+//    (top-p) over the distance to the largest logit, where tokens spread evenly over
+//    the bins: of 1/16, and if that holds too many tokens of 1/16384; the first CTA
+//    sorts the border bin's.  Where even that is too much (equal or nearly equal
+//    logits), by ever smaller ranges of keys.
+// Measured, 256 rows of 128,256 (131 MB; 20 us at the copy's rate): greedy 31 us,
+// no cuts 134 us (a weight costs some 45 instructions), top-k 1,000 151 us, top-p 0.95
+// 364 us (two histograms, two lists, the sum).  One row of 32,000, top-k 50 and
+// top-p: 15 us, a chain of dependent steps.
 //
 // Mass.  A token's weight is 2^((logit - max) log2(e) / T) as a 64-bit integer
 // in units of 2^-43: integer sums are the same in every order, so atomics and
