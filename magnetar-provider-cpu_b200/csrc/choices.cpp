@@ -51,13 +51,13 @@ mgb_status check_adapters(const mgb_adapters *ad, uint64_t m) {
 }
 
 mgb_status check_adapters_call(const mgb_adapters *ad, const float *ids, const float *x, uint64_t m,
-                               const float *base, const float *y) {
+                               const float *base, const float *y, const uint32_t *bad) {
   mgb_status s = check_adapters(ad, m);
   if (s != MGB_OK || !m) return s;
   if (!ad->a || !ad->b || !ids || !x || !y) return fail(MGB_INVALID_ARGUMENT, "null device pointer");
   const uint64_t e = element_bytes(ad->dtype);
   if (!aligned(ad->a, e) || !aligned(ad->b, e) || !aligned(ad->scales, 4) || !aligned(ids, 4) ||
-      !aligned(x, 4) || !aligned(base, 4) || !aligned(y, 4))
+      !aligned(x, 4) || !aligned(base, 4) || !aligned(y, 4) || !aligned(bad, 4))
     return fail(MGB_INVALID_ARGUMENT, "a device pointer is not aligned to its element size");
   return MGB_OK;
 }
@@ -91,7 +91,7 @@ mgb_status check_experts(const mgb_experts *ex, uint64_t m, uint64_t top_k) {
 
 mgb_status check_experts_call(const mgb_experts *ex, const float *x, uint64_t m, const float *ids,
                               const float *weights, uint64_t top_k, const float *addend,
-                              const float *y) {
+                              const float *y, const uint32_t *bad) {
   mgb_status s = check_experts(ex, m, top_k);
   if (s != MGB_OK || !m) return s;
   if (!ex->gate || !ex->up || !ex->down || !x || !ids || !weights || !y)
@@ -99,7 +99,8 @@ mgb_status check_experts_call(const mgb_experts *ex, const float *x, uint64_t m,
   if (!aligned(ex->gate, 16) || !aligned(ex->up, 16) || !aligned(ex->down, 16))
     return fail(MGB_INVALID_ARGUMENT, "packed expert pointers must be 16-byte aligned");
   if (!aligned(x, 16)) return fail(MGB_INVALID_ARGUMENT, "activation pointer is not 16-byte aligned");
-  if (!aligned(ids, 4) || !aligned(weights, 4) || !aligned(addend, 4) || !aligned(y, 4))
+  if (!aligned(ids, 4) || !aligned(weights, 4) || !aligned(addend, 4) || !aligned(y, 4) ||
+      !aligned(bad, 4))
     return fail(MGB_INVALID_ARGUMENT, "a device pointer is not aligned to its element size");
   return MGB_OK;
 }
@@ -145,7 +146,7 @@ uint64_t mgb_adapters_workspace_bytes(const mgb_adapters *adapters, uint64_t m) 
 mgb_status mgb_adapters_add(const mgb_adapters *adapters, const float *ids, const float *x,
                             uint64_t m, const float *base, float *y, uint32_t *bad,
                             void *workspace, uint64_t workspace_bytes, void *stream) {
-  mgb_status s = check_adapters_call(adapters, ids, x, m, base, y);
+  mgb_status s = check_adapters_call(adapters, ids, x, m, base, y, bad);
   if (s == MGB_OK) s = check_workspace(workspace, workspace_bytes, adapters_scratch_bytes(*adapters, m));
   if (s != MGB_OK) return s;
   cudaError_t e = launch_adapters(*adapters, ids, x, m, base, y, bad, workspace,
@@ -165,7 +166,7 @@ mgb_status mgb_qmatmul_adapters(int32_t format, const void *w, uint64_t n, uint6
                                 uint64_t addend_len, const mgb_adapters *adapters,
                                 const float *ids, uint32_t *bad, void *workspace,
                                 uint64_t workspace_bytes, void *stream) {
-  mgb_status s = check_adapters_call(adapters, ids, x, m, y, y);
+  mgb_status s = check_adapters_call(adapters, ids, x, m, y, y, bad);
   if (s != MGB_OK) return s;
   if (adapters->k != k || adapters->n != n)
     return fail(MGB_INVALID_ARGUMENT,
@@ -213,7 +214,7 @@ mgb_status mgb_moe_experts(const mgb_experts *experts, const float *x, uint64_t 
                            const float *ids, const float *weights, uint64_t top_k,
                            const float *addend, float *y, uint32_t *bad, void *workspace,
                            uint64_t workspace_bytes, void *stream) {
-  mgb_status s = check_experts_call(experts, x, m, ids, weights, top_k, addend, y);
+  mgb_status s = check_experts_call(experts, x, m, ids, weights, top_k, addend, y, bad);
   if (s == MGB_OK)
     s = check_workspace(workspace, workspace_bytes, moe_experts_scratch_bytes(*experts, m, top_k));
   if (s != MGB_OK) return s;
@@ -235,7 +236,7 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
                  round16(moe_experts_scratch_bytes(*experts, m, top_k));
   if (!ids) ids = reinterpret_cast<float *>(own);
   if (!weights) weights = reinterpret_cast<float *>(own + round16(m * top_k * 4));
-  s = check_experts_call(experts, x, m, ids, weights, top_k, addend, y);
+  s = check_experts_call(experts, x, m, ids, weights, top_k, addend, y, nullptr);
   if (s != MGB_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_moe_route(router, experts->experts, experts->hidden, x, m, top_k,

@@ -436,8 +436,9 @@ cudaError_t launch_moe_experts(const mgb_experts &ex, const float *x, uint64_t m
   const Parts gu{a.out, a.place, a.share, 2 * (int)ceil_div(ffn, moe::TILE),
                  (int)ceil_div(hidden, moe::stage_cols(ex.gate_up_format)), 2 * ffn};
   const uint32_t h_smem = (uint32_t)h_runs(ffn) * RUN * 4;
-  if (h_smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(mgb_moe_h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)h_smem);
+  if (h_smem > 40 * 1024) {  // (the widest rows' always: another thread's call may be between)
+    e = cudaFuncSetAttribute(mgb_moe_h_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             h_runs(MGB_MOE_MAX_WIDTH) * RUN * 4);
     if (e != cudaSuccess) return e;
   }
   e = launch_chained(mgb_moe_h_kernel, dim3((unsigned)slots * H_CTAS), dim3(H_THREADS), h_smem, stream, gu,

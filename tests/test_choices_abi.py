@@ -176,3 +176,13 @@ def test_empty_calls_do_nothing():
     assert lib.mgb_moe_experts(_experts(), None, 0, None, None, 2, None, None, None, None, 0,
                                None) == mgb.OK
     assert lib.mgb_moe_route(None, 8, 64, None, 0, 2, 1, 1.0, FAKE, FAKE, None, 0, None) == mgb.OK
+
+
+def test_a_misaligned_report_is_refused():
+    ad, ex = _adapters(), _experts()
+    assert mgb.lib().mgb_adapters_add(ad, FAKE, FAKE, 1, None, FAKE, FAKE + 2, FAKE, BIG, None) == \
+        mgb.INVALID_ARGUMENT
+    assert "aligned" in mgb.last_error()
+    assert mgb.lib().mgb_moe_experts(ex, FAKE, 1, FAKE, FAKE, 2, None, FAKE, FAKE + 2, FAKE, BIG, None) == \
+        mgb.INVALID_ARGUMENT
+    assert "aligned" in mgb.last_error()

@@ -154,3 +154,43 @@ def test_decode_steps(torch_cuda, oracle, m):
             for got, w in zip(state.results(), want):
                 assert torch.equal(got, w)
     assert mgb.take_device_error(0) == 0
+
+
+def test_two_host_threads(torch_cuda, oracle):
+    """Two threads drive a batch each on streams of their own."""
+    torch = torch_cuda
+    import threading
+
+    model = Model(torch, oracle)
+    want, sizes = [], (5, 40)
+    for m in sizes:
+        state = State(model, m)
+        for _ in range(12):
+            state.step()
+        torch.cuda.synchronize()
+        want.append(state.results())
+    states, errors = [State(model, m) for m in sizes], []
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(states), timeout=60)
+
+    def drive(state):
+        try:
+            side = torch.cuda.Stream()
+            start.wait()
+            with torch.cuda.stream(side):
+                for _ in range(12):
+                    state.step()
+            side.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=drive, args=(s,)) for s in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for state, results in zip(states, want):
+        for got, w in zip(state.results(), results):
+            assert torch.equal(got, w)
+    assert mgb.take_device_error(0) == 0

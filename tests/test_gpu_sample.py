@@ -347,3 +347,14 @@ def test_broad_rows(torch_cuda):
             _check(torch, z, temperature=torch.full((rows,), t), top_p=torch.full((rows,), p), uniform=u)
         _check(torch, 1.0 + z * 2.0 ** -20, top_p=torch.full((rows,), 0.3), uniform=u)
         _check(torch, z * 1e30, top_p=torch.full((rows,), 0.3), top_k=torch.full((rows,), 900.0), uniform=u)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 393216), (1, 393217), (3, (1 << 20) - 3), (76, 300001)])
+def test_vocabularies_past_the_shared_memory(torch_cuda, rows, vocab):
+    """The largest rows that are staged, and those that are read again; parts of a row
+    above 65,000 tokens."""
+    torch = torch_cuda
+    z, u = _rows(torch, rows, vocab, seed=3)
+    at = torch.arange(rows)
+    _check(torch, z, uniform=u, top_p=torch.tensor([0.9, 1.0, 0.3])[at % 3],
+           top_k=torch.tensor([0.0, 60.0, 5000.0, 0.0])[at % 4])
