@@ -19,7 +19,7 @@
 // chain of the plan, A, the exchange and B; 64 rows of some 40 adapters, n = 14,336,
 // 18.2 us (4.7), of which B takes 5 to 7 us at nine warps an SM (with the tensor
 // cores' tiles 29.1 us, at 300 instructions a block of 32 outputs); 2,048 rows of rank
-// 64 137 us (42): grouping 12, h 20, y 100, which waits for base a block ahead and for
+// 64 132 us (42): grouping 6, h 20, y 100, which waits for base a block ahead and for
 // the tensor cores in about equal parts (two blocks ahead, or three bf16 terms on
 // m16n8k16 instead of two tf32 ones: the same time).
 //
@@ -145,78 +145,117 @@ __device__ __forceinline__ int plan_small(const Params &p, SmallPlan &s, bool re
   return all;
 }
 
-__device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {  // exclusive
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int s = v;
+__device__ __forceinline__ int warp_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
   }
+  return v;
+}
+// Exclusive sum over 1,024 threads; warp_sums [32].
+__device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int s = warp_scan(v);
   __syncthreads();
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
-  }
-  return before + s - v;
+  const int sums = warp_scan(warp_sums[lane]);
+  total = __shfl_sync(0xffffffffu, sums, 31);
+  const int before = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0));
+  return (warp ? before : 0) + s - v;
 }
 
 // One CTA: rows by bucket (the adapter, modulo 4,095; the last bucket holds the
-// rows without one), then tiles of up to tile_rows neighbours of one adapter.
-// Up to CACHED rows the ids and the order stay in shared memory.
+// rows without one), in row order within a bucket (where a row lands decides in which
+// order its sums are taken), then tiles of up to tile_rows neighbours of one adapter.
+// Up to CACHED rows in shared memory, by two stable passes of 6 bits: every warp
+// counts its stretch of the rows and then places it, its digits' places known from a
+// scan over (digit, warp).  (2,048 rows took 12 us with the warps placing their rows
+// one after the other, which more than CACHED rows still do.)
 constexpr int CACHED = 4096;
 __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) {
-  __shared__ int at[BUCKETS];
-  __shared__ int ids[CACHED];      // by row, then by sorted position
-  __shared__ uint16_t sorted[CACHED];
+  __shared__ int ids[CACHED];                      // by row; not CACHED: the buckets
+  __shared__ uint16_t half[CACHED], sorted[CACHED];
+  __shared__ int counts[64 * 32];                  // [digit][warp]
   __shared__ int sums[32], s_carry[2];
+  static_assert(BUCKETS <= CACHED && BUCKETS == 64 * 64, "two digits");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_wait();
   grid_dependents();
   const bool cached = p.m <= CACHED;
-  for (int b = threadIdx.x; b < BUCKETS; b += 1024) at[b] = 0;
-  __syncthreads();
   auto bucket = [&](int id) { return id < 0 ? BUCKETS - 1 : id % (BUCKETS - 1); };
-  for (int r = threadIdx.x; r < p.m; r += 1024) {
-    int id = adapter_of(p.ids[r], p.count);
-    if (id == -2) {
-      if (p.bad) atomicMin(p.bad, (uint32_t)r);
-      id = -1;
-    }
-    if (cached) ids[r] = id;
-    atomicAdd(&at[bucket(id)], 1);
-  }
-  __syncthreads();
-  {
-    int c[4], v = 0, total;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = at[4 * threadIdx.x + i], v += c[i];
-    int s = block_scan(v, sums, total);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) at[4 * threadIdx.x + i] = s, s += c[i];
-  }
-  __syncthreads();
-  // in row order, a warp after the other: where a row lands decides in which order
-  // its sums are taken
-  for (int r0 = 0; r0 < p.m; r0 += 1024) {
-    const int r = r0 + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int id = r >= p.m ? -1 : cached ? ids[r] : max(adapter_of(p.ids[r], p.count), -1);
-    const int b = r < p.m ? bucket(id) : BUCKETS;
-    const uint32_t same = __match_any_sync(0xffffffffu, b);
-    for (int w = 0; w < 32 && r0 + 32 * w < p.m; ++w) {
-      if (warp == w) {  // (the whole warp)
-        const int i = r < p.m ? at[b] + __popc(same & ((1u << lane) - 1)) : 0;
-        __syncwarp();
-        if (r < p.m) {
-          p.order[i] = r;
-          if (cached) sorted[i] = (uint16_t)r;
-          if ((same >> lane) == 1u) at[b] = i + 1;  // the last of its bucket
-        }
+  if (cached) {
+    for (int r = threadIdx.x; r < p.m; r += 1024) {
+      int id = adapter_of(p.ids[r], p.count);
+      if (id == -2) {
+        if (p.bad) atomicMin(p.bad, (uint32_t)r);
+        id = -1;
       }
+      ids[r] = id;
+    }
+    const int per = ((p.m + 31) / 32 + 31) & ~31, i0 = warp * per, i1 = min(p.m, i0 + per);
+    for (int shift = 0; shift < 12; shift += 6) {
+      const uint16_t *from = shift ? half : nullptr;  // (first: the rows as they are)
+      uint16_t *to = shift ? sorted : half;
+      counts[threadIdx.x] = counts[threadIdx.x + 1024] = 0;
       __syncthreads();
+      for (int place = 0; place < 2; ++place) {
+        for (int i = i0 + lane; i - lane < i1; i += 32) {
+          const int r = i < i1 ? from ? from[i] : i : -1;
+          const int d = r < 0 ? 64 : bucket(ids[r]) >> shift & 63;
+          const uint32_t same = __match_any_sync(0xffffffffu, d);
+          int *at = counts + d * 32 + warp;  // this warp's own
+          if (place && r >= 0) to[*at + __popc(same & ((1u << lane) - 1))] = (uint16_t)r;
+          __syncwarp();
+          if (r >= 0 && (same >> lane) == 1u) *at += __popc(same);  // the last of its digit
+          __syncwarp();
+        }
+        __syncthreads();
+        if (place) break;
+        const int c0 = counts[2 * threadIdx.x], c1 = counts[2 * threadIdx.x + 1];
+        int total;
+        const int s = block_scan(c0 + c1, sums, total);
+        counts[2 * threadIdx.x] = s;
+        counts[2 * threadIdx.x + 1] = s + c0;
+        __syncthreads();
+      }
+    }
+  } else {
+    int *at = ids;
+    for (int b = threadIdx.x; b < BUCKETS; b += 1024) at[b] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < p.m; r += 1024) {
+      const int id = adapter_of(p.ids[r], p.count);
+      if (id == -2 && p.bad) atomicMin(p.bad, (uint32_t)r);
+      atomicAdd(&at[bucket(id)], 1);
+    }
+    __syncthreads();
+    {
+      int c[4], v = 0, total;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = at[4 * threadIdx.x + i], v += c[i];
+      int s = block_scan(v, sums, total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[4 * threadIdx.x + i] = s, s += c[i];
+    }
+    __syncthreads();
+    for (int r0 = 0; r0 < p.m; r0 += 1024) {
+      const int r = r0 + threadIdx.x;
+      const int b = r < p.m ? bucket(adapter_of(p.ids[r], p.count)) : BUCKETS;
+      const uint32_t same = __match_any_sync(0xffffffffu, b);
+      for (int w = 0; w < 32 && r0 + 32 * w < p.m; ++w) {
+        if (warp == w) {  // (the whole warp)
+          const int i = r < p.m ? at[b] + __popc(same & ((1u << lane) - 1)) : 0;
+          __syncwarp();
+          if (r < p.m) {
+            p.order[i] = r;
+            if ((same >> lane) == 1u) at[b] = i + 1;  // the last of its bucket
+          }
+        }
+        __syncthreads();
+      }
     }
   }
   auto id_at = [&](int i) {
@@ -231,34 +270,43 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
     if (i < p.m) {
       id = id_at(i);
       if (i) prev = id_at(i - 1);
+      if (cached) p.order[i] = sorted[i];
     }
     const bool head = i < p.m && id != prev;
     // the run's start: an inclusive maximum of the head positions
     int start = head ? i : -1;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto warp_max = [&](int v) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, start, o);
-      if (lane >= o) start = max(start, u);
-    }
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = max(v, u);
+      }
+      return v;
+    };
+    start = warp_max(start);
     __syncthreads();
     if (lane == 31) sums[warp] = start;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) start = max(start, sums[w]);
-    start = max(start, s_carry[0]);
+    const int warps = warp_max(sums[lane]), before = __shfl_sync(0xffffffffu, warps, max(warp - 1, 0));
+    start = max(max(start, warp ? before : -1), s_carry[0]);
     const bool tile = i < p.m && (i - start) % p.tile_rows == 0;
     int total;
     const int t = s_carry[1] + block_scan(tile, sums, total);
     __syncthreads();
     if (threadIdx.x == 1023) s_carry[0] = start;
     if (threadIdx.x == 0) s_carry[1] += total;
-    if (tile) p.tiles[t] = Tile{i, 0, id};
+    if (tile) {
+      p.tiles[t] = Tile{i, 0, id};
+      if (cached) half[t] = (uint16_t)i;
+    }
     __syncthreads();
   }
   const int n = s_carry[1];
   if (threadIdx.x == 0) *p.ntiles = n;
-  for (int t = threadIdx.x; t < n; t += 1024)
-    p.tiles[t].len = (t + 1 < n ? p.tiles[t + 1].start : p.m) - p.tiles[t].start;
+  for (int t = threadIdx.x; t < n; t += 1024) {
+    if (cached) p.tiles[t].len = (t + 1 < n ? (int)half[t + 1] : p.m) - half[t];
+    else p.tiles[t].len = (t + 1 < n ? p.tiles[t + 1].start : p.m) - p.tiles[t].start;
+  }
 }
 
 // The CTA's tile and its rows (row[i] of lanes' tokens, absent ones repeat the
