@@ -19,7 +19,7 @@
 // chain of the plan, A, the exchange and B; 64 rows of some 40 adapters, n = 14,336,
 // 18.2 us (4.7), of which B takes 5 to 7 us at nine warps an SM (with the tensor
 // cores' tiles 29.1 us, at 300 instructions a block of 32 outputs); 2,048 rows of rank
-// 64 132 us (42): grouping 6, h 20, y 100, which waits for base a block ahead and for
+// 64 107 us (42): grouping 6, h 25, y 76, which waits for base a block ahead and for
 // the tensor cores in about equal parts (two blocks ahead, or three bf16 terms on
 // m16n8k16 instead of two tf32 ones: the same time).
 //
@@ -965,7 +965,6 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   for (int i = threadIdx.x; i < tile.len * width; i += 32 * WARPS)
     h[i] = part[i / width * (width + 4) + i % width] * scale;
 }
-constexpr int Y_BLOCKS = 2;  // blocks of 32 outputs of a warp, with 16 rows a block of rows
 template <typename T, int RC, bool WIDE>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
     mgb_adapter_y_kernel(const Params p, int slices) {
@@ -1111,11 +1110,19 @@ cudaError_t launch_rc(const Params &p, unsigned tiles, int sms, cudaStream_t str
   if ((e = opt_in(mgb_adapter_y_kernel<T, RC, WIDE>, opted[2])) != cudaSuccess) return e;
   e = launch_chained(mgb_adapter_h_kernel<T, RC>, tiles * p.splits, 32 * WARPS, part, 1, stream, p);
   if (e != cudaSuccess) return e;
-  // slices of the outputs: a few blocks a warp, and the SMs covered
-  const uint64_t blocks = ceil_div(p.n, COLS);
-  uint64_t slices = ceil_div(blocks, WARPS * Y_BLOCKS);
-  const uint64_t cover = ceil_div(2 * (uint64_t)sms, tiles), most = ceil_div(blocks, WARPS);
-  if (slices < cover) slices = cover < most ? cover : most;
+  // Slices of the outputs: those with the fewest waves of CTAs (two an SM) times the
+  // blocks of a warp and one more, about what a CTA takes before its first block (the
+  // rows, h as operands); summed for the fewest tiles that the rows can make and for the
+  // middle of that and the most.  2,048 rows, 32 to 41 tiles, 14,336 outputs: 8 slices, a
+  // wave, 76 us; 14 slices 91 us, 28 slices 100 us.
+  const uint64_t blocks = ceil_div(p.n, COLS), full = ceil_div(p.m, p.tile_rows);
+  uint64_t slices = 1, least = ~0ull;
+  for (uint64_t s = 1; s <= 64 && s <= ceil_div(blocks, WARPS); ++s) {
+    const uint64_t waves =
+        ceil_div((tiles + full) / 2 * s, 2 * (uint64_t)sms) + ceil_div(full * s, 2 * (uint64_t)sms);
+    const uint64_t cost = waves * (ceil_div(ceil_div(blocks, s), WARPS) + 1);
+    if (cost <= least) least = cost, slices = s;
+  }
   const uint64_t fit = 0x7FFFFFFFull / tiles;  // CTAs of a grid
   if (slices > fit) slices = fit;
   return launch_chained(mgb_adapter_y_kernel<T, RC, WIDE>, (unsigned)(tiles * slices), 32 * WARPS, h + ring,
