@@ -19,12 +19,13 @@
 // chain of the plan, A, the exchange and B; 64 rows of some 40 adapters, n = 14,336,
 // 18.2 us (4.7), of which B takes 5 to 7 us at nine warps an SM (with the tensor
 // cores' tiles 29.1 us, at 300 instructions a block of 32 outputs); 2,048 rows of rank
-// 64 107 us (42): grouping 6, h 25, y 76, which waits for base a block ahead and for
-// the tensor cores in about equal parts (two blocks ahead, or three bf16 terms on
-// m16n8k16 instead of two tf32 ones: the same time).
+// 64 102 us (42): grouping 6, h 22, y 73, which waits for base a block ahead and for
+// the tensor cores in about equal parts (two blocks ahead: the same time).
 //
 // f32 accuracy from tf32: x and h are held as hi + lo, two tf32 terms (22 bits);
-// f16 and bf16 factors are tf32 numbers as they are, f32 factors are split too.
+// f16 factors are tf32 numbers as they are, f32 factors are split too.  Beside bf16
+// factors x and h are three bf16 terms, of m16n8k16: a quarter fewer MMAs, and no
+// factor is converted (2,048 rows 102 us instead of 107, 4,096 92 instead of 103).
 // The order of a product's K is free, so a lane takes runs of neighbouring
 // values of its row: every load is 16 bytes where the buffers allow it.
 #include <cooperative_groups.h>
@@ -172,15 +173,19 @@ __device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {
 // order its sums are taken), then tiles of up to tile_rows neighbours of one adapter.
 // Up to CACHED rows in shared memory, by two stable passes of 6 bits: every warp
 // counts its stretch of the rows and then places it, its digits' places known from a
-// scan over (digit, warp).  (2,048 rows took 12 us with the warps placing their rows
-// one after the other, which more than CACHED rows still do.)
-constexpr int CACHED = 4096;
+// scan over (digit, warp).  (2,048 rows took 12 us, now 6, with the warps placing their
+// rows one after the other, which more than CACHED rows still do.)
+constexpr int CACHED = 24576;
+// Dynamic shared memory: the ids by row and the rows after each pass; not cached: the
+// buckets.
+inline uint32_t plan_bytes(uint64_t m) { return m <= CACHED ? (uint32_t)(m + 1) / 2 * 16 : BUCKETS * 4; }
 __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) {
-  __shared__ int ids[CACHED];                      // by row; not CACHED: the buckets
-  __shared__ uint16_t half[CACHED], sorted[CACHED];
+  extern __shared__ __align__(16) int ids[];
+  const int even = (p.m + 1) & ~1;
+  uint16_t *half = reinterpret_cast<uint16_t *>(ids + even), *sorted = half + even;
   __shared__ int counts[64 * 32];                  // [digit][warp]
   __shared__ int sums[32], s_carry[2];
-  static_assert(BUCKETS <= CACHED && BUCKETS == 64 * 64, "two digits");
+  static_assert(BUCKETS == 64 * 64 && CACHED < 65536, "two digits; rows in 16 bits");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_wait();
   grid_dependents();
@@ -360,6 +365,29 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&hi)[4],
   }
 }
 
+// bf16 factors: K is 16, and the other operand's f32 values are three bf16 terms
+// (24 bits).
+template <typename T>
+constexpr bool THREE = std::is_same<T, __nv_bfloat16>::value;
+__device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  auto take = [&]() {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+    const uint32_t r = *reinterpret_cast<const uint32_t *>(&b);
+    x -= __uint_as_float(r << 16);
+    y -= __uint_as_float(r & 0xFFFF0000u);
+    return r;
+  };
+  hi = take();
+  mid = take();
+  lo = take();
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ float as_f32(float v) { return v; }
 __device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -439,7 +467,7 @@ __device__ __forceinline__ void cp_async_wait() {
 
 // RC: ranks of a pass (a lane of the second product: RC / 4 neighbours, K of
 // RC / 8 MMAs).  Shared memory: h as MMA operands (hi and lo, [rows / 16][ranks /
-// 8][lane][4]), then in turn this CTA's part of h ([rows][ranks + 4]) and, where
+// 8][lane][4], or three terms of 16 ranks), then in turn this CTA's part of h ([rows][ranks + 4]) and, where
 // the buffers allow 16-byte copies (WIDE), a ring of B's rows for every warp.
 template <typename T, int RC>
 struct Shared {
@@ -450,7 +478,10 @@ struct Shared {
   static constexpr uint32_t RING = WARPS * DEPTH * STAGE;
 };
 __host__ __device__ inline int h_width(int rank, int rc) { return (rank + rc - 1) / rc * rc; }
-__host__ __device__ inline uint32_t h_bytes(int tile_rows, int width) { return tile_rows * width * 8; }
+template <typename T>
+__host__ __device__ inline uint32_t h_bytes(int tile_rows, int width) {
+  return tile_rows * width * (THREE<T> ? 6 : 8);
+}
 __host__ __device__ inline uint32_t part_bytes(int tile_rows, int width) {
   return tile_rows * (width + 4) * 4;
 }
@@ -484,17 +515,34 @@ __device__ __forceinline__ void shrink(const Params &p, const Tile &tile, const 
           const int r = r0 + n * 8 + g;
           w[n].load(a + (uint64_t)min(r, p.rank - 1) * p.k + k0, r < p.rank ? left : 0, p.wide_a);
         }
+        if constexpr (THREE<T>) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          uint32_t hi[4], lo[4];
-          split(v0[2 * s], hi[0], lo[0]);
-          split(v1[2 * s], hi[1], lo[1]);
-          split(v0[2 * s + 1], hi[2], lo[2]);
-          split(v1[2 * s + 1], hi[3], lo[3]);
+          for (int s = 0; s < 2; ++s) {
+            uint32_t hi[4], mid[4], lo[4];
+            split3(v0[4 * s], v0[4 * s + 1], hi[0], mid[0], lo[0]);
+            split3(v1[4 * s], v1[4 * s + 1], hi[1], mid[1], lo[1]);
+            split3(v0[4 * s + 2], v0[4 * s + 3], hi[2], mid[2], lo[2]);
+            split3(v1[4 * s + 2], v1[4 * s + 3], hi[3], mid[3], lo[3]);
 #pragma unroll
-          for (int n = 0; n < RC / 8; ++n) {
-            const float2 v = w[n].pair(s);
-            multiply<T>(acc[n], hi, lo, v.x, v.y);
+            for (int n = 0; n < RC / 8; ++n) {
+              mma16816(acc[n], lo, w[n].r[2 * s], w[n].r[2 * s + 1]);
+              mma16816(acc[n], mid, w[n].r[2 * s], w[n].r[2 * s + 1]);
+              mma16816(acc[n], hi, w[n].r[2 * s], w[n].r[2 * s + 1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            uint32_t hi[4], lo[4];
+            split(v0[2 * s], hi[0], lo[0]);
+            split(v1[2 * s], hi[1], lo[1]);
+            split(v0[2 * s + 1], hi[2], lo[2]);
+            split(v1[2 * s + 1], hi[3], lo[3]);
+#pragma unroll
+            for (int n = 0; n < RC / 8; ++n) {
+              const float2 v = w[n].pair(s);
+              multiply<T>(acc[n], hi, lo, v.x, v.y);
+            }
           }
         }
       }
@@ -607,21 +655,34 @@ __device__ __forceinline__ void h_values(float *h, int len, int width, const F &
 }
 
 // h as operands: lane (g, t) of step q RC / 8 + s multiplies ranks q RC + t RC / 4 +
-// 2 s and the next.  sum(row, r): h of the tile's row at ranks r and r + 1.
-template <int RC, typename F>
+// 2 s and the next (THREE: of step q RC / 16 + s, 4 s and the next three).
+// sum(row, r): h of the tile's row at ranks r and r + 1.
+template <typename T, int RC, typename F>
 __device__ __forceinline__ void h_operands(uint4 *hs, int mts, int width, const F &sum) {
-  const int steps = width / 8;
+  constexpr int K = THREE<T> ? 16 : 8;
+  const int steps = width / K;
   for (int i = threadIdx.x; i < mts * steps * 32; i += 32 * WARPS) {
-    const int l = i & 31, step = (i >> 5) % steps, b = (i >> 5) / steps;
-    const int r = step / (RC / 8) * RC + (l & 3) * (RC / 4) + 2 * (step % (RC / 8));
-    const float2 v0 = sum(b * M + (l >> 2), r), v1 = sum(b * M + (l >> 2) + 8, r);
-    uint4 hi, lo;
-    split(v0.x, hi.x, lo.x);
-    split(v1.x, hi.y, lo.y);
-    split(v0.y, hi.z, lo.z);
-    split(v1.y, hi.w, lo.w);
-    hs[(b * steps + step) * 64 + l] = hi;
-    hs[(b * steps + step) * 64 + 32 + l] = lo;
+    const int l = i & 31, step = (i >> 5) % steps, b = (i >> 5) / steps, row = b * M + (l >> 2);
+    const int r = step / (RC / K) * RC + (l & 3) * (RC / 4) + K / 4 * (step % (RC / K));
+    const float2 v0 = sum(row, r), v1 = sum(row + 8, r);
+    if constexpr (THREE<T>) {
+      const float2 v2 = sum(row, r + 2), v3 = sum(row + 8, r + 2);
+      uint4 hi, mid, lo;
+      split3(v0.x, v0.y, hi.x, mid.x, lo.x);
+      split3(v1.x, v1.y, hi.y, mid.y, lo.y);
+      split3(v2.x, v2.y, hi.z, mid.z, lo.z);
+      split3(v3.x, v3.y, hi.w, mid.w, lo.w);
+      uint4 *at = hs + (b * steps + step) * 96 + l;
+      at[0] = hi, at[32] = mid, at[64] = lo;
+    } else {
+      uint4 hi, lo;
+      split(v0.x, hi.x, lo.x);
+      split(v1.x, hi.y, lo.y);
+      split(v0.y, hi.z, lo.z);
+      split(v1.y, hi.w, lo.w);
+      uint4 *at = hs + (b * steps + step) * 64 + l;
+      at[0] = hi, at[32] = lo;
+    }
   }
 }
 
@@ -779,11 +840,11 @@ __device__ __forceinline__ void expand(const Params &p, const Tile &tile, const 
   using SM = Shared<T, RC>;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int mts = (tile.len + M - 1) / M;
-  constexpr int PER = RC / 4, STEPS = RC / 8;
+  constexpr int PER = RC / 4, STEPS = RC / (THREE<T> ? 16 : 8);
   const int NEXT = copies.next, last = copies.last;
   const T *b = copies.b;
   const uint8_t *ring = copies.ring;
-  const int passes = copies.passes, steps = width / 8;
+  const int passes = copies.passes, steps = width / (THREE<T> ? 16 : 8);
   int slot = 0;
   // base (after the first pass: y) of lane (g, t)'s outputs c .. c + 7, c = c0 + 8 t,
   // of rows g and g + 8 of a block of rows; loaded one block ahead
@@ -855,13 +916,24 @@ __device__ __forceinline__ void expand(const Params &p, const Tile &tile, const 
         if (passes)
 #pragma unroll
           for (int s = 0; s < STEPS; ++s) {
-            const uint4 *f = hs + (mt * steps + q * STEPS + s) * 64 + lane;
-            const uint4 h0 = f[0], l0 = f[32];
-            const uint32_t hi[4] = {h0.x, h0.y, h0.z, h0.w}, lo[4] = {l0.x, l0.y, l0.z, l0.w};
+            if constexpr (THREE<T>) {
+              const uint4 *f = hs + (mt * steps + q * STEPS + s) * 96 + lane;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const float2 v = w[n].pair(s);
-              multiply<T>(acc[n], hi, lo, v.x, v.y);
+              for (int term = 2; term >= 0; --term) {
+                const uint4 a = f[32 * term];
+                const uint32_t v[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) mma16816(acc[n], v, w[n].r[2 * s], w[n].r[2 * s + 1]);
+              }
+            } else {
+              const uint4 *f = hs + (mt * steps + q * STEPS + s) * 64 + lane;
+              const uint4 h0 = f[0], l0 = f[32];
+              const uint32_t hi[4] = {h0.x, h0.y, h0.z, h0.w}, lo[4] = {l0.x, l0.y, l0.z, l0.w};
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const float2 v = w[n].pair(s);
+                multiply<T>(acc[n], hi, lo, v.x, v.y);
+              }
             }
           }
 #pragma unroll
@@ -902,7 +974,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   const int cta = (int)cluster.block_rank(), ctas = p.splits, warp = threadIdx.x >> 5;
   const int width = h_width(p.rank, RC);
   uint4 *hs = reinterpret_cast<uint4 *>(smem);
-  float *part = reinterpret_cast<float *>(smem + h_bytes(p.tile_rows, width));
+  float *part = reinterpret_cast<float *>(smem + h_bytes<T>(p.tile_rows, width));
   grid_wait();
   grid_dependents();
   Tile tile;
@@ -912,7 +984,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   // B's first copies are under way while h is taken, where shared memory holds both
   const int first = cta * WARPS + warp;
   Copies<T, RC, WIDE> copies(p, tile, width,
-                             smem + h_bytes(p.tile_rows, width) + (p.early ? part_bytes(p.tile_rows, width) : 0),
+                             smem + h_bytes<T>(p.tile_rows, width) + (p.early ? part_bytes(p.tile_rows, width) : 0),
                              first, (p.n + COLS - 1) / COLS, ctas * WARPS);
   if (p.early) copies.start();
   if (tile.id >= 0) {
@@ -934,7 +1006,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
       return make_float2(s.x * scale, s.y * scale);
     };
     if (few) h_values(reinterpret_cast<float *>(hs), tile.len, width, sum);
-    else h_operands<RC>(hs, (tile.len + M - 1) / M, width, sum);
+    else h_operands<T, RC>(hs, (tile.len + M - 1) / M, width, sum);
     cluster.sync();  // h is complete, and no CTA reads another's part any more
   }
   if (!p.early) copies.start();
@@ -991,12 +1063,12 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
       return s;
     };
     if (few) h_values(reinterpret_cast<float *>(hs), tile.len, width, sum);
-    else h_operands<RC>(hs, (tile.len + M - 1) / M, width, sum);
+    else h_operands<T, RC>(hs, (tile.len + M - 1) / M, width, sum);
     __syncthreads();
   }
   const int blocks = (p.n + COLS - 1) / COLS, per = (blocks + slices - 1) / slices;
   const int first = slice * per + warp;
-  Copies<T, RC, WIDE> copies(p, tile, width, smem + h_bytes(p.tile_rows, width), first,
+  Copies<T, RC, WIDE> copies(p, tile, width, smem + h_bytes<T>(p.tile_rows, width), first,
                              min(blocks, (slice + 1) * per), WARPS);
   copies.start();
   if (few) expand_few<T, RC, WIDE>(p, tile, rows, reinterpret_cast<float *>(hs), width, first * COLS, copies);
@@ -1095,7 +1167,7 @@ template <typename T, int RC, bool WIDE>
 cudaError_t launch_rc(const Params &p, unsigned tiles, int sms, cudaStream_t stream) {
   static std::atomic<uint64_t> opted[3];
   const int width = h_width(p.rank, RC);
-  const uint32_t h = h_bytes(p.tile_rows, width), part = part_bytes(p.tile_rows, width);
+  const uint32_t h = h_bytes<T>(p.tile_rows, width), part = part_bytes(p.tile_rows, width);
   const uint32_t ring = WIDE ? Shared<T, RC>::RING : 0;
   cudaError_t e;
   if (p.m <= INLINE_ROWS) {
@@ -1182,7 +1254,9 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
   p.wide_x = aligned16(x) && ad.k % 4 == 0;
   p.wide_y = aligned16(y) && aligned16(base) && ad.n % 4 == 0;
   if (m > INLINE_ROWS) {
-    e = launch_chained(mgb_adapter_plan_kernel, 1, 1024, 0, 1, stream, p);
+    static std::atomic<uint64_t> opted{0};
+    if ((e = opt_in(mgb_adapter_plan_kernel, opted)) != cudaSuccess) return e;
+    e = launch_chained(mgb_adapter_plan_kernel, 1, 1024, plan_bytes(m), 1, stream, p);
     if (e != cudaSuccess) return e;
   }
   const unsigned tiles = (unsigned)tile_bound(m, ad.count, p.tile_rows);

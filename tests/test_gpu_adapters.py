@@ -278,7 +278,8 @@ def test_other_stream_and_graph(torch_cuda):
         assert torch.equal(graphs[0][2], _call(torch, a, b, scales, "f16", ids, x * 2, base))
 
 
-@pytest.mark.parametrize("count,m", [(5000, 40), (5000, 600), (3, 5000), (4095, 4500), (9000, 4500)])
+@pytest.mark.parametrize("count,m", [(5000, 40), (5000, 600), (3, 5000), (4095, 4500), (9000, 4500),
+                                     (5000, 24576), (5000, 24577), (2, 25001)])
 def test_more_adapters_and_rows_than_the_sort_holds(torch_cuda, count, m):
     """Adapters whose ids share a bucket of the sort, and more rows than it keeps."""
     torch = torch_cuda
