@@ -40,7 +40,6 @@
 #pragma once
 
 #include "common.cuh"
-#include "decode.cuh"
 #include "kernels.h"
 
 namespace mgb {
