@@ -300,20 +300,13 @@ def _sample(s):
     return {"ids": token.float(), "logprob": logprob.float(), "kept": keep.sum(1, dtype=torch.int32)}
 
 
-_module = None
-
-
 def _package():
-    """The package, looked up once: a program imports what it calls before its first pass."""
-    global _module
-    if _module is None:
-        here = str(pathlib.Path(__file__).resolve().parents[1] / "magnetar-provider-cpu_b200")
-        if here not in sys.path:
-            sys.path.insert(0, here)
-        import magnetar_b200
+    here = str(pathlib.Path(__file__).resolve().parents[1] / "magnetar-provider-cpu_b200")
+    if here not in sys.path:
+        sys.path.insert(0, here)
+    import magnetar_b200
 
-        _module = magnetar_b200
-    return _module
+    return magnetar_b200
 
 
 def _own_adapters(s):
