@@ -79,10 +79,11 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
   double *zs = cluster.map_shared_rank(z, 0);
   const float *xr = x + (size_t)token * hidden;
   const bool wide = hidden % 4 == 0 && ((uintptr_t)router & 15) == 0 && ((uintptr_t)x & 15) == 0;
-  // few experts: several warps each, a stretch of the columns a warp
+  // few experts: several warps each, a stretch of the columns a warp (rounded up, so
+  // that the stretches cover every column; the last ones may be short or empty)
   int stretches = 1;
   while (experts * stretches * 2 <= WARPS && hidden >= 1024 * stretches) stretches *= 2;
-  const int columns = (hidden / stretches + 127) & ~127;
+  const int columns = ((hidden + stretches - 1) / stretches + 127) & ~127;
   for (int i = warp; i < experts * stretches; i += WARPS) {
     const int from = min(hidden, i % stretches * columns), to = min(hidden, from + columns);
     const float *r = router + (size_t)(i / stretches) * hidden;

@@ -375,3 +375,32 @@ def test_routing_by_several_warps(torch_cuda, experts, hidden):
     off = 2.0 ** -20 * (x.norm(dim=1) * router.norm(dim=1).max()).max().double()
     want = torch.softmax(z, 1).gather(1, best.indices)
     assert bool(((weights.cpu().double() - want).abs() <= 2 * off * want + 1e-7).all())
+
+
+@pytest.mark.parametrize("experts", [2, 8, 16, 32])
+@pytest.mark.parametrize("hidden", [1025, 1281, 2051, 4100, 4103])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_routing_reads_the_last_columns(torch_cuda, experts, hidden, offset):
+    """Widths that several warps cannot share evenly: the choice hangs on the last
+    column alone, whose terms lie 16 / experts apart while all others add up to less
+    than 0.1.  The router starts `offset` elements past an aligned address.
+
+    A logit is off by at most (hidden / 128 + 8) 2^-24 of the sum of its terms'
+    magnitudes, a weight by twice that and its own rounding."""
+    torch = torch_cuda
+    m, top_k = 3, 2
+    g = torch.Generator().manual_seed(experts + hidden)
+    router = (torch.rand(experts, hidden, generator=g) - 0.5) * (0.1 / hidden)
+    router[:, -1] = torch.randperm(experts, generator=g).float() * (4.0 / experts)
+    x = torch.rand(m, hidden, generator=g)
+    x[:, -1] = torch.tensor([4.0, -4.0, 2.0])
+    z = x.double() @ router.double().T
+    terms = (x.double().abs() @ router.double().abs().T).max()
+    buf = torch.zeros(router.numel() + offset, device="cuda")
+    buf[offset:] = router.flatten().cuda()
+    ids, weights = _route(torch, buf[offset:].view(router.shape), x.cuda(), top_k, False)
+    best = torch.topk(z, top_k)
+    assert torch.equal(ids.long(), best.indices)
+    want = torch.softmax(z, 1).gather(1, best.indices)
+    off = 2 * (hidden / 128 + 8) * 2.0 ** -24 * float(terms) + 2.0 ** -23
+    assert bool(((weights.double() - want).abs() <= off * want).all())
