@@ -397,7 +397,9 @@ typedef struct mgb_adapters {
     uint64_t count, rank, k, n;
     int32_t dtype;       /* MGB_DTYPE_* of a and b */
 } mgb_adapters;
-/* Scratch bytes of mgb_adapters_add for m rows (0 for a descriptor it refuses). */
+/* Scratch bytes of mgb_adapters_add for m rows (0 for a descriptor it refuses).
+ * They never fall as m grows: the workspace of the most rows that a program
+ * expects serves its smaller calls. */
 uint64_t mgb_adapters_workspace_bytes(const mgb_adapters *adapters, uint64_t m);
 /* y[r] = base[r] + scales[a] * (x[r] A_a^T) B_a^T with a = ids[r], for the m
  * rows of x [m, k]; y and base are [m, n], base may be y itself (added in
@@ -412,7 +414,9 @@ mgb_status mgb_adapters_add(const mgb_adapters *adapters, const float *ids, cons
 /* mgb_qmatmul and then mgb_adapters_add on its y: the shared packed projection
  * with every row's adapter beside it.  adapters->k and ->n equal k and n.  A
  * row without an adapter equals mgb_qmatmul's bit for bit.  The workspace
- * serves both in turn (mgb_qmatmul_adapters_workspace_bytes). */
+ * serves both in turn (mgb_qmatmul_adapters_workspace_bytes); what the
+ * adapters need is required, less than the projection prefers only costs it
+ * speed, as in mgb_qmatmul. */
 uint64_t mgb_qmatmul_adapters_workspace_bytes(int32_t format, uint64_t m, uint64_t n, uint64_t k,
                                               const mgb_adapters *adapters);
 mgb_status mgb_qmatmul_adapters(int32_t format, const void *w, uint64_t n, uint64_t k,

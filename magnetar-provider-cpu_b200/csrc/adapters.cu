@@ -1091,6 +1091,13 @@ int tile_rows_of(uint64_t rank) { return rank <= 64 ? 64 : rank <= 128 ? 32 : 16
 
 int pass_ranks(uint64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
+// The most slices of k of a grid.
+constexpr uint64_t MOST_SPLITS = 16;
+uint64_t most_splits(const mgb_adapters &ad) {
+  const uint64_t groups = ceil_div(ceil_div(ad.k, 32), WARPS);
+  return groups < MOST_SPLITS ? groups : MOST_SPLITS;
+}
+
 // Slices of k.  A cluster: as many CTAs as keep all clusters on the SMs at once
 // (two CTAs each), so that 64 rows of 64 adapters do not run in two waves.  The
 // grid: enough for two CTAs an SM, at least a group of 32 a warp.
@@ -1101,15 +1108,32 @@ int k_splits(const mgb_adapters &ad, uint64_t m, int sms) {
     while (s > 1 && tiles * s > 2 * (uint64_t)sms) s /= 2;
     return s;
   }
-  const uint64_t want = ceil_div(2 * (uint64_t)sms, tiles), most = ceil_div(ceil_div(ad.k, 32), WARPS);
-  const uint64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+  const uint64_t want = ceil_div(2 * (uint64_t)sms, tiles), most = most_splits(ad);
+  return (int)(want < most ? want : most);
+}
+
+// The most rows of h that any batch of up to m rows has, over its slices of k.  More
+// rows can have fewer slices and so fewer rows of h; a workspace of the largest batch
+// serves every smaller one all the same.
+uint64_t most_h_rows(const mgb_adapters &ad, uint64_t m, int sms) {
+  const uint64_t tile_rows = tile_rows_of(ad.rank);
+  uint64_t most = m;
+  for (uint64_t s = 2; s <= MOST_SPLITS; ++s) {
+    // s slices or more: ceil(2 sms / tiles) >= s, so up to `tiles` tiles
+    const uint64_t tiles = (2 * (uint64_t)sms - 1) / (s - 1);
+    uint64_t rows = tiles;  // the most that stay within them (tile_bound's inverse)
+    if (ad.count < BUCKETS - 1 && tiles > ad.count && (tiles - ad.count) * tile_rows - 1 > rows)
+      rows = (tiles - ad.count) * tile_rows - 1;
+    if (rows > m) rows = m;
+    if (s <= most_splits(ad) && s * rows > most) most = s * rows;
+  }
+  return most;
 }
 
 // Grouped rows' scratch (up to INLINE_ROWS rows need none of it).
 struct Scratch {
   uint64_t order, tiles, ntiles, h, total;
-  Scratch(const mgb_adapters &ad, uint64_t m, int splits) {
+  Scratch(const mgb_adapters &ad, uint64_t m, int sms) {
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
       const uint64_t r = at;
@@ -1120,7 +1144,7 @@ struct Scratch {
     order = take(planned * 4);
     tiles = take(planned ? tile_bound(m, ad.count, tile_rows_of(ad.rank)) * sizeof(Tile) : 0);
     ntiles = take(4);
-    h = take((uint64_t)splits * planned * h_width((int)ad.rank, pass_ranks(ad.rank)) * 4);
+    h = take((planned ? most_h_rows(ad, m, sms) : 0) * h_width((int)ad.rank, pass_ranks(ad.rank)) * 4);
     total = at;
   }
 };
@@ -1216,7 +1240,7 @@ cudaError_t launch_t(const Params &p, unsigned tiles, int sms, cudaStream_t stre
 }  // namespace
 
 uint64_t adapters_scratch_bytes(const mgb_adapters &ad, uint64_t m) {
-  return m ? Scratch(ad, m, k_splits(ad, m, current_sms())).total : 0;
+  return m ? Scratch(ad, m, current_sms()).total : 0;
 }
 
 cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const float *x, uint64_t m,
@@ -1242,7 +1266,7 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
   p.tile_rows = tile_rows_of(ad.rank);
   const int sms = current_sms();
   p.splits = k_splits(ad, m, sms);
-  const Scratch s(ad, m, p.splits);
+  const Scratch s(ad, m, sms);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   p.order = reinterpret_cast<int32_t *>(ws + s.order);
   p.tiles = reinterpret_cast<Tile *>(ws + s.tiles);

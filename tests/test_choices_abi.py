@@ -186,3 +186,16 @@ def test_a_misaligned_report_is_refused():
     assert mgb.lib().mgb_moe_experts(ex, FAKE, 1, FAKE, FAKE, 2, None, FAKE, FAKE + 2, FAKE, BIG, None) == \
         mgb.INVALID_ARGUMENT
     assert "aligned" in mgb.last_error()
+
+
+@pytest.mark.parametrize("count", [1, 8, 64, 4094, 5000])
+@pytest.mark.parametrize("rank", [16, 64, 100, 256])
+@pytest.mark.parametrize("k", [64, 4096])
+def test_a_larger_batch_never_needs_a_smaller_workspace(count, rank, k):
+    """A workspace sized once for the most rows serves every smaller call."""
+    ad = _adapters(count=count, rank=rank, k=k, n=4096)
+    most = 0
+    for m in list(range(0, 3000)) + list(range(3000, 40000, 7)) + [1 << 20, 1 << 24]:
+        need = mgb.adapters_workspace_bytes(ad, m)
+        assert need >= most, m
+        most = need

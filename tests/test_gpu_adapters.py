@@ -332,3 +332,38 @@ def test_tiles_on_both_sides_of_a_few_rows(torch_cuda, dtype, rank, k, n):
     rest = torch.arange(m) != 2
     _check(got[rest].cuda(), want[rest], mag[rest], base[rest], k, rank)
     assert ids[2] < 0 or not bool(got[2].isfinite().any())
+
+
+@pytest.mark.parametrize("count,rank", [(64, 64), (8, 16), (5000, 16)])
+def test_smaller_batches_take_the_largest_ones_workspace(torch_cuda, count, rank):
+    """A workspace sized once for the most rows serves every smaller call."""
+    torch = torch_cuda
+    k, n, most = 4096, 32, 704
+    fmt = mgb.Q4_K
+    stream = torch.cuda.current_stream().cuda_stream
+    g = torch.Generator(device="cuda").manual_seed(count)
+    a = torch.randn(count, rank, k, generator=g, device="cuda").to(torch.float16) / 64
+    b = torch.randn(count, n, rank, generator=g, device="cuda").to(torch.float16)
+    x = torch.randn(most, k, generator=g, device="cuda")
+    base = torch.randn(most, n, generator=g, device="cuda")
+    ids = (torch.arange(most, device="cuda") % min(count, 7) - 1).float()
+    ad = mgb.adapters(a.data_ptr(), b.data_ptr(), count, rank, k, n, mgb.F16)
+    src = torch.from_numpy(synthetic.packed_weights(fmt, n, k, seed=5)).cuda()
+    w = torch.empty(mgb.packed_bytes(fmt, n, k), dtype=torch.uint8, device="cuda")
+    mgb.repack(fmt, src.data_ptr(), n, k, w.data_ptr(), stream)
+    for call, need in ((mgb.adapters_add, mgb.adapters_workspace_bytes(ad, most)),
+                       (mgb.qmatmul_adapters, mgb.qmatmul_adapters_workspace_bytes(fmt, most, n, k, ad))):
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        for m in (0, 1, 128, 129, 147, 148, 300, 575, 576, 703, most):
+            y = torch.full((most, n), 7.0, device="cuda")
+            if call is mgb.adapters_add:
+                call(ad, ids.data_ptr(), x.data_ptr(), m, y.data_ptr(), base_ptr=base.data_ptr(),
+                     workspace_ptr=ws.data_ptr(), workspace_bytes=need, stream=stream)
+                own = _call(torch, a, b, None, "f16", ids[:m], x[:m], base[:m]) if m else y[:0]
+                assert torch.equal(y[:m], own)
+            else:
+                call(fmt, w.data_ptr(), n, k, x.data_ptr(), m, y.data_ptr(), ad, ids.data_ptr(),
+                     workspace_ptr=ws.data_ptr(), workspace_bytes=need, stream=stream)
+                torch.cuda.synchronize()
+                assert bool(y[:m].isfinite().all())
+            assert bool((y[m:] == 7.0).all())
