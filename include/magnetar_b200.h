@@ -495,8 +495,11 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
  * token as f32 (what mgb_embedding reads; vocab <= MGB_SAMPLE_MAX_VOCAB keeps
  * it exact), -1 for a row with nothing left; logprob [rows], the natural
  * logarithm of its probability among the kept tokens (-inf with nothing left);
- * kept [rows], how many tokens were kept (u32).  Probabilities are held as
- * 64-bit fixed-point numbers, so sums do not depend on their order. */
+ * kept [rows], how many tokens were kept (u32).  Probabilities are summed as
+ * 64-bit fixed-point numbers in units of 2^-43 of the largest (each within
+ * 2^-31 of itself or half a unit), so sums do not depend on their order; a
+ * token below half a unit is never drawn.  A log-probability is its logit's,
+ * less the logarithm of the kept sum. */
 #define MGB_SAMPLE_MAX_VOCAB (1u << 20)
 uint64_t mgb_sample_workspace_bytes(uint64_t rows, uint64_t vocab);
 mgb_status mgb_sample(const float *logits, uint64_t rows, uint64_t vocab, uint64_t ld,

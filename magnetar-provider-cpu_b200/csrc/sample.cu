@@ -31,7 +31,9 @@
 // Mass.  A token's weight is 2^((logit - max) log2(e) / T) as a 64-bit integer
 // in units of 2^-43: integer sums are the same in every order, so atomics and
 // any split of a row give the same token, and a border is only missed where
-// weights round (2^-31 relative).  2^20 tokens of weight 1 stay below 2^63.
+// weights round (2^-31 relative, and half a unit).  2^20 tokens of weight 1 stay below
+// 2^63.  A log-probability takes the kept total from them, and the token's own part from
+// its logit: a weight of few units has few bits.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -681,6 +683,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
   const float uf = p.uniform[r];
   const double u = uf > 0.f ? (double)fminf(uf, 0.99999994f) : 0.0;
   const u64 least = mf > 0.f ? (u64)ceil((double)fminf(mf, 1.f) * (double)(1ull << ONE_BITS)) : 0;
+  auto logprob_of = [&](float v, u64 total) {
+    const double own = v == row.top ? 0.0 : ((double)v - (double)row.top) / (double)temp;
+    return (float)(own - log((double)total * (1.0 / (double)(1ull << ONE_BITS))));
+  };
   auto mass_target = [&](u64 total) {  // of top-p, in [1, total]
     const double want = ceil((double)fmaxf(pf, 0.f) * (double)total);
     const u64 t = want < 1.0 ? 1ull : (u64)want;
@@ -714,7 +720,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
       for (uint32_t j = 0; j < n; ++j)
         if ((uint32_t)sorted[j] >= (uint32_t)mine) upto += s.list[j];
       if (upto > target && upto - w <= target)
-        answer(p, r, (float)index_of(mine), (float)(log((double)w) - log((double)total)), n);
+        answer(p, r, (float)index_of(mine), logprob_of(value_of(key), total), n);
     }
     return;
   }
@@ -828,7 +834,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
     else if (tie_key && key_of(v) == tie_key && ties_before++ < quota) weight = wt;
     sum += weight;
     if (sum > target) {
-      answer(p, r, (float)(row.first + i), (float)(log((double)weight) - log((double)total)), count);
+      answer(p, r, (float)(row.first + i), logprob_of(v, total), count);
       return;
     }
   }

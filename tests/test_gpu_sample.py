@@ -358,3 +358,27 @@ def test_vocabularies_past_the_shared_memory(torch_cuda, rows, vocab):
     at = torch.arange(rows)
     _check(torch, z, uniform=u, top_p=torch.tensor([0.9, 1.0, 0.3])[at % 3],
            top_k=torch.tensor([0.0, 60.0, 5000.0, 0.0])[at % 4])
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 12), (3, 5000), (100, 5000)])
+@pytest.mark.parametrize("top_k", [0, 5])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+def test_the_log_probability_of_an_unlikely_token(torch_cuda, rows, vocab, top_k, temperature):
+    """A uniform of 0 draws the first token, 25 to 28 nats below the largest: its weight is
+    a few units of 2^-43, its log-probability that of its logit.  The kept total is off by
+    at most 2^-44 a token and 2^-31 of itself, the answer besides by its own rounding."""
+    torch = torch_cuda
+    z = torch.full((rows, vocab), -INF if top_k else -60.0 * temperature)
+    nats = torch.linspace(25, 28, rows)
+    z[:, 0] = -nats * temperature
+    z[:, 7] = 0.0
+    z[:, 9] = -1.25
+    z[:, 3] = -40.0 * temperature
+    t = torch.full((rows,), temperature)
+    ids, logprob, _ = _call(torch, z, temperature=t, uniform=torch.zeros(rows),
+                            top_k=torch.full((rows,), float(top_k)))
+    assert (ids == 0).all()
+    zd = z.double() / t.double()[:, None]
+    want = (zd[:, 0] - torch.logsumexp(zd, 1)).numpy()
+    bound = 2.0 ** -24 * np.abs(want) + 2.0 ** -29
+    assert (np.abs(logprob.astype(np.float64) - want) <= bound).all()
