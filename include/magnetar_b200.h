@@ -449,7 +449,8 @@ uint64_t mgb_moe_route_workspace_bytes(uint64_t experts, uint64_t hidden, uint64
  * each token's top_k experts by z descending (equal z: the lower id first) in
  * ids [m, top_k] and their weights in weights [m, top_k]: the softmax of z
  * over all experts, or over the chosen ones when normalize != 0, times
- * `scale`.  z is summed so exactly (f32 products, f64 sums) that a choice
+ * `scale`.  z is an f64 sum of f32 chains of at most 16 products, off by at
+ * most 2^-20 of the sum of its terms' magnitudes at any width, so a choice
  * differs from the real numbers' only where they nearly tie.  A NaN z sorts
  * last. */
 mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden, const float *x,

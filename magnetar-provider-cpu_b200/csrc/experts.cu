@@ -60,8 +60,11 @@ __device__ __forceinline__ double order_value(uint64_t k) {
 }
 
 // One cluster per token: its warps take the experts' logits and, with `pack`,
-// the token's runs; the first CTA's first warp then picks.  A logit is a sum of
-// f32 products in chains of at most hidden / 128 a lane, joined in f64.
+// the token's runs; the first CTA's first warp then picks.  A logit is summed in f32
+// chains of at most CHAIN products, joined in f64, so that its error does not grow with
+// the width: at most 2^-20 of its terms' magnitudes, far less in practice.  (A chain of
+// one takes two conversions and an f64 operation a product.)
+constexpr int CHAIN = 16;
 __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREADS)
     mgb_moe_route_kernel(const float *__restrict__ router, int experts, int hidden,
                          const float *x, int top_k, int normalize, float scale, float *ids,
@@ -87,24 +90,28 @@ __global__ void __cluster_dims__(ROUTE_CTAS, 1, 1) __launch_bounds__(ROUTE_THREA
   for (int i = warp; i < experts * stretches; i += WARPS) {
     const int from = min(hidden, i % stretches * columns), to = min(hidden, from + columns);
     const float *r = router + (size_t)(i / stretches) * hidden;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (wide) {
+    double d = 0.0;
+    for (int j0 = from; j0 < to; j0 += 128 * CHAIN) {
+      const int j1 = min(to, j0 + 128 * CHAIN);
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      if (wide) {
 #pragma unroll 8
-      for (int j = from + lane * 4; j < to; j += 128) {
-        const float4 a = *reinterpret_cast<const float4 *>(xr + j);
-        const float4 b = __ldg(reinterpret_cast<const float4 *>(r + j));
-        s[0] = fmaf(a.x, b.x, s[0]);
-        s[1] = fmaf(a.y, b.y, s[1]);
-        s[2] = fmaf(a.z, b.z, s[2]);
-        s[3] = fmaf(a.w, b.w, s[3]);
-      }
-    } else {
-      for (int j = from + lane; j < to; j += 128)
+        for (int j = j0 + lane * 4; j < j1; j += 128) {
+          const float4 a = *reinterpret_cast<const float4 *>(xr + j);
+          const float4 b = __ldg(reinterpret_cast<const float4 *>(r + j));
+          s[0] = fmaf(a.x, b.x, s[0]);
+          s[1] = fmaf(a.y, b.y, s[1]);
+          s[2] = fmaf(a.z, b.z, s[2]);
+          s[3] = fmaf(a.w, b.w, s[3]);
+        }
+      } else {
+        for (int j = j0 + lane; j < j1; j += 128)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (j + 32 * c < to) s[c] = fmaf(xr[j + 32 * c], r[j + 32 * c], s[c]);
+          for (int c = 0; c < 4; ++c)
+            if (j + 32 * c < j1) s[c] = fmaf(xr[j + 32 * c], r[j + 32 * c], s[c]);
+      }
+      d += ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
     }
-    double d = ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) zs[i] = d;

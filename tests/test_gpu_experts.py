@@ -404,3 +404,45 @@ def test_routing_reads_the_last_columns(torch_cuda, experts, hidden, offset):
     want = torch.softmax(z, 1).gather(1, best.indices)
     off = 2 * (hidden / 128 + 8) * 2.0 ** -24 * float(terms) + 2.0 ** -23
     assert bool(((weights.double() - want).abs() <= off * want).all())
+
+
+def test_routing_sums_long_rows(torch_cuda):
+    """The widest rows: logits of about 2^18 that differ by 4.  Expert 9's terms 1 + 2^-14
+    are sums of up to 2^10 that f32 holds exactly; past that every other step of a longer
+    f32 chain loses the 2^-14.  Chains of 16 terms stay exact here, and so do their
+    64-bit sums: only the weights' own roundings are left."""
+    torch = torch_cuda
+    experts, hidden = 64, 1 << 18
+    router = torch.zeros(experts, hidden)
+    router[9] = 1 + 2.0 ** -14  # in all 2^18 + 16
+    router[4] = 1.0
+    router[4, 77] = 13.0        # 2^18 + 12
+    for offset in (0, 1):
+        buf = torch.zeros(router.numel() + offset, device="cuda")
+        buf[offset:] = router.flatten().cuda()
+        ids, weights = _route(torch, buf[offset:].view(router.shape),
+                              torch.ones(2, hidden, device="cuda"), 2, True)
+        assert ids.tolist() == [[9.0, 4.0]] * 2
+        want = torch.softmax(torch.tensor([4.0, 0.0]).double(), 0)
+        assert float((weights.double() - want).abs().max()) <= 2.0 ** -24
+
+
+def test_routing_of_wide_rows_against_64_bits(torch_cuda):
+    """2^18 columns: a logit's chains of 16 terms are off by at most 16 2^-24 of their
+    terms' magnitudes, and by about 2^-24 of each partial sum (independent roundings): far
+    below the margin of 1e-3 that the choices of these inputs have."""
+    torch = torch_cuda
+    experts, hidden, m, top_k = 40, 1 << 18, 2, 4
+    g = torch.Generator().manual_seed(6)
+    router = torch.randn(experts, hidden, generator=g) / 256
+    x = torch.randn(m, hidden, generator=g)
+    z = x.double() @ router.double().T
+    order = torch.sort(z, dim=1, descending=True)
+    assert float((order.values[:, :top_k] - order.values[:, 1:top_k + 1]).min()) > 1e-3
+    ids, weights = _route(torch, router.cuda(), x.cuda(), top_k, False)
+    assert torch.equal(ids.long(), order.indices[:, :top_k])
+    # 2^18 roundings of partial sums of up to 4 / 256 * 3, each at most 2^-24 of them: their
+    # root-sum-square is below 512 * 0.047 * 2^-24 = 1.5e-6; a logit is off by less than six
+    # times that, a weight by twice a logit and its own rounding
+    want = torch.softmax(z, 1).gather(1, ids.long())
+    assert bool(((weights.double() - want).abs() <= (2 * 9e-6 + 2.0 ** -23) * want).all())
