@@ -331,15 +331,24 @@ __device__ __forceinline__ bool find_tile(const Params &p, int t, SmallPlan &pla
 
 // ---- operands --------------------------------------------------------------------------------
 
+// Rounded to a term of an operand, infinities and what would round to one to the largest
+// finite term of their sign: what is left of them is for the next term.  (An infinity
+// here would leave NaN or one of the other sign.)
 __device__ __forceinline__ uint32_t tf32(float v) {
   uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
   return r;
 }
-// v = hi + lo to 22 bits
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+// v = hi + lo to 22 bits.  lo is cut where it could be rounded to half of that error: the
+// largest value's rest would be rounded up, and the sum overflow.
 __device__ __forceinline__ void split(float v, uint32_t &hi, uint32_t &lo) {
   hi = tf32(v);
-  lo = tf32(v - __uint_as_float(hi));
+  lo = __float_as_uint(v - __uint_as_float(hi)) & 0xFFFFE000u;
 }
 __device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -371,15 +380,15 @@ template <typename T>
 constexpr bool THREE = std::is_same<T, __nv_bfloat16>::value;
 __device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
   auto take = [&]() {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-    const uint32_t r = *reinterpret_cast<const uint32_t *>(&b);
+    const uint32_t r = bf16_pair(x, y);
     x -= __uint_as_float(r << 16);
     y -= __uint_as_float(r & 0xFFFF0000u);
     return r;
   };
   hi = take();
   mid = take();
-  lo = take();
+  const __nv_bfloat162 rest = __floats2bfloat162_rn(x, y);
+  lo = *reinterpret_cast<const uint32_t *>(&rest);
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -553,8 +562,10 @@ __device__ __forceinline__ void shrink(const Params &p, const Tile &tile, const 
         for (int n = 0; n < RC / 8; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float *at = part + (mt * M + g + 8 * (i >> 1)) * stride + r0 + n * 8 + 2 * t + (i & 1);
-            *at = k ? *at + acc[n][i] : acc[n][i];
+            const int r = r0 + n * 8 + 2 * t + (i & 1);
+            float *at = part + (mt * M + g + 8 * (i >> 1)) * stride + r;
+            // (behind the last rank 0, whatever x: infinities times zeros are none)
+            *at = r >= p.rank ? 0.f : k ? *at + acc[n][i] : acc[n][i];
           }
       __syncthreads();
     }

@@ -20,6 +20,7 @@ import synthetic
 
 pytestmark = pytest.mark.gpu
 
+INF = float("inf")
 DTYPES = {"f32": mgb.F32, "f16": mgb.F16, "bf16": mgb.BF16}
 
 
@@ -367,3 +368,57 @@ def test_smaller_batches_take_the_largest_ones_workspace(torch_cuda, count, rank
                 torch.cuda.synchronize()
                 assert bool(y[:m].isfinite().all())
             assert bool((y[m:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("count,per", [(4, 1), (2, 4), (2, 5), (3, 40), (8, 20)])
+@pytest.mark.parametrize("rank", [3, 16, 24, 72])
+@pytest.mark.parametrize("k", [37, 40])
+def test_infinite_and_largest_activations(torch_cuda, dtype, count, per, rank, k):
+    """Infinities stay what f32 arithmetic makes of them, and the largest finite values
+    stay finite, however many rows share the adapter.  A's first column passes x on to the
+    first rank alone, everything else is positive: an infinite x among values of its sign
+    makes every output infinite."""
+    torch = torch_cuda
+    n, m = 70, count * per
+    g = torch.Generator().manual_seed(rank + k)
+    dt = _torch_dtype(torch, dtype)
+    a = (0.5 + 0.5 * torch.rand(count, rank, k, generator=g)).to(dt)
+    a[:, :, 0] = 0
+    a[:, 0, 0] = 1
+    b = (0.0625 + 0.0625 * torch.rand(count, n, rank, generator=g)).to(dt)
+    one = torch.ones(count)
+    x = 0.1 + torch.rand(m, k, generator=g)
+    base = torch.randn(m, n, generator=g)
+    ids = (torch.arange(m) // per).float()
+    x[0, 5] = INF
+    x[1] *= -1
+    x[1, k - 1] = -INF
+    big = float(torch.finfo(torch.float32).max)
+    x[2], x[3] = 0, 0
+    x[2, 0], x[3, 0] = big, -big
+    dev = [t.cuda() for t in (a, b, one, ids, x, base)]
+    y = _call(torch, *dev[:3], dtype, *dev[3:])
+    assert bool((y[0] == INF).all()) and bool((y[1] == -INF).all())
+    x[:2] = 0
+    want, mag = _expected(a, b, one, ids, x, base)
+    _check(y[2:], want[2:], mag[2:], base[2:], k, rank)
+
+
+@pytest.mark.parametrize("per", [1, 4, 5, 40])
+def test_largest_f32_factors(torch_cuda, per):
+    """f32 factors next to the type's largest value."""
+    torch = torch_cuda
+    big = float(torch.finfo(torch.float32).max)
+    count, rank, k, n = 4, 8, 40, 36
+    m = count * per
+    a, b = torch.zeros(count, rank, k), torch.zeros(count, n, rank)
+    a[:, 0, 0], a[:, 1, 1] = big, 1.0   # h[0] = big x[0], h[1] = x[1]
+    b[:, ::2, 0], b[:, 1::2, 1] = 0.5, -big
+    x = torch.zeros(m, k)
+    x[:, :2] = 0.25
+    ids = (torch.arange(m) % count).float()
+    base, one = torch.zeros(m, n), torch.ones(count)
+    want, mag = _expected(a, b, one, ids, x, base)
+    dev = [t.cuda() for t in (a, b, one, ids, x)]
+    _check(_call(torch, *dev[:3], "f32", *dev[3:], None), want, mag, base, k, rank)
