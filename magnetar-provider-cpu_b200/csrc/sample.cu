@@ -674,15 +674,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
   Weigh weigh;
   weigh.top = row.top;
   weigh.pow2 = pow2;
+  const double log2e_t = 1.4426950408889634 / (double)temp;
   {
-    const double c = fmin(1.4426950408889634 / (double)temp, 1e30);  // 1 / T stays finite
+    const double c = fmin(log2e_t, 1e30);  // 1 / T stays finite
     weigh.chi = (float)c;
     weigh.clo = (float)(c - (double)weigh.chi);
   }
   const float pf = p.top_p ? p.top_p[r] : 1.f, mf = p.min_p ? p.min_p[r] : 0.f;
   const float uf = p.uniform[r];
   const double u = uf > 0.f ? (double)fminf(uf, 0.99999994f) : 0.0;
-  const u64 least = mf > 0.f ? (u64)ceil((double)fminf(mf, 1.f) * (double)(1ull << ONE_BITS)) : 0;
+  // min-p compares probabilities by their logits: their weights are rounded, and small
+  // ones have few bits or none
+  const bool min_p = mf > 0.f;
+  const double deepest = min_p ? -log2((double)fminf(mf, 1.f)) : 0.0;  // octaves below the largest
+  auto likely = [&](float v) { return v == row.top || ((double)row.top - (double)v) * log2e_t <= deepest; };
   auto logprob_of = [&](float v, u64 total) {
     const double own = v == row.top ? 0.0 : ((double)v - (double)row.top) / (double)temp;
     return (float)(own - log((double)total * (1.0 / (double)(1ull << ONE_BITS))));
@@ -708,7 +713,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
     u64 total;
     const u64 sum = block_scan(w, s, total);
     if (pf < 1.f) n = __syncthreads_count(i < n && sum - w < mass_target(total));
-    n = __syncthreads_count(i < n && (w >= least || key == row.top_key));
+    if (min_p) n = __syncthreads_count(i < n && likely(value_of(key)));
     s.list[i] = w;
     if (i + 1 == n) s.above = sum;  // the kept total
     __syncthreads();
@@ -730,11 +735,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
   if (kf >= 1.f && floorf(kf) < (float)live)
     cut_at<false, THREADS>(row, [&](u64) { return (u64)kf; }, weigh, s, cluster, cut);
   if (pf < 1.f) cut_at<true, THREADS>(row, mass_target, weigh, s, cluster, cut);
-  if (least) {  // weights fall with the key: the smallest that is heavy enough
+  if (min_p) {  // probabilities fall with the key: the smallest that is likely enough
     uint32_t l = LOWEST, h = row.top_key;
     while (l < h) {
       const uint32_t m = l + (h - l) / 2;
-      if (weigh(value_of(m)) >= least) h = m;
+      if (likely(value_of(m))) h = m;
       else l = m + 1;
     }
     const u64 light = ((u64)l << 32) - 1;

@@ -382,3 +382,25 @@ def test_the_log_probability_of_an_unlikely_token(torch_cuda, rows, vocab, top_k
     want = (zd[:, 0] - torch.logsumexp(zd, 1)).numpy()
     bound = 2.0 ** -24 * np.abs(want) + 2.0 ** -29
     assert (np.abs(logprob.astype(np.float64) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 12), (3, 5000), (100, 5000)])
+@pytest.mark.parametrize("top_k", [0, 9])
+def test_small_min_p(torch_cuda, rows, vocab, top_k):
+    """Borders below and between the units of 2^-43 in which masses are summed, and next to
+    the largest: what is kept is what the definition keeps."""
+    torch = torch_cuda
+    base = torch.full((rows, vocab), -INF)
+    near = float(np.nextafter(np.float32(2.0 ** -10), np.float32(0)))
+    for values, min_p, kept in (([-33.0, 0.0, -31.0, -1.0], 1e-14, 3),    # e^-31 = 3.4e-14
+                                ([0.0, -28.8, -2.0], 3.2e-13, 2),          # e^-28.8 = 3.11e-13
+                                ([0.0, -28.7, -2.0], 3.4e-13, 3),          # e^-28.7 = 3.43e-13
+                                ([-80.0, -87.0, 0.0, -90.0], 1e-38, 3),    # e^-87 = 1.6e-38
+                                ([2.0 ** -10, near, 0.0], 1.0, 1)):        # 1 - 5.8e-11
+        z = base.clone()
+        z[:, 2:2 + len(values)] = torch.tensor(values)
+        _check(torch, z, uniform=torch.full((rows,), 0.3), min_p=torch.full((rows,), min_p),
+               top_k=torch.full((rows,), float(top_k)))
+        n = _call(torch, z, uniform=torch.full((rows,), 0.3), min_p=torch.full((rows,), min_p),
+                  top_k=torch.full((rows,), float(top_k)))[2]
+        assert (n == kept).all(), (values, n)
