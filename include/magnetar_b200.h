@@ -481,7 +481,8 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
 
 /* One token per row of logits [rows, vocab] (row stride ld >= vocab values).
  * Row parameters, f32 device arrays of `rows` values (NULL: the neutral value):
- *   temperature  p ~ exp(logit / temperature); <= 0 or NaN: greedy (neutral: 1)
+ *   temperature  p ~ exp(logit / temperature); <= 0 or NaN: greedy (neutral: 1);
+ *                below 2^-127 it acts as about that
  *   top_k        keeps the first top_k tokens; < 1 or NaN: all (neutral: 0)
  *   top_p        keeps the shortest prefix whose share of the probability left
  *                by top_k is at least top_p; >= 1 or NaN: all (neutral: 1)
@@ -501,7 +502,8 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
  * kept [rows], how many tokens were kept (u32).  Probabilities are summed as
  * 64-bit fixed-point numbers in units of 2^-43 of the largest (each within
  * 2^-31 of itself or half a unit), so sums do not depend on their order; a
- * token below half a unit is never drawn.  A log-probability is its logit's,
+ * token below half a unit, or further from the largest logit than f32 reaches,
+ * is never drawn.  A log-probability is its logit's,
  * less the logarithm of the kept sum. */
 #define MGB_SAMPLE_MAX_VOCAB (1u << 20)
 uint64_t mgb_sample_workspace_bytes(uint64_t rows, uint64_t vocab);

@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
   weigh.pow2 = pow2;
   const double log2e_t = 1.4426950408889634 / (double)temp;
   {
-    const double c = fmin(log2e_t, 1e30);  // 1 / T stays finite
+    const double c = fmin(log2e_t, (double)FLT_MAX);  // (finite for every T that is not subnormal)
     weigh.chi = (float)c;
     weigh.clo = (float)(c - (double)weigh.chi);
   }

@@ -404,3 +404,13 @@ def test_small_min_p(torch_cuda, rows, vocab, top_k):
         n = _call(torch, z, uniform=torch.full((rows,), 0.3), min_p=torch.full((rows,), min_p),
                   top_k=torch.full((rows,), float(top_k)))[2]
         assert (n == kept).all(), (values, n)
+
+
+def test_the_smallest_temperatures(torch_cuda):
+    """Temperatures down to the smallest normal number divide logits that are as close."""
+    torch = torch_cuda
+    for t in (1e-29, 1e-31, 1e-33, 1.2e-38):
+        z = torch.tensor([[0.0, -t, -2 * t, -300 * t if t > 1e-36 else -1.0]])
+        for kw in ({}, dict(top_p=[0.7]), dict(top_k=[2.0]), dict(top_k=[3.0], top_p=[0.7]), dict(min_p=[0.2])):
+            for u in (0.1, 0.8):
+                _check(torch, z, temperature=[t], uniform=[u], **kw)
