@@ -444,7 +444,9 @@ typedef struct mgb_experts {
     int32_t gate_up_format, down_format;
 } mgb_experts;
 /* Scratch bytes of mgb_moe_layer and mgb_moe_experts for m tokens of top_k
- * experts each (0 for arguments they refuse), and of mgb_moe_route. */
+ * experts each (0 for arguments they refuse; never falling as m or top_k
+ * grows), and of mgb_moe_route, which takes none: 0, and its workspace may be
+ * NULL. */
 uint64_t mgb_moe_workspace_bytes(const mgb_experts *experts, uint64_t m, uint64_t top_k);
 uint64_t mgb_moe_route_workspace_bytes(uint64_t experts, uint64_t hidden, uint64_t m);
 /* Routing: z = x [m, hidden] * router^T (router f32 [experts, hidden]), then
@@ -506,6 +508,7 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
  * is never drawn.  A log-probability is its logit's,
  * less the logarithm of the kept sum. */
 #define MGB_SAMPLE_MAX_VOCAB (1u << 20)
+/* 0: sampling takes no scratch, and its workspace may be NULL. */
 uint64_t mgb_sample_workspace_bytes(uint64_t rows, uint64_t vocab);
 mgb_status mgb_sample(const float *logits, uint64_t rows, uint64_t vocab, uint64_t ld,
                       const float *temperature, const float *top_k, const float *top_p,

@@ -314,17 +314,20 @@ __global__ void __launch_bounds__(1024) mgb_adapter_plan_kernel(const Params p) 
   }
 }
 
-// The CTA's tile and its rows (row[i] of lanes' tokens, absent ones repeat the
-// first); false: no such tile.
-__device__ __forceinline__ bool find_tile(const Params &p, int t, SmallPlan &plan, int (&rows)[MOST_ROWS],
+// The CTA's tile and its rows (absent ones repeat the first); false: no such tile.  Up
+// to INLINE_ROWS rows, by a plan of its own, and from the grouped rows.
+__device__ __forceinline__ bool plan_tile(const Params &p, int t, SmallPlan &plan, int (&rows)[MOST_ROWS],
                                           bool report, Tile &tile) {
-  const bool small = p.m <= INLINE_ROWS;
-  if (t >= (small ? plan_small(p, plan, report) : *p.ntiles)) return false;
-  tile = small ? plan.tiles[t] : p.tiles[t];
-  if (threadIdx.x < MOST_ROWS) {
-    const int i = tile.start + (threadIdx.x < tile.len ? threadIdx.x : 0);
-    rows[threadIdx.x] = small ? plan.order[i] : p.order[i];
-  }
+  if (t >= plan_small(p, plan, report)) return false;
+  tile = plan.tiles[t];
+  if (threadIdx.x < MOST_ROWS) rows[threadIdx.x] = plan.order[tile.start + (threadIdx.x < tile.len ? threadIdx.x : 0)];
+  __syncthreads();
+  return true;
+}
+__device__ __forceinline__ bool grouped_tile(const Params &p, int t, int (&rows)[MOST_ROWS], Tile &tile) {
+  if (t >= *p.ntiles) return false;
+  tile = p.tiles[t];
+  if (threadIdx.x < MOST_ROWS) rows[threadIdx.x] = p.order[tile.start + (threadIdx.x < tile.len ? threadIdx.x : 0)];
   __syncthreads();
   return true;
 }
@@ -990,7 +993,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   grid_dependents();
   Tile tile;
   // (the whole cluster has one tile)
-  if (!find_tile(p, blockIdx.x / ctas, plan, rows, blockIdx.x == 0, tile)) return;
+  if (!plan_tile(p, blockIdx.x / ctas, plan, rows, blockIdx.x == 0, tile)) return;
   const bool few = few_rows(p, tile);
   // B's first copies are under way while h is taken, where shared memory holds both
   const int first = cta * WARPS + warp;
@@ -1030,7 +1033,6 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
 template <typename T, int RC>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapter_h_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ SmallPlan plan;
   __shared__ int rows[MOST_ROWS];
   const int width = h_width(p.rank, RC);
   float *part = reinterpret_cast<float *>(smem);
@@ -1038,7 +1040,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2) mgb_adapte
   grid_dependents();
   Tile tile;
   const int split = blockIdx.x % p.splits;
-  if (!find_tile(p, blockIdx.x / p.splits, plan, rows, false, tile) || tile.id < 0) return;
+  if (!grouped_tile(p, blockIdx.x / p.splits, rows, tile) || tile.id < 0) return;
   const int groups = (p.k + 31) / 32, per = (groups + p.splits - 1) / p.splits;
   const int g0 = min(groups, split * per), g1 = min(groups, g0 + per);
   if (few_rows(p, tile)) shrink_few<T>(p, tile, rows, g0, g1, width, part);
@@ -1052,7 +1054,6 @@ template <typename T, int RC, bool WIDE>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
     mgb_adapter_y_kernel(const Params p, int slices) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ SmallPlan plan;
   __shared__ int rows[MOST_ROWS];
   const int width = h_width(p.rank, RC), warp = threadIdx.x >> 5;
   uint4 *hs = reinterpret_cast<uint4 *>(smem);
@@ -1060,7 +1061,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 4 ? 1 : 2)
   grid_dependents();
   Tile tile;
   const int slice = blockIdx.x % slices;
-  if (!find_tile(p, blockIdx.x / slices, plan, rows, false, tile)) return;
+  if (!grouped_tile(p, blockIdx.x / slices, rows, tile)) return;
   const bool few = few_rows(p, tile);
   if (tile.id >= 0) {
     auto sum = [&](int row, int r) {

@@ -182,12 +182,8 @@ mgb_status mgb_qmatmul_adapters(int32_t format, const void *w, uint64_t n, uint6
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "adapter launch");
 }
 
-uint64_t mgb_moe_route_workspace_bytes(uint64_t experts, uint64_t hidden, uint64_t m) {
-  if (!experts || experts > MGB_MOE_MAX_EXPERTS || !hidden || hidden > MGB_MOE_MAX_WIDTH ||
-      m > MGB_MOE_MAX_TOKENS)
-    return 0;
-  return round16(moe_route_scratch_bytes(experts, hidden, m));
-}
+// (routing and sampling need no scratch)
+uint64_t mgb_moe_route_workspace_bytes(uint64_t, uint64_t, uint64_t) { return 0; }
 
 // The experts' scratch, then room for mgb_moe_layer's ids and weights.
 uint64_t mgb_moe_workspace_bytes(const mgb_experts *experts, uint64_t m, uint64_t top_k) {
@@ -197,16 +193,14 @@ uint64_t mgb_moe_workspace_bytes(const mgb_experts *experts, uint64_t m, uint64_
 
 mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden, const float *x,
                          uint64_t m, uint64_t top_k, int32_t normalize, float scale, float *ids,
-                         float *weights, void *workspace, uint64_t workspace_bytes, void *stream) {
+                         float *weights, void *, uint64_t, void *stream) {
   mgb_status s = check_route(router, experts, hidden, x, m, top_k);
   if (s == MGB_OK && m && (!ids || !weights)) s = fail(MGB_INVALID_ARGUMENT, "null device pointer");
   if (s == MGB_OK && (!aligned(ids, 4) || !aligned(weights, 4)))
     s = fail(MGB_INVALID_ARGUMENT, "a device pointer is not aligned to its element size");
-  if (s == MGB_OK)
-    s = check_workspace(workspace, workspace_bytes, moe_route_scratch_bytes(experts, hidden, m));
   if (s != MGB_OK) return s;
   cudaError_t e = launch_moe_route(router, experts, hidden, x, m, top_k, normalize != 0, scale, ids,
-                                   weights, nullptr, workspace, static_cast<cudaStream_t>(stream));
+                                   weights, nullptr, nullptr, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "routing launch");
 }
 
@@ -247,15 +241,12 @@ mgb_status mgb_moe_layer(const mgb_experts *experts, const float *router, const 
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "expert launch");
 }
 
-uint64_t mgb_sample_workspace_bytes(uint64_t rows, uint64_t vocab) {
-  if (!vocab || vocab > MGB_SAMPLE_MAX_VOCAB || rows > (1ull << 31)) return 0;
-  return sample_scratch_bytes(rows, vocab);
-}
+uint64_t mgb_sample_workspace_bytes(uint64_t, uint64_t) { return 0; }
 
 mgb_status mgb_sample(const float *logits, uint64_t rows, uint64_t vocab, uint64_t ld,
                       const float *temperature, const float *top_k, const float *top_p,
                       const float *min_p, const float *uniform, float *ids, float *logprob,
-                      uint32_t *kept, void *workspace, uint64_t workspace_bytes, void *stream) {
+                      uint32_t *kept, void *, uint64_t, void *stream) {
   if (!vocab || vocab > MGB_SAMPLE_MAX_VOCAB)
     return fail(MGB_INVALID_ARGUMENT, "vocabulary of %llu tokens, expected 1 to %u",
                 (unsigned long long)vocab, MGB_SAMPLE_MAX_VOCAB);
@@ -269,11 +260,10 @@ mgb_status mgb_sample(const float *logits, uint64_t rows, uint64_t vocab, uint64
                         (const void *)ids, (const void *)logprob, (const void *)kept})
     if (!aligned(p, 4))
       return fail(MGB_INVALID_ARGUMENT, "a device pointer is not aligned to its element size");
-  mgb_status s = check_workspace(workspace, workspace_bytes, sample_scratch_bytes(rows, vocab));
-  if (s != MGB_OK || !rows) return s;
+  if (!rows) return MGB_OK;
   const SampleArgs a{logits, rows,  vocab,   ld,  temperature, top_k,
                      top_p,  min_p, uniform, ids, logprob,     kept};
-  cudaError_t e = launch_sample(a, workspace, static_cast<cudaStream_t>(stream));
+  cudaError_t e = launch_sample(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "sampling launch");
 }
 

@@ -311,8 +311,6 @@ __global__ void __launch_bounds__(256)
   y[at] = addend ? addend[at] + a : a;
 }
 
-uint64_t moe_route_scratch_bytes(uint64_t, uint64_t, uint64_t) { return 0; }
-
 static int current_sms() {
   int dev = 0;
   cudaGetDevice(&dev);

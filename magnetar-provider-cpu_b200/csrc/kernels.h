@@ -70,7 +70,6 @@ cudaError_t launch_adapters(const mgb_adapters &ad, const float *ids, const floa
 
 // experts.cu.  With pack_for (the experts of mgb_moe_layer, `workspace` theirs)
 // the routing kernel also packs the activations for the products.
-uint64_t moe_route_scratch_bytes(uint64_t experts, uint64_t hidden, uint64_t m);
 uint64_t moe_experts_scratch_bytes(const mgb_experts &ex, uint64_t m, uint64_t top_k);
 cudaError_t launch_moe_route(const float *router, uint64_t experts, uint64_t hidden,
                              const float *x, uint64_t m, uint64_t top_k, int normalize,
@@ -90,8 +89,7 @@ struct SampleArgs {
   float *ids, *logprob;
   uint32_t *kept;
 };
-uint64_t sample_scratch_bytes(uint64_t rows, uint64_t vocab);
-cudaError_t launch_sample(const SampleArgs &a, void *workspace, cudaStream_t stream);
+cudaError_t launch_sample(const SampleArgs &a, cudaStream_t stream);
 
 int device_sms(int device);
 

@@ -845,8 +845,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2)
   }
 }
 
-uint64_t sample_scratch_bytes(uint64_t, uint64_t) { return 0; }
-
 template <int THREADS, bool STAGED>
 static cudaError_t launch_sample_kernel(const SampleArgs &a, uint32_t ctas, uint32_t chunk, int dev,
                                         cudaStream_t stream) {
@@ -889,7 +887,7 @@ static cudaError_t launch_sample_kernel(const SampleArgs &a, uint32_t ctas, uint
   return cudaSuccess;
 }
 
-cudaError_t launch_sample(const SampleArgs &a, void *, cudaStream_t stream) {
+cudaError_t launch_sample(const SampleArgs &a, cudaStream_t stream) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;

@@ -199,3 +199,16 @@ def test_a_larger_batch_never_needs_a_smaller_workspace(count, rank, k):
         need = mgb.adapters_workspace_bytes(ad, m)
         assert need >= most, m
         most = need
+
+
+@pytest.mark.parametrize("gate_up,down,experts,hidden,ffn", [
+    (mgb.Q4_K, mgb.Q6_K, 8, 4096, 14336), (mgb.Q8_0, mgb.Q8_0, 64, 4096, 1536),
+    (mgb.IQ4_NL, mgb.Q8_0, 20, 1440, 992), (mgb.Q5_K, mgb.Q4_0, 1, 256, 256)])
+def test_more_tokens_never_need_a_smaller_workspace(gate_up, down, experts, hidden, ffn):
+    ex = _experts(gate_up_fmt=gate_up, down_fmt=down, count=experts, hidden=hidden, ffn=ffn)
+    size = [[mgb.moe_workspace_bytes(ex, m, top_k) for top_k in range(1, 33)] for m in range(257)]
+    assert all(a <= b for row in size for a, b in zip(row, row[1:]))
+    assert all(a <= b for row, after in zip(size, size[1:]) for a, b in zip(row, after))
+    # routing and sampling take none
+    assert mgb.moe_route_workspace_bytes(experts, hidden, 256) == 0
+    assert mgb.sample_workspace_bytes(256, 128256) == 0
