@@ -422,3 +422,29 @@ def test_largest_f32_factors(torch_cuda, per):
     want, mag = _expected(a, b, one, ids, x, base)
     dev = [t.cuda() for t in (a, b, one, ids, x)]
     _check(_call(torch, *dev[:3], "f32", *dev[3:], None), want, mag, base, k, rank)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,k,rank,count", [(64, 4096, 16, 1), (128, 8192, 64, 1), (1000, 8192, 128, 3),
+                                            (20000, 4096, 16, 1), (20000, 8192, 64, 4)])
+def test_sums_over_long_rows(torch_cuda, dtype, m, k, rank, count):
+    """The 2-norm's error of long sums, whose lengths a thread depend on the batch.
+
+    A thread adds at most k / 64 sums of 32 products, each addition off by up to 2^-24 of
+    the running sum; those are independent, and running sums grow with the root of their
+    number: 0.3 2^-24 (k / 128)^(1/2), 2.4 2^-24 for k = 8,192.  A tensor core's sum is cut at
+    each of up to 12 steps, by half of 2^-23 of what it holds: 6 2^-24 within a group of 32
+    products, and for h, rank / 8 times 3 of them (in passes of 64: 24), 12 2^-24 in y, two
+    thirds of each on average over the growing sum.  In all below 16 2^-24 = 2^-20."""
+    torch = torch_cuda
+    n = 96
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    dt = _torch_dtype(torch, dtype)
+    randn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    a, b = (randn(count, rank, k) / k ** 0.5).to(dt), (randn(count, n, rank) / rank ** 0.5).to(dt)
+    x, ids = randn(m, k), (torch.arange(m, device="cuda") % count).float()
+    y = _call(torch, a, b, None, dtype, ids, x, None)
+    want = torch.empty(m, n, dtype=torch.float64, device="cuda")
+    for i in range(count):
+        want[ids == i] = (x[ids == i].double() @ a[i].double().T) @ b[i].double().T
+    assert float((y - want).norm() / want.norm()) < 2.0 ** -20
