@@ -407,14 +407,16 @@ uint64_t mgb_adapters_workspace_bytes(const mgb_adapters *adapters, uint64_t m);
  * base[r] bit for bit, as does a row with an invalid id (not a whole number
  * below count; reported in `bad`).  Rows with the same id read its adapter
  * together.  f32 accuracy: products accumulate in f32 from operands of at
- * least 22 bits.  Infinite and largest finite activations and f32 factors give
- * what f32 arithmetic gives, in their row alone; an infinite f16 or bf16 factor
- * gives its rows infinities or NaN.  Deterministic. */
+ * least 22 bits.  Infinite and largest finite activations and f32
+ * factors give what f32 arithmetic gives, in their row alone; an infinite f16
+ * or bf16 factor gives its rows infinities or NaN.  Deterministic.  x does not
+ * overlap y, and base is y or does not overlap it (refused). */
 mgb_status mgb_adapters_add(const mgb_adapters *adapters, const float *ids, const float *x,
                             uint64_t m, const float *base, float *y, uint32_t *bad,
                             void *workspace, uint64_t workspace_bytes, void *stream);
 /* mgb_qmatmul and then mgb_adapters_add on its y: the shared packed projection
- * with every row's adapter beside it.  adapters->k and ->n equal k and n.  A
+ * with every row's adapter beside it.  adapters->k and ->n equal k and n; x
+ * does not overlap y.  A
  * row without an adapter equals mgb_qmatmul's bit for bit.  The workspace
  * serves both in turn (mgb_qmatmul_adapters_workspace_bytes); what the
  * adapters need is required, less than the projection prefers only costs it

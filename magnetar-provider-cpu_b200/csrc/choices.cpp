@@ -30,6 +30,12 @@ mgb_status check_workspace(const void *workspace, uint64_t have, uint64_t need) 
   return MGB_OK;
 }
 
+// Whether two buffers of f32 values share any of them.
+bool overlap(const float *a, uint64_t a_len, const float *b, uint64_t b_len) {
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  return a0 < b0 + b_len * 4 && b0 < a0 + a_len * 4;
+}
+
 uint64_t element_bytes(int32_t dtype) { return dtype == MGB_DTYPE_F32 ? 4 : 2; }
 
 // The descriptor alone and m (the size queries and the calls).
@@ -149,6 +155,10 @@ mgb_status mgb_adapters_add(const mgb_adapters *adapters, const float *ids, cons
   mgb_status s = check_adapters_call(adapters, ids, x, m, base, y, bad);
   if (s == MGB_OK) s = check_workspace(workspace, workspace_bytes, adapters_scratch_bytes(*adapters, m));
   if (s != MGB_OK) return s;
+  // (other rows' x and base are still read while a row's y is written)
+  const uint64_t n = adapters->n;
+  if (overlap(x, m * adapters->k, y, m * n) || (base && base != y && overlap(base, m * n, y, m * n)))
+    return fail(MGB_INVALID_ARGUMENT, "y overlaps x, or base without being it");
   cudaError_t e = launch_adapters(*adapters, ids, x, m, base, y, bad, workspace,
                                   static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MGB_OK : cuda_fail(e, "adapter launch");

@@ -212,3 +212,11 @@ def test_more_tokens_never_need_a_smaller_workspace(gate_up, down, experts, hidd
     # routing and sampling take none
     assert mgb.moe_route_workspace_bytes(experts, hidden, 256) == 0
     assert mgb.sample_workspace_bytes(256, 128256) == 0
+
+
+def test_adapters_refuse_overlapping_buffers():
+    ad = _adapters()  # k 64, n 96
+    x, y = FAKE, FAKE + 2 * 96 * 4
+    for bad in (dict(x=y, y=y), dict(x=y + 4 * 191, y=y), dict(x=y - 4 * 127, y=y),
+                dict(x=x - 4096, y=y, base=y + 4), dict(x=x - 4096, y=y, base=y - 4 * 191)):
+        assert "overlaps" in _add(ad, **bad)[1]
