@@ -448,3 +448,23 @@ def test_sums_over_long_rows(torch_cuda, dtype, m, k, rank, count):
     for i in range(count):
         want[ids == i] = (x[ids == i].double() @ a[i].double().T) @ b[i].double().T
     assert float((y - want).norm() / want.norm()) < 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m", [4, 40, 200])
+def test_activations_next_to_the_smallest_values(torch_cuda, dtype, m):
+    """Rows of 1e-30 down to subnormal ones.  A term of an operand is a multiple of 2^-136
+    (tf32) or 2^-133 (bf16), so x and h are within 2^-133 besides their 22 bits, and every
+    sum within f32's own smallest step, 2^-149."""
+    torch = torch_cuda
+    k, n, rank = 256, 64, 16
+    a, b, one, x, _ = _inputs(torch, m, k, n, rank, 1, dtype)
+    one[:] = 1
+    x *= 10.0 ** torch.linspace(-30, -43, m).double()[:, None]
+    x = x.float()
+    ids = torch.zeros(m)
+    want, mag = _expected(a, b, one, ids, x, torch.zeros(m, n))
+    y = _call(torch, *[t.cuda() for t in (a, b, one)], dtype, ids.cuda(), x.cuda(), None)
+    step = 2.0 ** -133 * (a[0].double().abs().sum(1) + 1) + k * 2.0 ** -149
+    small = b[0].double().abs() @ step + rank * 2.0 ** -149
+    assert bool(((y.double().cpu() - want).abs() <= (8 + k + rank) * 2.0 ** -24 * mag + 2.0 ** -23 * want.abs() + small).all())
