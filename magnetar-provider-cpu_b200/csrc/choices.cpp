@@ -87,7 +87,9 @@ mgb_status check_experts(const mgb_experts *ex, uint64_t m, uint64_t top_k) {
   if (!top_k || top_k > MGB_MOE_MAX_TOP_K)
     return fail(MGB_INVALID_ARGUMENT, "top_k %llu, expected 1 to %d", (unsigned long long)top_k,
                 MGB_MOE_MAX_TOP_K);
-  // blocks of 128 rows by 256 columns are counted in 32 bits
+  // Stages of 128 rows by at least 128 columns are counted in 32 bits.  Gate and up have
+  // two of them a block, but a pass of its own for more than half of the slots needs that
+  // many experts: above 2^30 blocks of 2^14 weights, more than a GPU holds.
   const uint64_t blocks = (ex->hidden / 128 + 1) * (ex->ffn / 128 + 1);
   if (m * top_k * blocks >= (1ull << 31))
     return fail(MGB_INVALID_ARGUMENT, "expert sizes are too large for %llu tokens",

@@ -446,3 +446,21 @@ def test_routing_of_wide_rows_against_64_bits(torch_cuda):
     # times that, a weight by twice a logit and its own rounding
     want = torch.softmax(z, 1).gather(1, ids.long())
     assert bool(((weights.double() - want).abs() <= (2 * 9e-6 + 2.0 ** -23) * want).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_infinities_stay_in_their_token(torch_cuda, oracle, fmt):
+    """Infinite activations, and finite ones whose h overflows: NaN for that token, and the
+    others' results as without it, in passes of 8 and of 16 tokens."""
+    torch = torch_cuda
+    layer = Layer(torch, oracle, fmt, fmt, 2, 256, 256)
+    for m in (6, 40):
+        x = _x(torch, m, 256)
+        ids, weights = _choices(torch, m, 2, 2)
+        clean = layer.run(x, ids.cuda(), weights.cuda())
+        x[1, 7], x[3, 200] = float("inf"), float("-inf")
+        x[5] *= 1e30
+        y = layer.run(x, ids.cuda(), weights.cuda())
+        assert bool(y[[1, 3, 5]].isnan().all())
+        rest = [t for t in range(m) if t not in (1, 3, 5)]
+        assert torch.equal(y[rest], clean[rest])
