@@ -470,7 +470,8 @@ mgb_status mgb_moe_route(const float *router, uint64_t experts, uint64_t hidden,
  * counts twice.  Each chosen expert's packed rows are read once for all its
  * tokens; f32 accuracy: weights enter exactly,
  * activations with at least 22 bits (values below 2^-27 of their row's largest:
- * 2^-40 of the largest), sums in f32.  A token with an infinite or NaN
+ * 2^-40 of the largest), sums in f32 (within 256 columns cut, not rounded: y is
+ * some 1e-6 off).  A token with an infinite or NaN
  * activation, or whose silu(gate) * up overflows, gets NaN, itself alone.
  * Deterministic.  The first call on a
  * device allocates its error word (see mgb_take_device_error), as mgb_qmatmul's

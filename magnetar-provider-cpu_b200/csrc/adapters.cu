@@ -15,17 +15,17 @@
 // products are bound by the adapters' bytes or, with many rows, by base and y: rank
 // operations a value, far from what tcgen05 is for.
 //
-// Measured (floors at the copy's rate): one row, k = n = 4,096, rank 16, 5.8 us, a
-// chain of the plan, A, the exchange and B; 64 rows of some 40 adapters, n = 14,336,
-// 18.2 us (4.7), of which B takes 5 to 7 us at nine warps an SM (with the tensor
+// Measured on the device (floors at the copy's rate): one row, k = n = 4,096, rank 16,
+// 5.8 us, a chain of the plan, A, the exchange and B; 64 rows of some 40 adapters, n =
+// 14,336, 18.6 us (4.7), of which B takes 5 to 7 us at nine warps an SM (with the tensor
 // cores' tiles 29.1 us, at 300 instructions a block of 32 outputs); 2,048 rows of rank
-// 64 102 us (42): grouping 6, h 22, y 73, which waits for base a block ahead and for
-// the tensor cores in about equal parts (two blocks ahead: the same time).
+// 64, bf16 94 us (42), f16 161, f32 174: in bf16 grouping 6, h 22, y 66, which waits for
+// base a block ahead and for the tensor cores (two blocks ahead: the same time).
 //
 // f32 accuracy from tf32: x and h are held as hi + lo, two tf32 terms (22 bits);
 // f16 factors are tf32 numbers as they are, f32 factors are split too.  Beside bf16
 // factors x and h are three bf16 terms, of m16n8k16: a quarter fewer MMAs, and no
-// factor is converted (2,048 rows 102 us instead of 107, 4,096 92 instead of 103).
+// factor is converted (2,048 rows 102 us instead of 107 when that came).
 // The order of a product's K is free, so a lane takes runs of neighbouring
 // values of its row: every load is 16 bytes where the buffers allow it.
 #include <cooperative_groups.h>
@@ -336,7 +336,8 @@ __device__ __forceinline__ bool grouped_tile(const Params &p, int t, int (&rows)
 
 // Rounded to a term of an operand, infinities and what would round to one to the largest
 // finite term of their sign: what is left of them is for the next term.  (An infinity
-// here would leave NaN or one of the other sign.)
+// here would leave NaN or one of the other sign.)  The conversion does it at no cost; a
+// minimum and a maximum a term took 0.5 us of 100 (2,048 rows of rank 64).
 __device__ __forceinline__ uint32_t tf32(float v) {
   uint32_t r;
   asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
@@ -606,8 +607,8 @@ __device__ __forceinline__ void shrink(const Params &p, const Tile &tile, const 
 
 // Few rows (of an adapter of up to 64 ranks): plain f32 arithmetic, of which a tensor
 // core's tile would leave most unused.  48 rows in tiles of 1, 2, 3 and 4 (k = 4,096, n =
-// 8,192): rank 16 bf16 10.8, 9.0, 10.5 and 8.7 us, as MMAs 19.3, 13.0, 12.6 and 11.0;
-// rank 64 f32 42.6, 31.9, 36.4 and 19.0, as MMAs 96, 61, 60 and 31.  More rows' partial
+// 8,192): rank 16 bf16 10.5, 8.6, 10.3 and 8.5 us, as MMAs 17.8, 12.6, 12.4 and 10.8;
+// rank 64 f32 40.5, 26.0, 30.8 and 16.7, as MMAs 83, 50, 50 and 26.5.  More rows' partial
 // sums would not fit a tile's shared memory.
 constexpr int FEW = 4;
 __device__ __forceinline__ bool few_rows(const Params &p, const Tile &tile) {
@@ -1250,8 +1251,8 @@ cudaError_t launch_rc(const Params &p, unsigned tiles, int sms, cudaStream_t str
   // Slices of the outputs: those with the fewest waves of CTAs (two an SM) times the
   // blocks of a warp and one more, about what a CTA takes before its first block (the
   // rows, h as operands); summed for the fewest tiles that the rows can make and for the
-  // middle of that and the most.  2,048 rows, 32 to 41 tiles, 14,336 outputs: 8 slices, a
-  // wave, 76 us; 14 slices 91 us, 28 slices 100 us.
+  // middle of that and the most.  2,048 rows, 32 to 41 tiles, 14,336 outputs, y alone when
+  // the rule was set: 8 slices, a wave, 76 us (now 66); 14 slices 91 us, 28 slices 100 us.
   const uint64_t blocks = ceil_div(p.n, COLS), full = ceil_div(p.m, p.tile_rows);
   uint64_t slices = 1, least = ~0ull;
   for (uint64_t s = 1; s <= 64 && s <= ceil_div(blocks, WARPS); ++s) {

@@ -30,9 +30,9 @@
 // tile whose stages fall to several CTAs gets a partial result from each; the
 // kernel that reads the product adds them in order.
 //
-// Measured: 64 tokens, 8 experts of 4,096 x 14,336, Q4_K and Q5_K 472 us the layer
-// (132 at the copy's rate of the packed bytes); 16 tokens on 64 experts of 4,096 x
-// 1,536, Q8_0, 274 us (175); one token on two wide experts 112 us (36).  Bound by
+// Measured on the device: 64 tokens, 8 experts of 4,096 x 14,336, Q4_K and Q5_K 475 to
+// 480 us the layer (132 at the copy's rate of the packed bytes); 16 tokens on 64 experts
+// of 4,096 x 1,536, Q8_0, 270 us (175); one token on two wide experts 111 us (36).  Bound by
 // instruction issue (2.4 to 2.6 a cycle and SM, 3.6 lane instructions a Q4_K weight,
 // 6.8 a Q6_K one) and, for one token, by what every launch takes before its first
 // weight.  Smaller steps with two A operands in TMEM: 143 us and 644 us instead of

@@ -23,10 +23,10 @@
 //    the bins: of 1/16, and if that holds too many tokens of 1/16384; the first CTA
 //    sorts the border bin's.  Where even that is too much (equal or nearly equal
 //    logits), by ever smaller ranges of keys.
-// Measured, 256 rows of 128,256 (131 MB; 20 us at the copy's rate): greedy 31 us,
-// no cuts 134 us (a weight costs some 45 instructions), top-k 1,000 151 us, top-p 0.95
-// 364 us (two histograms, two lists, the sum).  One row of 32,000, top-k 50 and
-// top-p: 15 us, a chain of dependent steps.
+// Measured on the device, 256 rows of 128,256 (131 MB; 20 us at the copy's rate): greedy
+// 31 us, no cuts 133 us (a weight costs some 45 instructions), min-p 76 us, top-k 50 72 us,
+// top-k 1,000 150 us, top-p 0.95 360 us (two histograms, two lists, the sum).  One row of
+// 32,000, top-k 50 and top-p: 15 us, a chain of dependent steps.
 //
 // Mass.  A token's weight is 2^((logit - max) log2(e) / T) as a 64-bit integer
 // in units of 2^-43: integer sums are the same in every order, so atomics and
