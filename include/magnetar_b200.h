@@ -407,10 +407,11 @@ uint64_t mgb_adapters_workspace_bytes(const mgb_adapters *adapters, uint64_t m);
  * base[r] bit for bit, as does a row with an invalid id (not a whole number
  * below count; reported in `bad`).  Rows with the same id read its adapter
  * together.  f32 accuracy: products accumulate in f32 from operands of at
- * least 22 bits (beside more than four rows of an adapter within 2^-133, which
- * values below 2^-111 notice).  Infinite and largest finite activations and f32
- * factors give what f32 arithmetic gives, in their row alone; an infinite f16
- * or bf16 factor gives its rows infinities or NaN.  Deterministic.  x does not
+ * least 22 bits (beside more than four rows of an adapter, or ranks above 64,
+ * within 2^-133, which values below 2^-111 notice).  Infinite activations, and
+ * the largest finite activations and f32 factors, give what f32 arithmetic
+ * gives, in their row alone; an infinite factor gives its rows infinities or
+ * NaN.  Deterministic.  x does not
  * overlap y, and base is y or does not overlap it (refused). */
 mgb_status mgb_adapters_add(const mgb_adapters *adapters, const float *ids, const float *x,
                             uint64_t m, const float *base, float *y, uint32_t *bad,

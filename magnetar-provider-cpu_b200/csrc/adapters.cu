@@ -19,7 +19,7 @@
 // 5.8 us, a chain of the plan, A, the exchange and B; 64 rows of some 40 adapters, n =
 // 14,336, 18.6 us (4.7), of which B takes 5 to 7 us at nine warps an SM (with the tensor
 // cores' tiles 29.1 us, at 300 instructions a block of 32 outputs); 2,048 rows of rank
-// 64, bf16 94 us (42), f16 161, f32 174: in bf16 grouping 6, h 22, y 66, which waits for
+// 64, bf16 94 us (42), f16 160, f32 187: in bf16 grouping 6, h 22, y 66, which waits for
 // base a block ahead and for the tensor cores (two blocks ahead: the same time).
 //
 // f32 accuracy from tf32: x and h are held as hi + lo, two tf32 terms (22 bits);
@@ -31,6 +31,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -361,7 +362,9 @@ __device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// c += (hi + lo) * (b0, b1) for factors of type T, to 22 bits of each, in two parts
+// c += (hi + lo) * (b0, b1) for factors of type T, to 22 bits of each, in two parts.
+// (lo times lo is up to 2^-22: without it 2,048 rows of f32 factors take 173 us, not 187,
+// and a product is off by half more.)
 template <typename T>
 __device__ __forceinline__ void multiply_small(float (&c)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
                                                float b0, float b1) {
@@ -369,6 +372,10 @@ __device__ __forceinline__ void multiply_small(float (&c)[4], const uint32_t (&h
     uint32_t h0, h1, l0, l1;
     split(b0, h0, l0);
     split(b1, h1, l1);
+    uint32_t finite[4];  // (an infinity, which lo carries, times a lower term may be NaN)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) finite[i] = fabsf(__uint_as_float(lo[i])) <= FLT_MAX ? lo[i] : 0u;
+    mma1688(c, finite, l0, l1);
     mma1688(c, lo, h0, h1);
     mma1688(c, hi, l0, l1);
   } else {
@@ -608,7 +615,7 @@ __device__ __forceinline__ void shrink(const Params &p, const Tile &tile, const 
 // Few rows (of an adapter of up to 64 ranks): plain f32 arithmetic, of which a tensor
 // core's tile would leave most unused.  48 rows in tiles of 1, 2, 3 and 4 (k = 4,096, n =
 // 8,192): rank 16 bf16 10.5, 8.6, 10.3 and 8.5 us, as MMAs 17.8, 12.6, 12.4 and 10.8;
-// rank 64 f32 40.5, 26.0, 30.8 and 16.7, as MMAs 83, 50, 50 and 26.5.  More rows' partial
+// rank 64 f32 41.5, 25.9, 30.8 and 16.7, as MMAs 83, 50, 50 and 26.5.  More rows' partial
 // sums would not fit a tile's shared memory.
 constexpr int FEW = 4;
 __device__ __forceinline__ bool few_rows(const Params &p, const Tile &tile) {

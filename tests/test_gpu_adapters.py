@@ -468,3 +468,20 @@ def test_activations_next_to_the_smallest_values(torch_cuda, dtype, m):
     step = 2.0 ** -133 * (a[0].double().abs().sum(1) + 1) + k * 2.0 ** -149
     small = b[0].double().abs() @ step + rank * 2.0 ** -149
     assert bool(((y.double().cpu() - want).abs() <= (8 + k + rank) * 2.0 ** -24 * mag + 2.0 ** -23 * want.abs() + small).all())
+
+
+@pytest.mark.parametrize("m", [1, 5, 150])
+@pytest.mark.parametrize("k,n,rank", [(1, 1, 1), (8, 36, 16), (33, 40, 70)])
+def test_f32_factors_low_terms_multiply(torch_cuda, m, k, n, rank):
+    """v = 1 + 2^-11 - 2^-22 is two terms exactly, and v v ends in the product of the lower
+    ones, 2^-22: left out, four times the 2^-24 that a rounded result is off by.  What is
+    left here is one cut of a sum just above 1, below 2^-23, and y's rounding."""
+    torch = torch_cuda
+    v = 1 + 2.0 ** -11 - 2.0 ** -22
+    x, ids, one = torch.zeros(m, k), torch.zeros(m), torch.ones(1)
+    x[:, 0] = v
+    for first, second in ((v, 1.0), (1.0, v)):
+        a, b = torch.zeros(1, rank, k), torch.zeros(1, n, rank)
+        a[0, 0, 0], b[0, :, 0] = first, second
+        y = _call(torch, *[t.cuda() for t in (a, b, one)], "f32", ids.cuda(), x.cuda(), None)
+        assert float((y.double() - v * v).abs().max()) <= 3 * 2.0 ** -24
